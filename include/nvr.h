@@ -669,6 +669,70 @@ NVR_API int nvr_fill_weight(nvr_half *dst, int64_t rows, int64_t cols, int64_t l
                             int64_t row0, int64_t col0, uint64_t key, float scale, void *stream);
 NVR_API int nvr_fill_const(nvr_half *dst, int64_t n, float value, void *stream);
 
+/* ------------------------------------ operators around a step of many requests ---- */
+/* Rotary positions, low-rank adapters, tokens from given numbers, and a cache that forgets.  Pointers and types as above: nvr_ops_set_dtype names the type of the nvr_half
+ * tensors, all three included; scores, logits, scales and probabilities are f32.  Argument errors are found before anything is enqueued; what lies on the device (slots,
+ * adapter ids, block tables, lengths) is kept in bounds by the kernels as said below.  A workspace belongs to one call at a time (calls on one stream, or replays of one
+ * graph, may share it), is aligned to 16 bytes, and holds nothing between calls. */
+
+/* How positions are stretched.  NVR_ROPE_PLAIN: freq_j = theta^(-2j/rotary_dim), j < rotary_dim / 2.  LINEAR: freq_j / factor.  NTK: theta * factor^(rotary_dim / (rotary_dim - 2))
+ * in theta's place.  YARN: freq_j (1 - r_j) + freq_j / factor * r_j with r_j rising linearly from the pair that turns `high` times within original_len positions (rounded down) to the one
+ * that turns `low` times (rounded up), amplitude 0.1 ln(factor) + 1 for factors above 1.  BANDS: freq_j where a pair turns `high` times and more within original_len, freq_j / factor where it turns `low`
+ * times or less, in between (1 - s) freq_j / factor + s freq_j with s = (turns - low) / (high - low). */
+typedef enum nvr_rope_scaling_kind { NVR_ROPE_PLAIN = 0, NVR_ROPE_LINEAR = 1, NVR_ROPE_NTK = 2, NVR_ROPE_YARN = 3, NVR_ROPE_BANDS = 4 } nvr_rope_scaling_kind;
+typedef struct nvr_rope_scaling {
+    int32_t kind;
+    double theta, factor;          /* factor: ignored by PLAIN */
+    double original_len;           /* YARN, BANDS: positions of the original context */
+    double low, high;              /* YARN (commonly 1 and 32), BANDS (1 and 4): turns within original_len */
+} nvr_rope_scaling;
+/* turns_dev [rotary_dim / 2] f64: freq_j / (2 pi), the turns that a position makes in pair j; *amplitude: what the rotated numbers are multiplied by */
+NVR_API int nvr_rope_frequencies(const nvr_rope_scaling *sc, int64_t rotary_dim, double *turns_dev, float *amplitude);
+/* Rotates the first rotary_dim columns of every head of q [T, H, D] and k [T, KVH, D] (rows ldq / ldk numbers apart): pairs are columns (j, j + rotary_dim / 2), or (2j, 2j + 1) with
+ * interleaved != 0; the other columns pass through.  q_out / k_out may be q / k themselves (with the same stride).  With caches [num_slots, KVH, D], the k rows (k_out may then be null) and the v
+ * rows [T, KVH, D] are also stored at slot_mapping (a slot outside 0 .. num_slots - 1: not stored; two rows of one slot: either).  Caches, v and slot_mapping may be null together. */
+NVR_API int nvr_rope_rotate_store_kv(const nvr_half *q, int64_t ldq, const nvr_half *k, int64_t ldk, const nvr_half *v, int64_t ldv, const int64_t *positions,
+                                     const int32_t *slot_mapping, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t rotary_dim, int interleaved, const double *turns,
+                                     float amplitude, nvr_half *q_out, int64_t ldqo, nvr_half *k_out, int64_t ldko, nvr_half *k_cache, nvr_half *v_cache, int64_t num_slots,
+                                     void *stream);
+
+/* y[t] = base[t] + scales[a] (x[t] A_a^T) B_a^T with a = adapters[t]: what the adapter of row t's request adds to a shared projection (nvr_linear and its like wrote base; a part of a packed
+ * projection is addressed by its pointer and ldb / ldy).  x [T, K], base and y [T, N] with strides ldx / ldb / ldy, base may be y itself; A [num_adapters, R, K], B [num_adapters, N, R];
+ * scales [num_adapters] f32, null: 1.  A row whose adapters[t] is not in 0 .. num_adapters - 1 has none: y[t] = base[t].  Rows may come in any order; ranks (R) up to 256, fewer than 8192 adapters.
+ * The inner product stays in f32 (16-bit types: two numbers of 16 bits); y is rounded once.  workspace: nvr_lora_workspace_bytes. */
+NVR_API size_t nvr_lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R);
+NVR_API int nvr_lora_add(const nvr_half *x, int64_t ldx, const nvr_half *A, const nvr_half *B, const float *scales, const int32_t *adapters, int64_t num_adapters, int64_t T,
+                         int64_t K, int64_t N, int64_t R, const nvr_half *base, int64_t ldb, nvr_half *y, int64_t ldy, void *workspace, void *stream);
+
+/* A token for each row of logits [B, V] (rows ld numbers apart) from the row's uniform[i] in [0, 1): the filters apply one behind the other to the weights w = exp((x - max) / temperature[i]),
+ * in descending order (ties: ascending index): top_k[i] > 0 keeps the first top_k[i]; 0 <= top_p[i] < 1 keeps the prefix up to the first that brings its sum to top_p[i] of what is left; min_p[i] > 0
+ * keeps weights of min_p[i] (at most 1) and more.  The token is the first in index order whose summed weight exceeds uniform[i] times the sum of all kept.  temperature 0 (or less): the largest logit, lowest
+ * index on ties.  NaN counts as -inf; tokens of weight below e^-42 may be left out; a row of nothing but -inf answers -1.  Any of temperature (1), top_k, top_p, min_p may be null.
+ * out_logprobs (nullable): ln of the token's share of the kept weights (greedy: 0; no token: -inf).  workspace: nvr_sample_uniform_workspace_bytes.  V up to 2^22. */
+NVR_API size_t nvr_sample_uniform_workspace_bytes(int64_t B, int64_t V);
+NVR_API int nvr_sample_uniform(const float *logits, int64_t ld, int64_t B, int64_t V, const float *temperature, const int64_t *top_k, const float *top_p, const float *min_p,
+                               const float *uniform, int64_t *out_ids, float *out_logprobs, void *workspace, void *stream);
+
+/* nvr_paged_attn_decode that also scores the keys: new_scores[key] = decay * scores[key] + the key's softmax weight, summed over the H / KVH query heads of its kv head, for the keys
+ * j < scored_lens[b] of sequence b, and the weight alone for the others (scored_lens null: all but the newest key have a score).  Score pools are [num_blocks, KVH, block_size] f32, addressed by the block
+ * table like the caches [num_blocks, block_size, KVH, D]; new_scores may be scores itself; entries of keys that no sequence of the batch has stay as they are.  Keys whose block is not in
+ * 0 .. num_blocks - 1 are not there; contexts are cut at max_context_len and at max_blocks * block_size; a sequence without keys answers 0.  head_dim 64, 128 or 256, up to 16 query heads a kv head.
+ * The block of a key is one sequence's alone (two sequences that share a block would both write its scores).  workspace: nvr_paged_attn_scored_workspace_bytes (of meta's max_context_len). */
+NVR_API size_t nvr_paged_attn_scored_workspace_bytes(int64_t B, int64_t H, int64_t KVH, int64_t D, int64_t max_context_len);
+NVR_API int nvr_paged_attn_decode_scored(const nvr_half *q, int64_t ldq, const nvr_half *k_cache, const nvr_half *v_cache, const nvr_attn_meta *meta, int64_t H, int64_t KVH,
+                                         int64_t D, int64_t block_size, int64_t num_blocks, float scale, const float *scores, const int32_t *scored_lens, float decay,
+                                         float *new_scores, nvr_half *out, void *workspace, void *stream);
+/* Brings every sequence of more than `budget` keys down to `budget`, each kv head for itself: its first keep_first keys, its last keep_last, and of the others those with the largest scores (ties:
+ * the earlier key; NaN: below all).  The kept keys' rows of K, V and scores close up in their order: in place (to_tables null), or in the blocks of to_tables [B, to_max_blocks], which hold none of the
+ * sequences' own (prompt blocks that other sequences share are left alone that way; shorter sequences are copied as they are).  In place, a block is one sequence's alone.
+ * new_lens [B] (not meta's context_lens) gets the lengths; kept [B, KVH, budget] (nullable) the kept keys' former places, -1 behind the last.  Blocks behind the new length are the caller's to free.
+ * A sequence whose tables name a block outside 0 .. num_blocks - 1 for one of its keys, or whose to_tables row has too few blocks, stays as it is: new_lens -1, kept all -1.
+ * keep_first + keep_last <= budget; rows of a multiple of 16 bytes.  workspace: nvr_kv_evict_workspace_bytes (null allowed where kept is given). */
+NVR_API size_t nvr_kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_context_len);
+NVR_API int nvr_kv_evict(nvr_half *k_cache, nvr_half *v_cache, float *scores, const nvr_attn_meta *meta, int64_t KVH, int64_t D, int64_t block_size, int64_t num_blocks,
+                         int64_t budget, int64_t keep_first, int64_t keep_last, const int32_t *to_tables, int64_t to_max_blocks, int32_t *new_lens, int32_t *kept,
+                         void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

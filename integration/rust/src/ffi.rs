@@ -54,6 +54,11 @@ pub const NVR_ACT_GELU: i32 = 1;
 pub const NVR_ACT_RELU: i32 = 2;
 pub const NVR_ACT_SILU_AND_MUL: i32 = 3;
 pub const NVR_ACT_GELU_AND_MUL: i32 = 4;
+pub const NVR_ROPE_PLAIN: i32 = 0;
+pub const NVR_ROPE_LINEAR: i32 = 1;
+pub const NVR_ROPE_NTK: i32 = 2;
+pub const NVR_ROPE_YARN: i32 = 3;
+pub const NVR_ROPE_BANDS: i32 = 4;
 pub const NVR_TOKENIZE_MAX_CHARS: usize = 100;
 pub const NVR_LM_HEAD_MAX_PARTS: usize = 2048;
 
@@ -212,6 +217,17 @@ pub struct nvr_attn_meta {
     pub max_blocks: i32,
     pub batch: i32,
     pub max_context_len: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct nvr_rope_scaling {
+    pub kind: i32,
+    pub theta: f64,
+    pub factor: f64,
+    pub original_len: f64,
+    pub low: f64,
+    pub high: f64,
 }
 
 #[link(name = "nvr")]
@@ -410,4 +426,14 @@ extern "C" {
     pub fn nvr_weight_scale(std: f64) -> f32;
     pub fn nvr_fill_weight(dst: *mut u16, rows: i64, cols: i64, ld: i64, global_cols: i64, row0: i64, col0: i64, key: u64, scale: f32, stream: *mut c_void) -> c_int;
     pub fn nvr_fill_const(dst: *mut u16, n: i64, value: f32, stream: *mut c_void) -> c_int;
+    pub fn nvr_rope_frequencies(sc: *const nvr_rope_scaling, rotary_dim: i64, turns_dev: *mut f64, amplitude: *mut f32) -> c_int;
+    pub fn nvr_rope_rotate_store_kv(q: *const u16, ldq: i64, k: *const u16, ldk: i64, v: *const u16, ldv: i64, positions: *const i64, slot_mapping: *const i32, T: i64, H: i64, KVH: i64, D: i64, rotary_dim: i64, interleaved: c_int, turns: *const f64, amplitude: f32, q_out: *mut u16, ldqo: i64, k_out: *mut u16, ldko: i64, k_cache: *mut u16, v_cache: *mut u16, num_slots: i64, stream: *mut c_void) -> c_int;
+    pub fn nvr_lora_workspace_bytes(T: i64, K: i64, N: i64, R: i64) -> usize;
+    pub fn nvr_lora_add(x: *const u16, ldx: i64, A: *const u16, B: *const u16, scales: *const f32, adapters: *const i32, num_adapters: i64, T: i64, K: i64, N: i64, R: i64, base: *const u16, ldb: i64, y: *mut u16, ldy: i64, workspace: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn nvr_sample_uniform_workspace_bytes(B: i64, V: i64) -> usize;
+    pub fn nvr_sample_uniform(logits: *const f32, ld: i64, B: i64, V: i64, temperature: *const f32, top_k: *const i64, top_p: *const f32, min_p: *const f32, uniform: *const f32, out_ids: *mut i64, out_logprobs: *mut f32, workspace: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn nvr_paged_attn_scored_workspace_bytes(B: i64, H: i64, KVH: i64, D: i64, max_context_len: i64) -> usize;
+    pub fn nvr_paged_attn_decode_scored(q: *const u16, ldq: i64, k_cache: *const u16, v_cache: *const u16, meta: *const nvr_attn_meta, H: i64, KVH: i64, D: i64, block_size: i64, num_blocks: i64, scale: f32, scores: *const f32, scored_lens: *const i32, decay: f32, new_scores: *mut f32, out: *mut u16, workspace: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn nvr_kv_evict_workspace_bytes(B: i64, KVH: i64, budget: i64, max_context_len: i64) -> usize;
+    pub fn nvr_kv_evict(k_cache: *mut u16, v_cache: *mut u16, scores: *mut f32, meta: *const nvr_attn_meta, KVH: i64, D: i64, block_size: i64, num_blocks: i64, budget: i64, keep_first: i64, keep_last: i64, to_tables: *const i32, to_max_blocks: i64, new_lens: *mut i32, kept: *mut i32, workspace: *mut c_void, stream: *mut c_void) -> c_int;
 }

@@ -115,6 +115,10 @@ class AttnMetaC(C.Structure):
                 ("batch", C.c_int32), ("max_context_len", C.c_int32)]
 
 
+class RopeScalingC(C.Structure):                             # nvr_rope_scaling
+    _fields_ = [("kind", C.c_int32), ("theta", C.c_double), ("factor", C.c_double), ("original_len", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
 _lib: Optional[C.CDLL] = None
 _P = C.c_void_p
 _SIGS = {
@@ -261,6 +265,18 @@ _SIGS = {
     "nvr_fill_weight": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_uint64,
                                   C.c_float, _P]),
     "nvr_fill_const": (C.c_int, [_P, C.c_int64, C.c_float, _P]),
+    "nvr_rope_frequencies": (C.c_int, [C.POINTER(RopeScalingC), C.c_int64, _P, C.POINTER(C.c_float)]),
+    "nvr_rope_rotate_store_kv": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int, _P, C.c_float,
+                                           _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, _P]),
+    "nvr_lora_workspace_bytes": (C.c_size_t, [C.c_int64] * 4),
+    "nvr_lora_add": (C.c_int, [_P, C.c_int64, _P, _P, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P]),
+    "nvr_sample_uniform_workspace_bytes": (C.c_size_t, [C.c_int64] * 2),
+    "nvr_sample_uniform": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "nvr_paged_attn_scored_workspace_bytes": (C.c_size_t, [C.c_int64] * 5),
+    "nvr_paged_attn_decode_scored": (C.c_int, [_P, C.c_int64, _P, _P, C.POINTER(AttnMetaC), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float, _P, _P, C.c_float,
+                                               _P, _P, _P, _P]),
+    "nvr_kv_evict_workspace_bytes": (C.c_size_t, [C.c_int64] * 4),
+    "nvr_kv_evict": (C.c_int, [_P, _P, _P, C.POINTER(AttnMetaC), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, _P, _P, _P, _P]),
     "nvr_ops_set_dtype": (C.c_int, [C.c_char_p]), "nvr_ops_dtype": (C.c_char_p, []),
 }
 

@@ -1,0 +1,229 @@
+// kv_evict.hip — a sequence's cache brought down to `budget` keys a kv head: its first and last keys, and the best of the others by their scores (ties: the earlier key), close up in their order.
+//
+// First launch, a workgroup a (sequence, kv head): the score that the last of the kept keys has, by a radix select over the scores (held in LDS up to kHeld of them), then the kept keys in
+// order (each thread owns a run of keys; one scan tells where its kept ones go) and the scores at their new places.  Second launch: the rows of K and V.
+// Into other blocks, every row is on its own: a copy, bound by memory.  In place, row i comes from row kept[i] >= i, which is overwritten by a later row: a workgroup takes a (sequence, kv head)'s
+// strip of 128 bytes of the rows, from the front in steps of kStep rows: all of a step are read before any is written, and no later step reads what it writes.
+#include <algorithm>
+#include "serving.h"
+#include "elem.h"
+#include "../common.h"
+
+namespace nvr { namespace kx {
+
+namespace {
+constexpr int kPick = 1024, kHeld = 10240, kRadix = 2048;
+struct EvictParams {
+    EvictArgs a;
+    int32_t *kept;                                                        // [B][KVH][budget]
+    int32_t row_bytes, strip, rows;                                       // of a key's row of a head; bytes of it that a workgroup moves; rows of a step
+};
+__device__ __forceinline__ int length_of(const EvictArgs &a, int b) {
+    const long long most = (long long)a.max_blocks * a.block_size;
+    return (int)max(0ll, min((long long)min(a.ctx_lens[b], a.max_ctx), most));
+}
+__device__ __forceinline__ int row_in(const int32_t *table, int block_size, int j) {
+    const int block = (int)((unsigned)j / (unsigned)block_size);
+    return table[block] * block_size + (j - block * block_size);
+}
+__device__ __forceinline__ int64_t score_at(const EvictArgs &a, const int32_t *table, int g, int j) {
+    const int block = (int)((unsigned)j / (unsigned)a.block_size);
+    return ((int64_t)table[block] * a.KVH + g) * a.block_size + (j - block * a.block_size);
+}
+// larger score, larger number; not a number: below all
+__device__ __forceinline__ unsigned int rank_of(float f) {
+    if (!(f == f)) return 0u;
+    const unsigned int u = __float_as_uint(f + 0.f);                      // (-0 is 0)
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+}  // namespace
+
+__global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
+    __shared__ unsigned int held[kHeld], hist[kRadix];
+    __shared__ unsigned int waves[16];
+    __shared__ unsigned long long waves2[16];
+    __shared__ int found;
+    __shared__ unsigned int above;
+    const EvictArgs &a = p.a;
+    const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int len = length_of(a, b), n = min(len, a.budget);
+    const int32_t *table = a.block_tables + (int64_t)b * a.max_blocks, *to = a.to_tables ? a.to_tables + (int64_t)b * a.to_max_blocks : table;
+    int32_t *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
+    // a sequence whose tables name a block outside the pool, or too few, stays as it is
+    int bad = a.to_tables && (long long)a.to_max_blocks * a.block_size < n;
+    for (int i = tid; i < (len + a.block_size - 1) / a.block_size; i += kPick) bad |= table[i] < 0 || table[i] >= a.num_blocks;
+    if (a.to_tables && !bad)
+        for (int i = tid; i < (n + a.block_size - 1) / a.block_size; i += kPick) bad |= to[i] < 0 || to[i] >= a.num_blocks;
+    if (__syncthreads_or(bad)) {
+        if (g == 0 && tid == 0) a.new_lens[b] = -1;
+        for (int i = tid; i < a.budget; i += kPick) kept[i] = -1;
+        return;
+    }
+    if (g == 0 && tid == 0) a.new_lens[b] = n;
+    for (int i = n + tid; i < a.budget; i += kPick) kept[i] = -1;
+    if (len <= a.budget) {
+        for (int i = tid; i < n; i += kPick) kept[i] = i;
+    } else {
+        const int first = a.first, end = len - a.last, count = end - first;        // the keys that compete
+        unsigned int need = a.budget - a.first - a.last;                  // < count
+        auto load = [&](int i) { return rank_of(a.scores[score_at(a, table, g, first + i)]); };
+        for (int i = tid; i < min(count, kHeld); i += kPick) held[i] = load(i);
+        auto rank = [&](int i) { return i < kHeld ? held[i] : load(i); };
+        unsigned int prefix = 0, mask = 0, want = need;
+        if (need) {
+            for (int pass = 0; pass < 3; ++pass) {
+                const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
+                for (int i = tid; i < kRadix; i += kPick) hist[i] = 0;
+                if (tid == 0) found = kRadix;
+                __syncthreads();
+                for (int i = tid; i < count; i += kPick) { const unsigned int k = rank(i); if ((k & mask) == prefix) atomicAdd(&hist[wide - 1 - ((k >> at) & (wide - 1))], 1u); }
+                __syncthreads();
+                const unsigned int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+                unsigned int v = c0 + c1;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) { const unsigned int o = __shfl_up(v, d); if (lane >= d) v += o; }
+                if (lane == 63) waves[wave] = v;
+                __syncthreads();
+                for (int w = 0; w < wave; ++w) v += waves[w];
+                if (c0 && v - c1 >= want) atomicMin(&found, 2 * tid);
+                else if (c1 && v >= want) atomicMin(&found, 2 * tid + 1);
+                __syncthreads();
+                if (tid == found / 2) above = (found & 1) ? v - c1 : v - c1 - c0;
+                __syncthreads();
+                prefix |= (unsigned int)(wide - 1 - found) << at; mask |= (unsigned int)(wide - 1) << at;
+                want -= above;
+                __syncthreads();
+            }
+        } else { prefix = 0xffffffffu; __syncthreads(); }
+        // want of the keys with rank `prefix`, the earliest, and all above it.  A thread's run of keys: its counts of both, and where they begin
+        const int per = (count + kPick - 1) / kPick, i0 = min(count, tid * per), i1 = min(count, i0 + per);
+        unsigned int more = 0, same = 0;
+        for (int i = i0; i < i1; ++i) { const unsigned int k = rank(i); more += need && k > prefix; same += need && k == prefix; }
+        unsigned long long v = ((unsigned long long)more << 32) | same;
+        const unsigned long long own = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const unsigned long long o = __shfl_up(v, d); if (lane >= d) v += o; }
+        if (lane == 63) waves2[wave] = v;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) v += waves2[w];
+        v -= own;
+        unsigned int seen = (unsigned int)v, at = first + (unsigned int)(v >> 32) + min(seen, want);
+        for (int i = i0; i < i1; ++i) {
+            const unsigned int k = rank(i);
+            const bool tie = need && k == prefix;
+            if ((need && k > prefix) || (tie && seen < want)) kept[at++] = first + i;
+            seen += tie;
+        }
+        for (int i = tid; i < a.first; i += kPick) kept[i] = i;
+        for (int i = tid; i < a.last; i += kPick) kept[a.budget - a.last + i] = end + i;
+    }
+    if (!a.to_tables && len <= a.budget) return;
+    __threadfence_block();
+    __syncthreads();
+    // the scores, from the front: of a step all are read before any is written
+    for (int i0 = 0; i0 < n; i0 += kPick) {
+        const int i = i0 + tid;
+        float s = 0.f;
+        if (i < n) s = a.scores[score_at(a, table, g, kept[i])];
+        asm volatile("" : "+v"(s));
+        __syncthreads();
+        if (i < n) a.scores[score_at(a, to, g, i)] = s;
+    }
+}
+
+// 16 bytes a lane, `strip` bytes of a row; the step in front of the next one's writes is on its way
+constexpr int kMoves = 4;
+__global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
+    const EvictArgs &a = p.a;
+    const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int len = length_of(a, b);
+    if (len <= a.budget || a.new_lens[b] < 0) return;
+    const int n = a.budget, strips = p.row_bytes / p.strip, which = blockIdx.x;
+    char *pool = (char *)(which < strips ? a.k : a.v);
+    const int32_t *table = a.block_tables + (int64_t)b * a.max_blocks, *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
+    const int lanes = p.strip / 16, piece = tid % lanes, lead = tid / lanes, rows = kPick / lanes;    // rows of a request
+    const int64_t row = (int64_t)a.KVH * p.row_bytes, off = (int64_t)g * p.row_bytes + (which % strips) * p.strip + piece * 16;
+    float4_t v[kMoves];
+    auto request = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kMoves; ++u) {
+            const int i = i0 + u * rows + lead;
+            if (lead < rows && i < n) { const int j = kept[i]; if (j != i) v[u] = *reinterpret_cast<const float4_t *>(pool + row_in(table, a.block_size, j) * row + off); }
+        }
+    };
+    request(0);
+    for (int i0 = 0; i0 < n; i0 += kMoves * rows) {
+        float4_t w[kMoves];
+#pragma unroll
+        for (int u = 0; u < kMoves; ++u) { w[u] = v[u]; asm volatile("" : "+v"(w[u])); }      // (here: what this step reads has arrived)
+        __syncthreads();
+        if (i0 + kMoves * rows < n) request(i0 + kMoves * rows);
+#pragma unroll
+        for (int u = 0; u < kMoves; ++u) {
+            const int i = i0 + u * rows + lead;
+            if (lead < rows && i < n && kept[i] != i) *reinterpret_cast<float4_t *>(pool + row_in(table, a.block_size, i) * row + off) = w[u];
+        }
+    }
+}
+
+// Into other blocks: a lane 16 bytes of K and of V, kMoves rows on their way
+__global__ __launch_bounds__(256) void kv_evict_copy_kernel(EvictParams p) {
+    const EvictArgs &a = p.a;
+    const int g = blockIdx.y, b = blockIdx.z;
+    const int n = a.new_lens[b];
+    const int lanes = p.row_bytes / 16, rows = 256 / lanes, i0 = blockIdx.x * rows * kMoves, lead = threadIdx.x / lanes, piece = threadIdx.x % lanes;
+    if (i0 >= n || lead >= rows) return;
+    const int32_t *table = a.block_tables + (int64_t)b * a.max_blocks, *to = a.to_tables + (int64_t)b * a.to_max_blocks, *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
+    const int64_t row = (int64_t)a.KVH * p.row_bytes, off = (int64_t)g * p.row_bytes + piece * 16;
+    float4_t k[kMoves], v[kMoves];
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u) {
+        const int i = min(i0 + u * rows + lead, n - 1);
+        const int64_t at = row_in(table, a.block_size, kept[i]) * row + off;
+        k[u] = *reinterpret_cast<const float4_t *>((const char *)a.k + at);
+        v[u] = *reinterpret_cast<const float4_t *>((const char *)a.v + at);
+    }
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u) {
+        const int i = i0 + u * rows + lead;
+        if (i >= n) break;
+        const int64_t at = row_in(to, a.block_size, i) * row + off;
+        *reinterpret_cast<float4_t *>((char *)a.k + at) = k[u];
+        *reinterpret_cast<float4_t *>((char *)a.v + at) = v[u];
+    }
+}
+
+size_t kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_ctx) {
+    (void)max_ctx;
+    return B <= 0 || KVH <= 0 || budget <= 0 ? 0 : (size_t)(B * KVH * budget * 4);
+}
+int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
+    const char *me = "nvr_kv_evict";
+    if (a.B < 0 || a.KVH <= 0 || a.D <= 0 || a.block_size <= 0 || a.max_blocks < 0 || a.num_blocks < 0 || a.max_ctx < 0 || a.to_max_blocks < 0)
+        return nvr::fail(NVR_ERR_INVALID_ARG, "%s: batch %d, %d kv heads of %d, blocks of %d", me, a.B, a.KVH, a.D, a.block_size);
+    if (a.budget <= 0 || a.first < 0 || a.last < 0 || (int64_t)a.first + a.last > a.budget)
+        return nvr::fail(NVR_ERR_INVALID_ARG, "%s: a budget of %d keys with the first %d and the last %d", me, a.budget, a.first, a.last);
+    const int64_t bytes = (int64_t)a.D * (dt == DT_F32 ? 4 : 2);
+    if (bytes % 16 || bytes > 1024) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: rows of %ld bytes a head (multiples of 16 up to 1024)", me, (long)bytes);
+    if (a.num_blocks * a.block_size > 0x7fffffffll || a.B > 65535 || a.KVH > 65535) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: a pool of 2^31 rows and more, or more than 65535 sequences", me);
+    if (a.B == 0) return 0;
+    if (!a.k || !a.v || !a.scores || !a.ctx_lens || !a.block_tables || !a.new_lens || (!a.kept && !a.workspace)) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: null argument", me);
+    if (a.new_lens == a.ctx_lens) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: new_lens is the context_lens that other workgroups still read", me);
+    if (a.to_tables == a.block_tables) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: in place is asked for with to_tables null", me);
+    if ((((uintptr_t)a.k | (uintptr_t)a.v) & 15) != 0) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: the caches have to be aligned to 16 bytes", me);
+    EvictParams p{};
+    p.a = a;
+    p.kept = a.kept ? a.kept : (int32_t *)a.workspace;
+    p.row_bytes = (int32_t)bytes;
+    p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
+    const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
+    kv_evict_select_kernel<<<dim3(G, B), kPick, 0, s>>>(p);
+    if (a.to_tables) {
+        const int rows = 256 / (p.row_bytes / 16) * kMoves, most = std::min(a.budget, a.max_ctx);
+        if (most > 0) kv_evict_copy_kernel<<<dim3((unsigned)((most + rows - 1) / rows), G, B), 256, 0, s>>>(p);
+    } else if (a.max_ctx > a.budget) kv_evict_close_kernel<<<dim3((unsigned)(2 * (p.row_bytes / p.strip)), G, B), kPick, 0, s>>>(p);
+    NVR_KX_LAUNCHED("kv_evict");
+    return 0;
+}
+
+}}  // namespace nvr::kx

@@ -1,0 +1,387 @@
+// lora.hip — low-rank adapters of many requests beside a shared projection: y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T, a = the adapter of row t's request.
+//
+// Two products of inner sizes K and R, on the matrix cores, over TILES: up to 16 or 64 rows that share an adapter, wherever they stand in the step (up to 256 rows every workgroup finds its tile
+// itself; more are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
+//   down: v = scale x A^T, the waves of a workgroup (and `splits` workgroups of few rows) share K; partial sums stay in 32 bits in the workspace, [split][row][rank]
+//   up:   y = base + v B^T; v in two 16-bit numbers (its rounding and the rounded rest), so that the product sees it in 16 (bfloat16) or 22 bits; the sum with base is rounded once
+// Both are bound by memory for prompts (x, base and y once; 2 R flops a byte) and by their two launches for decode steps.
+#include <algorithm>
+#include "serving.h"
+#include "elem.h"
+#include "../common.h"
+
+namespace nvr { namespace kx {
+
+namespace {
+constexpr int kSmall = 256;                                               // rows up to which a workgroup finds its tile itself
+constexpr int kMaxAdapters = 8192;                                        // counters of the grouping launch (LDS)
+
+struct LoraTile { int32_t start, count, adapter; };                       // rows order[start ..) of one adapter; adapter n: rows without one
+struct LoraParams {
+    LoraArgs a;
+    int32_t splits, rp, copies;                                           // copies: rows without an adapter are tiles too (base is another tensor)
+    const int32_t *order; const LoraTile *tiles; const int32_t *num_tiles;
+    float *v;                                                             // [splits][T][rp]
+    bool xw, aw, bw, yw;                                                  // whole 16-byte pieces of x, A, B and base / y
+};
+
+__device__ __forceinline__ int adapter_of(const LoraParams &p, int64_t t) {
+    const int id = p.a.ids[t];
+    return id >= 0 && id < (int)p.a.n ? id : p.copies ? (int)p.a.n : -1;
+}
+
+// float16: v may be beyond its range, or far below it, so each row of v is multiplied by the power of two that brings its largest number to 2^13 .. 2^14 (exponents of -100 .. 100)
+__device__ __forceinline__ int range_of(unsigned int most) {
+    const int e = (int)(most >> 23) - 127;
+    return most == 0 || e == 128 ? 0 : min(max(13 - e, -100), 100);
+}
+
+// rows of tile `tile` (rows[0 .. count), LDS) and its adapter; count 0: no such tile.  256 threads, T <= 256, tiles of 16 rows: row t is number rank(t) of its adapter's rows, the rows of rank 0, 16,
+// .. lead a tile, tiles go by their leaders.
+__device__ __forceinline__ int tile_of_small(const LoraParams &p, int tile, int *rows, int *ids, int *note, int &adapter) {
+    const int t = threadIdx.x, T = (int)p.a.T;
+    const int id = t < T ? adapter_of(p, t) : -1;
+    ids[t] = id;
+    if (t < 2) note[t] = 0;
+    __syncthreads();
+    int rank = 0;
+    const int4 *v = reinterpret_cast<const int4 *>(ids);
+    for (int j = 0; j < (T + 3) / 4; ++j) {
+        const int4 o = v[j];
+        rank += (o.x == id && 4 * j < t) + (o.y == id && 4 * j + 1 < t) + (o.z == id && 4 * j + 2 < t) + (o.w == id && 4 * j + 3 < t);
+    }
+    const bool lead = id >= 0 && (rank & 15) == 0;
+    const unsigned long long b = __ballot(lead);
+    int *per_wave = note + 4;
+    if ((t & 63) == 0) per_wave[t >> 6] = __popcll(b);
+    __syncthreads();
+    int before = __popcll(b & ((1ull << (t & 63)) - 1));
+    for (int w = 0; w < t >> 6; ++w) before += per_wave[w];
+    if (lead && before == tile) { note[0] = 1; note[2] = id; note[3] = rank; }
+    __syncthreads();
+    if (!note[0]) return 0;
+    adapter = note[2];
+    const int first = note[3];
+    if (id == adapter && rank >= first && rank < first + 16) { rows[rank - first] = t; atomicAdd(&note[1], 1); }
+    __syncthreads();
+    return note[1];
+}
+template <int TR, bool GROUPED>
+__device__ __forceinline__ int tile_rows(const LoraParams &p, int tile, int *rows, int *ids, int *note, int &adapter) {
+    if constexpr (!GROUPED) return tile_of_small(p, tile, rows, ids, note, adapter);
+    if (tile >= *p.num_tiles) return 0;
+    const LoraTile d = p.tiles[tile];
+    adapter = d.adapter;
+    if (threadIdx.x < d.count) rows[threadIdx.x] = p.order[d.start + threadIdx.x];
+    __syncthreads();
+    return d.count;
+}
+}  // namespace
+
+// The rows of more than 256, adapter by adapter (their order inside one is of no consequence: a row's sums are its own), and the tiles they make.
+__global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p, int tr, int32_t *order, LoraTile *tiles, int32_t *num_tiles) {
+    extern __shared__ int32_t count[];                                    // [n + 1] rows of an adapter, then where its next row goes
+    __shared__ int32_t sum_rows[16], sum_tiles[16], base_rows, base_tiles;
+    const int n = (int)p.a.n + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < n; i += 1024) count[i] = 0;
+    if (tid == 0) base_rows = base_tiles = 0;
+    __syncthreads();
+    auto add = [&](int id) {                                              // (returns the row's place; lanes of the first lane's adapter add together: a prompt's rows are all of one)
+        int at = 0;
+        const unsigned long long have = __ballot(id >= 0);
+        if (!have) return at;
+        const int first = __ffsll((long long)have) - 1, lead = __shfl(id, first);
+        const unsigned long long same = __ballot(id == lead);
+        int start = 0;
+        if (lane == first) start = atomicAdd(&count[lead], __popcll(same));
+        start = __shfl(start, first);
+        if (id == lead) at = start + __popcll(same & ((1ull << lane) - 1));
+        else if (id >= 0) at = atomicAdd(&count[id], 1);
+        return at;
+    };
+    const int64_t T = p.a.T;
+    for (int64_t c = 0; c < T; c += 1024) add(c + tid < T ? adapter_of(p, c + tid) : -1);
+    __syncthreads();
+    for (int c = 0; c < n; c += 1024) {                                   // exclusive sums of rows and tiles over the adapters
+        const int i = c + tid, rows = i < n ? count[i] : 0, mine = (rows + tr - 1) / tr;
+        int r = rows, t = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int ur = __shfl_up(r, d), ut = __shfl_up(t, d);
+            if (lane >= d) { r += ur; t += ut; }
+        }
+        if (lane == 63) { sum_rows[wave] = r; sum_tiles[wave] = t; }
+        __syncthreads();
+        int r0 = base_rows, t0 = base_tiles;
+        for (int w = 0; w < wave; ++w) { r0 += sum_rows[w]; t0 += sum_tiles[w]; }
+        __syncthreads();
+        if (tid == 1023) { base_rows = r0 + r; base_tiles = t0 + t; }
+        r0 += r - rows; t0 += t - mine;
+        if (i < n) {
+            count[i] = r0;
+            for (int k = 0; k < mine; ++k) tiles[t0 + k] = LoraTile{r0 + k * tr, min(tr, rows - k * tr), i};
+        }
+        __syncthreads();
+    }
+    if (tid == 0) *num_tiles = base_tiles;
+    for (int64_t c = 0; c < T; c += 1024) {
+        const int id = c + tid < T ? adapter_of(p, c + tid) : -1;
+        const int at = add(id);
+        if (id >= 0) order[at] = (int32_t)(c + tid);
+    }
+}
+
+// D(rank x row) = A . x^T: a lane's 4 sums are neighbours in v.  The waves take the steps of KS columns in turn; U steps are requested together.
+template <class E, int MT, int RT, bool GROUPED>
+__global__ __launch_bounds__(256) void lora_down_kernel(LoraParams p) {
+    typedef typename E::T T; typedef typename E::V V;
+    constexpr int TR = MT * 16, U = MT == 1 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) int ids[GROUPED ? 4 : kSmall];
+    __shared__ int rows[TR], note[8];
+    __shared__ float4_t part[2][MT * RT][64];
+    int adapter = -1;
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, ids, note, adapter);
+    if (!count || adapter >= (int)p.a.n) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
+    const int K = (int)p.a.K, R = (int)p.a.R, r0 = blockIdx.z * RT * 16;
+    const int steps = (K + E::KS - 1) / E::KS, per = (steps + p.splits - 1) / p.splits, first = blockIdx.y * per, last = min(steps, first + per);
+    const T *x[MT], *w[RT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) { const int t = m * 16 + lm; x[m] = (const T *)p.a.x + (int64_t)rows[t < count ? t : 0] * p.a.ldx; }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) w[r] = (const T *)p.a.A + ((int64_t)adapter * R + min(r0 + r * 16 + lm, R - 1)) * K;
+    float4_t acc[MT][RT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[m][r] = (float4_t){0.f, 0.f, 0.f, 0.f};
+    int s = first + wave;
+    if (p.xw && p.aw)                                                     // whole steps: requests without a test
+        for (const int whole = min(last, K / E::KS); s + 4 * (U - 1) < whole; s += 4 * U) {
+            V xv[U][MT], wv[U][RT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = (s + 4 * u) * E::KS + lq * E::W;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) xv[u][m] = *reinterpret_cast<const V *>(x[m] + k);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wv[u][r] = *reinterpret_cast<const V *>(w[r] + k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[m][r] = E::mma(wv[u][r], xv[u][m], acc[m][r]);
+        }
+    for (; s < last; s += 4) {
+        const int k = s * E::KS + lq * E::W, n = K - k;                   // numbers of the row from k on (0 or fewer: this lane's part is behind the row)
+        V xv[MT], wv[RT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xv[m] = n > 0 ? load16<E>(x[m] + k, p.xw, n) : zero16<E>();
+#pragma unroll
+        for (int r = 0; r < RT; ++r) wv[r] = n > 0 ? load16<E>(w[r] + k, p.aw, n) : zero16<E>();
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[m][r] = E::mma(wv[r], xv[m], acc[m][r]);
+    }
+    // the waves' sums in a fixed order: (0 + 2) + (1 + 3)
+    if (wave >= 2)
+#pragma unroll
+        for (int i = 0; i < MT * RT; ++i) part[wave - 2][i][lane] = acc[i / RT][i % RT];
+    __syncthreads();
+    if (wave < 2)
+#pragma unroll
+        for (int i = 0; i < MT * RT; ++i) part[wave][i][lane] = acc[i / RT][i % RT] + part[wave][i][lane];
+    __syncthreads();
+    const float scale = p.a.scales ? p.a.scales[adapter] : 1.f;
+    for (int i = wave; i < MT * RT; i += 4) {
+        const int m = i / RT, r = i % RT, t = m * 16 + lm;
+        const float4_t v = part[0][i][lane] + part[1][i][lane];
+        if (t < count && r0 + r * 16 < p.rp) *reinterpret_cast<float4_t *>(p.v + ((int64_t)blockIdx.y * p.a.T + rows[t]) * p.rp + r0 + r * 16 + lq * 4) = v * scale;
+    }
+}
+
+// D(column x row) = B . v^T: a lane's NT * 4 = W sums are neighbours in y (row m of tile i of B is column (m / 4) W + 4 i + m % 4 of the group).  A wave takes groups of NT * 16 columns.
+template <class E, int MT, bool GROUPED>
+__global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p, int groups) {
+    typedef typename E::T T; typedef typename E::V V;
+    constexpr int TR = MT * 16, W = E::W, NT = W / 4, GN = NT * 16;
+    constexpr bool F = sizeof(T) == 4;
+    constexpr bool H = __is_same(E, F16);
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // v: [hi, lo] [TR][ldv]; 32 bits: [TR][ldv]
+    __shared__ unsigned int high[TR];                                     // float16: bits of a row's largest |v|
+    __shared__ __attribute__((aligned(16))) int ids[GROUPED ? 4 : kSmall];
+    __shared__ int rows[TR], note[8];
+    int adapter = -1;
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, ids, note, adapter);
+    if (!count) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
+    const int R = (int)p.a.R, N = (int)p.a.N, ks = (R + E::KS - 1) / E::KS, ldv = ks * E::KS + W;    // (a row's stride is 16 bytes off a multiple of 64: neighbours lie in other banks)
+    const bool real = adapter < (int)p.a.n;
+    T *hi = reinterpret_cast<T *>(smem), *lo = hi + TR * ldv;
+    if (real) {
+        const int per = ks * E::KS / 4;                                   // pieces of 4 sums; a thread has up to 8 (64 rows of rank 128, 16 of rank 256)
+        float4_t v[8];
+        if (H && threadIdx.x < TR) high[threadIdx.x] = 0;
+        if (H) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
+            v[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            if (i < TR * per && t < count && r < p.rp) {
+                const float *at = p.v + (int64_t)rows[t] * p.rp + r;
+                for (int s = 0; s < p.splits; ++s, at += p.a.T * p.rp) v[n] += *reinterpret_cast<const float4_t *>(at);
+            }
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (r + e >= R) v[n][e] = 0.f;                            // (behind R there are repeats of the last row of A)
+                most = fmaxf(most, fabsf(v[n][e]));
+            }
+            if (H && i < TR * per) atomicMax(&high[t], __float_as_uint(most));
+        }
+        if (H) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
+            if (i >= TR * per) break;
+            const float f = H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = v[n][e] * f;
+                const T h = (T)x;
+                hi[t * ldv + r + e] = h;
+                if constexpr (!F) lo[t * ldv + r + e] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
+            }
+        }
+    }
+    __syncthreads();
+    const int64_t at0 = (int64_t)lq * W;
+    int64_t row[MT];
+    float back[MT];                                                       // what undoes the row's range
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int t = m * 16 + lm;
+        row[m] = rows[t < count ? t : 0];
+        back[m] = H && real ? __uint_as_float((unsigned)(127 - range_of(high[t])) << 23) : 1.f;
+    }
+    const T *B = (const T *)p.a.B + (int64_t)adapter * N * R;
+    for (int g = (blockIdx.x * 4 + wave) * groups, end = g + groups; g < end; ++g) {
+        const int64_t n0 = (int64_t)g * GN;
+        if (n0 >= N) return;
+        const int left = (int)min((int64_t)W, N - n0 - at0);              // columns of this lane that there are
+        V b[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) b[m] = left > 0 ? load16<E>((const T *)p.a.base + row[m] * p.a.ldb + n0 + at0, p.yw, left) : zero16<E>();
+        float4_t acc[NT][MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[i][m] = (float4_t){0.f, 0.f, 0.f, 0.f};
+        if (real) {
+            const T *bp[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) bp[i] = B + min(n0 + (lm >> 2) * W + 4 * i + (lm & 3), (int64_t)N - 1) * R;
+            for (int k = 0; k < ks; ++k) {
+                const int r = k * E::KS + lq * W, n = R - r;
+                V bv[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) bv[i] = n >= W && p.bw ? *reinterpret_cast<const V *>(bp[i] + r) : n > 0 ? load16<E>(bp[i] + r, false, n) : zero16<E>();
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const V vh = *reinterpret_cast<const V *>(hi + (m * 16 + lm) * ldv + r);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) acc[i][m] = E::mma(bv[i], vh, acc[i][m]);
+                    if constexpr (!F) {
+                        const V vl = *reinterpret_cast<const V *>(lo + (m * 16 + lm) * ldv + r);
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) acc[i][m] = E::mma(bv[i], vl, acc[i][m]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m * 16 + lm >= count || left <= 0) continue;
+            V o;
+#pragma unroll
+            for (int e = 0; e < W; ++e) o[e] = real ? (T)(H ? fmaf(acc[e / 4][m][e % 4], back[m], (float)b[m][e]) : (float)b[m][e] + acc[e / 4][m][e % 4]) : b[m][e];
+            T *y = (T *)p.a.y + row[m] * p.a.ldy + n0 + at0;
+            if (left == W && p.yw) *reinterpret_cast<V *>(y) = o;
+            else
+#pragma unroll
+                for (int e = 0; e < W; ++e) if (e < left) y[e] = o[e];
+        }
+    }
+}
+
+static int lora_splits_most(int64_t T, int64_t K) {                       // (a wave has two steps at least; the sums of many rows are long enough without)
+    const int64_t steps = (K + 31) / 32;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(T <= kSmall ? 16 : 4, steps / 8));
+}
+static int64_t lora_rp(int64_t R) { return (R + 15) / 16 * 16; }
+size_t lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R) {
+    (void)N;
+    if (T <= 0 || K <= 0 || R <= 0) return 0;
+    return (size_t)T * lora_splits_most(T, K) * lora_rp(R) * 4 + (T > kSmall ? ((size_t)T * (4 + sizeof(LoraTile)) + 64) : 0);
+}
+
+template <class E, int MT, bool GROUPED>
+static void lora_launch(const LoraParams &p, int64_t tiles, hipStream_t s) {
+    const int rt = (int)(p.rp / 16);
+    const unsigned t = (unsigned)tiles, z = (unsigned)p.splits;
+    if (rt == 1) lora_down_kernel<E, MT, 1, GROUPED><<<dim3(t, z, 1), 256, 0, s>>>(p);
+    else if (rt == 2) lora_down_kernel<E, MT, 2, GROUPED><<<dim3(t, z, 1), 256, 0, s>>>(p);
+    else lora_down_kernel<E, MT, 4, GROUPED><<<dim3(t, z, (rt + 3) / 4), 256, 0, s>>>(p);
+    constexpr int GN = E::W / 4 * 16;
+    const int64_t all = (p.a.N + GN - 1) / GN;                            // groups of columns: a wave takes 1 to 4, as long as there are workgroups for two rounds of the chip
+    int groups = 4;
+    while (groups > 1 && (all + 4 * groups - 1) / (4 * groups) * tiles < 512) groups /= 2;
+    const int ldv = (int)((p.a.R + E::KS - 1) / E::KS * E::KS + E::W);
+    lora_up_kernel<E, MT, GROUPED><<<dim3((unsigned)((all + 4 * groups - 1) / (4 * groups)), t), 256, (size_t)MT * 16 * ldv * 4, s>>>(p, groups);
+}
+
+template <class E>
+static int lora_of(const LoraArgs &a, hipStream_t s) {
+    LoraParams p{};
+    p.a = a;
+    p.copies = a.base != a.y;
+    p.rp = (int)lora_rp(a.R);
+    auto whole = [](const void *q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && ld % E::W == 0; };
+    p.xw = whole(a.x, a.ldx); p.aw = whole(a.A, a.K); p.bw = whole(a.B, a.R); p.yw = whole(a.y, a.ldy) && whole(a.base, a.ldb);
+    // the tiles there can be: full ones, and one begun per adapter (rows without one count as one); 64 rows where the adapters have as many, else 16
+    const int64_t kinds = std::min<int64_t>(a.n + p.copies, a.T);
+    const int tr = a.T > kSmall && a.T >= 32 * kinds && a.R <= 128 ? 64 : 16;   // (up: 64 rows of v in LDS, 34 KB at rank 128)
+    const int64_t tiles = std::min<int64_t>(a.T, a.T / tr + kinds);
+    const int64_t zs = (p.rp / 16 + 3) / 4;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(lora_splits_most(a.T, a.K), (512 + tiles * zs - 1) / (tiles * zs)));
+    p.v = (float *)a.workspace;
+    if (a.T > kSmall) {
+        char *at = (char *)a.workspace + (size_t)a.T * lora_splits_most(a.T, a.K) * p.rp * 4;
+        LoraTile *td = (LoraTile *)at;
+        int32_t *order = (int32_t *)(at + (size_t)a.T * sizeof(LoraTile)), *nt = order + a.T;
+        p.tiles = td; p.order = order; p.num_tiles = nt;
+        lora_group_kernel<<<dim3(1), dim3(1024), (size_t)(a.n + 1) * 4, s>>>(p, tr, order, td, nt);
+        if (tr == 64) lora_launch<E, 4, true>(p, tiles, s);
+        else lora_launch<E, 1, true>(p, tiles, s);
+    } else lora_launch<E, 1, false>(p, tiles, s);
+    NVR_KX_LAUNCHED("lora_add");
+    return 0;
+}
+
+int lora_add(int dt, const LoraArgs &a, hipStream_t s) {
+    if (a.T < 0 || a.K <= 0 || a.N <= 0 || a.R <= 0 || a.n < 0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: T=%ld K=%ld N=%ld R=%ld adapters=%ld", (long)a.T, (long)a.K, (long)a.N, (long)a.R, (long)a.n);
+    if (a.R > 256 || a.n >= kMaxAdapters || a.K > (1 << 24) || a.N > (1 << 24) || a.T > (1 << 24))
+        return nvr::fail(NVR_ERR_UNSUPPORTED, "nvr_lora_add: ranks up to 256, fewer than %d adapters, sizes up to 2^24 (T=%ld K=%ld N=%ld R=%ld adapters=%ld)", kMaxAdapters, (long)a.T, (long)a.K, (long)a.N, (long)a.R, (long)a.n);
+    if (a.T == 0) return 0;
+    if (!a.x || !a.ids || !a.base || !a.y || !a.workspace || (a.n && (!a.A || !a.B))) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: null argument");
+    if (((uintptr_t)a.workspace & 15) != 0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: the workspace is not aligned to 16 bytes");
+    if (a.ldx < a.K || a.ldb < a.N || a.ldy < a.N) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: rows overlap");
+    if (a.base == a.y && a.ldb != a.ldy) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: in place with another stride");
+    if (a.n == 0 && a.base == a.y) return 0;
+    NVR_BY_DTYPE(dt, return lora_of<E>(a, s));
+}
+
+}}  // namespace nvr::kx

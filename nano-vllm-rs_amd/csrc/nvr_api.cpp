@@ -11,6 +11,8 @@
 #include "engine.h"
 #include "kernels/kernels.h"
 #include "kernels/device_utils.h"
+#include "kernels/elem.h"
+#include "kernels/serving.h"
 
 namespace k = nvr::k;
 uint64_t nvr_weight_key_impl(uint64_t seed, uint64_t tid);
@@ -843,6 +845,84 @@ int nvr_fill_weight(nvr_half *dst, int64_t rows, int64_t cols, int64_t ld, int64
 int nvr_fill_const(nvr_half *dst, int64_t n, float v, void *s) {
     if (g_ops_f32) return nvr::kf::fill_const(FP(dst), n, v, (hipStream_t)s);
     return KO(fill_const(dst, n, v, (hipStream_t)s));
+}
+
+// ---- operators around a step of many requests (kernels/serving.h)
+static int ops_dtype() { return g_ops_f32 ? nvr::kx::DT_F32 : g_ops_bf16 ? nvr::kx::DT_BF16 : nvr::kx::DT_F16; }
+static bool fits32(std::initializer_list<int64_t> v) { for (int64_t x : v) if (x < INT32_MIN || x > INT32_MAX) return false; return true; }
+int nvr_rope_frequencies(const nvr_rope_scaling *sc, int64_t rd, double *turns_dev, float *amplitude) {
+    NVR_GUARD_BEGIN
+    if (!sc || !turns_dev || !amplitude) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: null argument");
+    if (rd <= 0 || rd % 2 || rd > 4096) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: rotary_dim %ld has to be even, 2 .. 4096", (long)rd);
+    if (!(sc->theta > 0) || !std::isfinite(sc->theta)) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: theta %g", sc->theta);
+    if (sc->kind < NVR_ROPE_PLAIN || sc->kind > NVR_ROPE_BANDS) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: scaling kind %d", (int)sc->kind);
+    const double s = sc->kind == NVR_ROPE_PLAIN ? 1.0 : sc->factor, around = 6.283185307179586476925286766559;
+    if (!(s > 0) || !std::isfinite(s)) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: factor %g", s);
+    const bool ranged = sc->kind == NVR_ROPE_YARN || sc->kind == NVR_ROPE_BANDS;
+    if (ranged && (!(sc->original_len > 0) || !std::isfinite(sc->original_len) || !(sc->low > 0) || !(sc->high > sc->low) || !std::isfinite(sc->high)))
+        return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: original_len %g, turns %g .. %g", sc->original_len, sc->low, sc->high);
+    if (sc->kind == NVR_ROPE_NTK && rd == 2) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: NTK needs more than one pair");
+    if (sc->kind == NVR_ROPE_YARN && sc->theta == 1.0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_frequencies: pairs of one frequency (theta 1) have no range");
+    const double n = (double)rd, theta = sc->kind == NVR_ROPE_NTK ? sc->theta * std::pow(s, n / (n - 2)) : sc->theta;
+    double from = 0, to = 0;
+    if (sc->kind == NVR_ROPE_YARN) {
+        auto pair_of = [&](double turns) { return n * std::log(sc->original_len / (turns * around)) / (2 * std::log(theta)); };
+        from = std::max(std::floor(pair_of(sc->high)), 0.0); to = std::min(std::ceil(pair_of(sc->low)), n - 1);
+    }
+    std::vector<double> turns(rd / 2);
+    for (int64_t j = 0; j < rd / 2; ++j) {
+        double f = std::pow(theta, -2.0 * (double)j / n);
+        if (sc->kind == NVR_ROPE_LINEAR) f /= s;
+        else if (sc->kind == NVR_ROPE_YARN) {
+            const double r = std::min(std::max(((double)j - from) / std::max(to - from, 1e-3), 0.0), 1.0);
+            f = f / s * r + f * (1 - r);
+        } else if (sc->kind == NVR_ROPE_BANDS) {
+            const double r = std::min(std::max((sc->original_len * f / around - sc->low) / (sc->high - sc->low), 0.0), 1.0);
+            f = (1 - r) * f / s + r * f;
+        }
+        turns[j] = f / around;
+    }
+    *amplitude = sc->kind == NVR_ROPE_YARN && s > 1 ? (float)(0.1 * std::log(s) + 1.0) : 1.0f;
+    NVR_HIP_CHECK(hipMemcpy(turns_dev, turns.data(), turns.size() * sizeof(double), hipMemcpyHostToDevice));
+    return NVR_OK;
+    NVR_GUARD_END(NVR_ERR_INVARIANT)
+}
+int nvr_rope_rotate_store_kv(const nvr_half *q, int64_t ldq, const nvr_half *k, int64_t ldk, const nvr_half *v, int64_t ldv, const int64_t *positions, const int32_t *slots,
+                             int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t rd, int interleaved, const double *turns, float amplitude, nvr_half *q_out, int64_t ldqo,
+                             nvr_half *k_out, int64_t ldko, nvr_half *kc, nvr_half *vc, int64_t num_slots, void *s) {
+    if (!fits32({H, KVH, D, rd}) || H + KVH > 65536) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_rope_rotate_store_kv: H=%ld KVH=%ld D=%ld rotary_dim=%ld", (long)H, (long)KVH, (long)D, (long)rd);
+    nvr::kx::RopeArgs a{q, k, v, ldq, ldk, ldv, positions, slots, T, (int32_t)H, (int32_t)KVH, (int32_t)D, (int32_t)rd, interleaved != 0, turns, amplitude, q_out, k_out, ldqo, ldko, kc, vc, num_slots};
+    return nvr::kx::rope_rotate_store(ops_dtype(), a, (hipStream_t)s);
+}
+size_t nvr_lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R) { return nvr::kx::lora_workspace_bytes(T, K, N, R); }
+int nvr_lora_add(const nvr_half *x, int64_t ldx, const nvr_half *A, const nvr_half *B, const float *scales, const int32_t *ids, int64_t n, int64_t T, int64_t K, int64_t N, int64_t R,
+                 const nvr_half *base, int64_t ldb, nvr_half *y, int64_t ldy, void *ws, void *s) {
+    nvr::kx::LoraArgs a{x, ldx, A, B, scales, ids, n, T, K, N, R, base, ldb, y, ldy, ws};
+    return nvr::kx::lora_add(ops_dtype(), a, (hipStream_t)s);
+}
+size_t nvr_sample_uniform_workspace_bytes(int64_t B, int64_t V) { return nvr::kx::sample_uniform_workspace_bytes(B, V); }
+int nvr_sample_uniform(const float *logits, int64_t ld, int64_t B, int64_t V, const float *temperature, const int64_t *top_k, const float *top_p, const float *min_p, const float *uniform,
+                       int64_t *ids, float *logprobs, void *ws, void *s) {
+    nvr::kx::SampleArgs a{logits, ld, B, V, temperature, top_k, top_p, min_p, uniform, ids, logprobs, ws};
+    return nvr::kx::sample_uniform(a, (hipStream_t)s);
+}
+size_t nvr_paged_attn_scored_workspace_bytes(int64_t B, int64_t H, int64_t KVH, int64_t D, int64_t max_ctx) { return nvr::kx::paged_attn_scored_workspace_bytes(B, H, KVH, D, max_ctx); }
+int nvr_paged_attn_decode_scored(const nvr_half *q, int64_t ldq, const nvr_half *kc, const nvr_half *vc, const nvr_attn_meta *m, int64_t H, int64_t KVH, int64_t D, int64_t bs, int64_t nb,
+                                 float scale, const float *scores, const int32_t *scored, float decay, float *new_scores, nvr_half *out, void *ws, void *s) {
+    if (!m) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_paged_attn_decode_scored: meta is null");
+    if (!fits32({H, KVH, D, bs, nb})) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_paged_attn_decode_scored: H=%ld KVH=%ld D=%ld block_size=%ld num_blocks=%ld", (long)H, (long)KVH, (long)D, (long)bs, (long)nb);
+    nvr::kx::ScoredArgs a{q, ldq, kc, vc, m->context_lens, m->block_tables, m->max_blocks, (int32_t)bs, nb, m->batch, (int32_t)H, (int32_t)KVH, (int32_t)D, m->max_context_len, scale,
+                          scores, scored, decay, new_scores, out, ws};
+    return nvr::kx::paged_attn_scored(ops_dtype(), a, (hipStream_t)s);
+}
+size_t nvr_kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_ctx) { return nvr::kx::kv_evict_workspace_bytes(B, KVH, budget, max_ctx); }
+int nvr_kv_evict(nvr_half *kc, nvr_half *vc, float *scores, const nvr_attn_meta *m, int64_t KVH, int64_t D, int64_t bs, int64_t nb, int64_t budget, int64_t first, int64_t last,
+                 const int32_t *to, int64_t to_max_blocks, int32_t *new_lens, int32_t *kept, void *ws, void *s) {
+    if (!m) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_kv_evict: meta is null");
+    if (!fits32({KVH, D, bs, nb, budget, first, last, to_max_blocks})) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_kv_evict: KVH=%ld D=%ld block_size=%ld num_blocks=%ld budget=%ld", (long)KVH, (long)D, (long)bs, (long)nb, (long)budget);
+    nvr::kx::EvictArgs a{kc, vc, scores, m->context_lens, m->block_tables, m->max_blocks, (int32_t)bs, nb, m->batch, (int32_t)KVH, (int32_t)D, m->max_context_len, (int32_t)budget, (int32_t)first,
+                         (int32_t)last, to, (int32_t)to_max_blocks, new_lens, kept, ws};
+    return nvr::kx::kv_evict(ops_dtype(), a, (hipStream_t)s);
 }
 
 }  // extern "C"

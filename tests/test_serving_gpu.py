@@ -1,0 +1,575 @@
+"""GPU tests (-m gpu) of the operators around a serving step against their definitions in 64 bits (serving_util).
+
+Tolerances come from the arithmetic: a value rounded once is off by half a step of its type (HALF_STEP), a sum of n products in 32 bits by at most n 2^-24 of the sum of the products' sizes."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import nvr_import
+from serving_util import DTYPES, F32, HALF_STEP, SENTINEL, SMALLEST, Arena, attend, byref, decode, encode, evict, kind, meta, rope, rope_turns, sample, tables, typed
+
+nvr = nvr_import.load()
+pytestmark = pytest.mark.gpu
+L = nvr.lib()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    assert nvr.device_count() >= 1, "no HIP device visible: the GPU tests must run on an MI355X"
+    nvr.check(L.nvr_device_set(0))
+    yield
+    nvr.synchronize()
+    typed("float16")
+
+
+@pytest.fixture
+def arena():
+    a = Arena()
+    yield a
+    nvr.synchronize()
+    a.kept.clear()
+
+
+def within(got, want, tol, what=""):
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), "%s: %d of %d off, worst %g of the %g allowed" % (what, bad.sum(), bad.size, np.abs(got - want)[bad].max(), np.broadcast_to(tol, want.shape)[bad].min())
+
+
+# ------------------------------------------------------------------------------------------------------------ rotary positions
+KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+@pytest.mark.parametrize("rotary", [2, 64, 128])
+@pytest.mark.parametrize("name,factor,low,high", [("plain", 1.0, 1.0, 32.0), ("linear", 8.0, 1.0, 32.0), ("ntk", 4.0, 1.0, 32.0), ("yarn", 16.0, 1.0, 32.0), ("yarn", 0.5, 1.0, 32.0), ("bands", 8.0, 1.0, 4.0)])
+def test_rope_frequencies(arena, name, factor, low, high, rotary):
+    sc = nvr.RopeScalingC(KINDS[name], 500000.0, factor, 8192.0, low, high)
+    if name == "ntk" and rotary == 2:
+        pytest.skip("refused: NTK needs more than one pair")
+    d, amplitude = arena.space(rotary // 2 * 8), C.c_float()
+    nvr.check(L.nvr_rope_frequencies(byref(sc), rotary, d.ptr, byref(amplitude)))
+    turns, a = rope_turns(name, rotary, 500000.0, factor, 8192.0, low, high)
+    assert np.allclose(d.to_numpy((rotary // 2,), np.float64), turns, rtol=1e-13, atol=0)      # (powers and logarithms of 64 bits: a few steps of 2^-53)
+    assert abs(amplitude.value - a) <= a * 2 ** -23
+
+
+ROPE_CASES = [  # T, H, KVH, D, rotary, pairs, far, extra columns between rows
+    (1, 4, 2, 128, 128, False, 10, 0), (33, 16, 8, 128, 128, False, 4096, 0), (7, 3, 1, 64, 32, True, 1000000, 0), (5, 2, 2, 80, 32, False, 100, 0), (9, 2, 1, 96, 24, True, 100, 8),
+    (3, 1, 1, 2, 2, False, 50, 0), (4, 2, 1, 10, 6, True, 50, 3), (4100, 2, 1, 64, 64, False, 1 << 40, 0), (2050, 1, 1, 128, 64, True, 130000, 0), (6, 0, 2, 64, 64, False, 9, 0), (6, 2, 0, 64, 64, True, 9, 0),
+    (13, 4, 2, 256, 256, False, 70000, 0), (2, 1, 1, 1024, 1024, False, 70000, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,G,D,rotary,pairs,far,gap", ROPE_CASES)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rope_rotate_store(arena, dtype, T, H, G, D, rotary, pairs, far, gap, in_place):
+    rng = np.random.default_rng(T * 31 + D)
+    typed(dtype)
+    w, ld = np.dtype(kind(dtype)).itemsize, (H + 2 * G) * D + gap
+    x, bits = encode(rng.standard_normal((T, ld)) * 4, dtype)
+    positions = rng.integers(-far if far < 1000 else 0, far, T)
+    turns, amplitude = rope_turns("yarn", rotary, 10000.0, 4.0)
+    slots_n = T + 5
+    slots = rng.permutation(slots_n)[:T].astype(np.int32)
+    if T > 2:
+        slots[1] = -1 if T % 2 else slots_n                        # not stored
+    buf = arena.dev(bits)
+    kc, vc = arena.space(slots_n * max(G, 1) * D * w), arena.space(slots_n * max(G, 1) * D * w)
+    at = buf.ptr
+    q_out, k_out = (None, None) if in_place else (arena.space(T * max(H, 1) * D * w), arena.space(T * max(G, 1) * D * w))
+    qo, ldqo = (at, ld) if in_place else (q_out.ptr, H * D)
+    ko, ldko = (at + H * D * w, ld) if in_place else (k_out.ptr, G * D)
+    nvr.check(L.nvr_rope_rotate_store_kv(at, ld, at + H * D * w, ld, at + (H + G) * D * w, ld, arena.dev(positions.astype(np.int64)).ptr, arena.dev(slots).ptr, T, H, G, D, rotary, int(pairs),
+                                         arena.dev(turns).ptr, amplitude, qo, ldqo, ko, ldko, kc.ptr, vc.ptr, slots_n, None))
+    heads = x[:, :(H + G) * D].reshape(T, H + G, D)
+    amplitude = float(np.float32(amplitude))
+    want = rope(heads, positions, turns, amplitude, pairs)
+    # cos and sin rounded, two products of which one is rounded, one sum: 3 roundings of 32 bits of either term, then the store's
+    size = np.abs(rope(np.abs(heads), positions * 0, turns, amplitude, pairs)) + amplitude * np.abs(heads).max(-1, keepdims=True)
+    tol = 4 * F32 * size + HALF_STEP[dtype] * np.abs(want) * (1 + 2 ** -10) + SMALLEST[dtype]
+    if in_place:
+        all_ = decode(buf.to_numpy((T, ld), kind(dtype)), dtype)
+        q, k = all_[:, :H * D].reshape(T, H, D), all_[:, H * D:(H + G) * D].reshape(T, G, D)
+        assert np.array_equal(all_[:, (H + G) * D:], x[:, (H + G) * D:])
+    else:
+        q, k = decode(q_out.to_numpy((T, H, D), kind(dtype)), dtype), decode(k_out.to_numpy((T, G, D), kind(dtype)), dtype)
+    within(np.concatenate([q, k], 1), want, tol, "rotated")
+    assert np.array_equal(np.concatenate([q, k], 1)[..., rotary:], heads[..., rotary:])
+    if G:
+        K, V = kc.to_numpy((slots_n, G, D), kind(dtype)), vc.to_numpy((slots_n, G, D), kind(dtype))
+        stored = np.zeros(slots_n, bool)
+        for t in range(T):
+            if 0 <= slots[t] < slots_n:
+                stored[slots[t]] = True
+                assert np.array_equal(decode(K[slots[t]], dtype), k[t])
+                assert np.array_equal(decode(V[slots[t]], dtype), x[t, (H + G) * D:(H + 2 * G) * D].reshape(G, D))
+        untouched = np.frombuffer(bytes([SENTINEL]) * w, kind(dtype))[0]
+        assert (K[~stored] == untouched).all() and (V[~stored] == untouched).all()
+
+
+def test_rope_without_caches_and_unaligned_rows(arena):
+    """Rotation alone; rows that begin 2 bytes off a piece of 16 take the form that reads numbers one by one, with the same values."""
+    rng = np.random.default_rng(5)
+    typed("bfloat16")
+    T, H, G, D = 11, 4, 2, 64
+    turns, _ = rope_turns("plain", 64)
+    x, bits = encode(rng.standard_normal((T, (H + G) * D)), "bfloat16")
+    pos = arena.dev(rng.integers(0, 5000, T))
+    answers = []
+    for off in (0, 1):
+        src = np.zeros(T * (H + G) * D + 8, np.uint16)
+        src[off:off + bits.size] = bits.ravel()
+        buf, q, k = arena.dev(src), arena.space(T * H * D * 2 + 16), arena.space(T * G * D * 2 + 16)
+        at, ld = buf.ptr + 2 * off, (H + G) * D
+        nvr.check(L.nvr_rope_rotate_store_kv(at, ld, at + H * D * 2, ld, None, 0, pos.ptr, None, T, H, G, D, 64, 0, arena.dev(turns).ptr, 1.0, q.ptr + 2 * off, H * D, k.ptr + 2 * off, G * D,
+                                             None, None, 0, None))
+        answers.append((q.to_numpy((T * H * D + 8,), np.uint16)[off:off + T * H * D], k.to_numpy((T * G * D + 8,), np.uint16)[off:off + T * G * D]))
+    assert np.array_equal(answers[0][0], answers[1][0]) and np.array_equal(answers[0][1], answers[1][1])
+
+
+# ------------------------------------------------------------------------------------------------------------ low-rank adapters
+def lora_case(arena, dtype, T, K, N, R, n, ids, in_place=False, gap=0, scales=True, seed=0, amplify=1.0, off=0):
+    rng = np.random.default_rng(seed + T + K + N + R)
+    typed(dtype)
+    w = np.dtype(kind(dtype)).itemsize
+    x, xb = encode(rng.standard_normal((T, K + gap)) * amplify, dtype)
+    A, Ab = encode(rng.standard_normal((max(n, 1), R, K)) * K ** -0.5 * amplify, dtype)
+    B, Bb = encode(rng.standard_normal((max(n, 1), N, R)) * R ** -0.5 / amplify ** 2, dtype)
+    base, bb = encode(rng.standard_normal((T, N + gap)), dtype)
+    sc = (0.5 + rng.random(max(n, 1))).astype(np.float32)
+    ids = np.asarray(ids, np.int32)
+    pad = np.zeros(off, kind(dtype))
+    dx, da, db = (arena.dev(np.concatenate([pad, b.ravel()])).ptr + off * w for b in (xb, Ab, Bb))
+    dbase = arena.dev(bb)
+    dy = dbase if in_place else arena.space(T * (N + gap) * w)
+    ws = arena.space(L.nvr_lora_workspace_bytes(T, K, N, R), 0xFF)       # (NaN wherever something stale would be read)
+    nvr.check(L.nvr_lora_add(dx, K + gap, da, db, arena.dev(sc).ptr if scales else None, arena.dev(ids).ptr, n, T, K, N, R, dbase.ptr, N + gap, dy.ptr, N + gap, ws.ptr, None))
+    bits = dy.to_numpy((T, N + gap), kind(dtype))
+    got = decode(bits, dtype)[:, :N]
+    want, tol = base[:, :N].copy(), np.zeros((T, N))
+    two = {"float16": 2.0 ** -21, "bfloat16": 2.0 ** -15, "float32": 0.0}[dtype]        # v in two numbers: half a step of half a step, relative to the row's largest (float16), to itself (bfloat16)
+    for a in range(n):
+        rows = ids == a
+        if not rows.any():
+            continue
+        s = float(sc[a]) if scales else 1.0
+        v = s * x[rows, :K] @ A[a].T
+        dv = s * (K + 8) * F32 * (np.abs(x[rows, :K]) @ np.abs(A[a]).T) + two * np.abs(v).max(1, keepdims=True)
+        want[rows] += v @ B[a].T
+        tol[rows] = dv @ np.abs(B[a]).T + (R + 8) * F32 * (np.abs(v) @ np.abs(B[a]).T) + F32 * np.abs(base[rows, :N])
+    touched = (ids >= 0) & (ids < n)
+    tol += HALF_STEP[dtype] * (np.abs(want) + tol) + SMALLEST[dtype]
+    within(got[touched], want[touched], tol[touched], "adapters")
+    assert np.array_equal(got[~touched], base[~touched, :N])
+    if gap:
+        assert np.array_equal(bits[:, N:], bb[:, N:] if in_place else np.full((T, gap), np.frombuffer(bytes([SENTINEL]) * w, kind(dtype))[0]))
+    return bits
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,N,R,n", [(1, 64, 64, 8, 1), (1, 1024, 2048, 16, 3), (5, 256, 100, 1, 2), (17, 96, 72, 5, 4), (32, 1024, 512, 16, 32), (64, 200, 1000, 33, 7), (251, 512, 264, 64, 7),
+                                       (256, 128, 64, 96, 300), (3, 40, 17, 256, 2), (16, 2048, 33, 128, 1), (7, 33, 31, 3, 2)])
+def test_lora_few_rows(arena, dtype, T, K, N, R, n):
+    rng = np.random.default_rng(T)
+    lora_case(arena, dtype, T, K, N, R, n, rng.integers(-1, n + 1, T))          # n: not an adapter either
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K,N,R,n,order", [(257, 64, 96, 16, 3, "mixed"), (1000, 128, 200, 32, 5, "runs"), (1001, 72, 64, 7, 300, "mixed"), (2049, 256, 128, 64, 2, "mixed"), (700, 64, 64, 200, 1, "runs"),
+                                             (513, 64, 40, 128, 1, "runs"), (4097, 32, 32, 8, 64, "mixed")])
+def test_lora_many_rows(arena, dtype, T, K, N, R, n, order):
+    rng = np.random.default_rng(T)
+    ids = rng.integers(-1, n, T) if order == "mixed" else np.minimum(np.arange(T) * (n + 1) // T - 1, n - 1)
+    lora_case(arena, dtype, T, K, N, R, n, ids)
+
+
+@pytest.mark.parametrize("T", [40, 600])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lora_in_place_with_strides_and_unaligned_tensors(arena, dtype, T):
+    rng = np.random.default_rng(1)
+    ids = rng.integers(-1, 3, T)
+    lora_case(arena, dtype, T, 96, 56, 16, 3, ids, in_place=True, gap=8)
+    lora_case(arena, dtype, T, 96, 56, 16, 3, ids, in_place=True, gap=3, off=1)
+    lora_case(arena, dtype, T, 96, 56, 16, 3, ids, scales=False, gap=5, off=3)
+
+
+@pytest.mark.parametrize("T", [30, 500])
+def test_lora_rows_without_adapters_and_no_adapters(arena, T):
+    lora_case(arena, "bfloat16", T, 64, 48, 8, 2, np.full(T, -1))
+    lora_case(arena, "bfloat16", T, 64, 48, 8, 2, np.full(T, -1), in_place=True)
+    lora_case(arena, "float16", T, 64, 48, 8, 0, np.zeros(T))
+
+
+@pytest.mark.parametrize("amplify", [2.0 ** 6, 2.0 ** -8])
+def test_lora_inner_products_beyond_float16(arena, amplify):
+    """x A^T of 10^5 (beyond float16) and of 10^-5 (among its subnormals) against B that undoes it."""
+    lora_case(arena, "float16", 20, 512, 40, 16, 2, np.arange(20) % 2, amplify=amplify)
+
+
+def test_lora_rows_do_not_depend_on_their_step(arena):
+    """A row's bits are the same whatever other rows the step has, up to 256 rows and the same number of K's shares."""
+    typed("bfloat16")
+    ids = np.array([0, 1, 0, 2, 1, 0])
+    a = lora_case(arena, "bfloat16", 6, 64, 64, 16, 3, ids, seed=3)
+    b = lora_case(arena, "bfloat16", 6, 64, 64, 16, 3, ids, seed=3)
+    assert np.array_equal(a, b)
+
+
+def test_lora_of_infinite_rows_stays_in_its_rows(arena):
+    typed("float16")
+    T, K, N, R = 20, 64, 32, 8
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((T, K)).astype(np.float16)
+    x[3, 5], x[4, 6] = np.inf, np.nan
+    A, B, base = rng.standard_normal((1, R, K)).astype(np.float16), rng.standard_normal((1, N, R)).astype(np.float16), rng.standard_normal((T, N)).astype(np.float16)
+    y, ws = arena.space(T * N * 2), arena.space(L.nvr_lora_workspace_bytes(T, K, N, R))
+    nvr.check(L.nvr_lora_add(arena.dev(x).ptr, K, arena.dev(A).ptr, arena.dev(B).ptr, None, arena.dev(np.zeros(T, np.int32)).ptr, 1, T, K, N, R, arena.dev(base).ptr, N, y.ptr, N, ws.ptr, None))
+    got = y.to_numpy((T, N), np.float16)
+    fine = np.isfinite(got).all(1)
+    assert not np.isfinite(got[[3, 4]]).any() and fine[[t for t in range(T) if t not in (3, 4)]].all()
+
+
+# ------------------------------------------------------------------------------------------------------------ tokens from given numbers
+def sample_rows(arena, x, T, k, p, m, u, ld=None, logprobs=True, off=0):
+    B, V = x.shape
+    ld = ld or V
+    buf = np.full(B * ld + off, np.nan, np.float32)
+    for r in range(B):
+        buf[off + r * ld:off + r * ld + V] = x[r]
+    ids, lp = arena.space(B * 8), arena.space(B * 4)
+    ws = arena.space(L.nvr_sample_uniform_workspace_bytes(B, V), 0xFF)
+
+    def opt(a, t):
+        return None if a is None else arena.dev(np.asarray(a, t)).ptr
+    nvr.check(L.nvr_sample_uniform(arena.dev(buf).ptr + 4 * off, ld, B, V, opt(T, np.float32), opt(k, np.int64), opt(p, np.float32), opt(m, np.float32), opt(u, np.float32), ids.ptr,
+                                   lp.ptr if logprobs else None, ws.ptr, None))
+    return ids.to_numpy((B,), np.int64), lp.to_numpy((B,), np.float32)
+
+
+def check_sample(arena, x, T, k, p, m, u, **kw):
+    x = np.asarray(x, np.float32)
+    B = len(x)
+    T, k, p, m, u = (np.broadcast_to(np.asarray(a, t), (B,)) for a, t in ((T, np.float32), (k, np.int64), (p, np.float32), (m, np.float32), (u, np.float32)))
+    ids, lp = sample_rows(arena, x, T, k, p, m, u, **kw)
+    want = [sample(x[r], float(T[r]), int(k[r]), float(p[r]), float(m[r]), float(u[r])) for r in range(B)]
+    assert ids.tolist() == [w[0] for w in want]
+    for got, (_, w) in zip(lp.tolist(), want):
+        assert got == w if math.isinf(w) else abs(got - w) <= 1e-7 * max(1.0, abs(w)), (got, w)       # (64 bits inside: one rounding to 32, 6e-8)
+
+
+@pytest.mark.parametrize("B,V", [(1, 1), (3, 2), (5, 100), (4, 4096), (3, 4097), (2, 16385), (7, 50001), (2, 151936), (70, 40000)])
+def test_sample_settings(arena, B, V):
+    rng = np.random.default_rng(V)
+    for std in (0.3, 2.0, 8.0):
+        x = rng.standard_normal((B, V)) * std
+        for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.3, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.05), (0.8, 40, 0.95, 0.02), (0.0, 5, 0.5, 0.1), (2.5, 1000, 0.99, 0.0), (0.05, 3, 0.2, 0.9)):
+            check_sample(arena, x, T, k, p, m, rng.random(B).astype(np.float32))
+
+
+def test_sample_rows_of_their_own_settings(arena):
+    rng = np.random.default_rng(9)
+    B, V = 40, 30000
+    x = rng.standard_normal((B, V)) * 3
+    check_sample(arena, x, rng.choice([0.0, 0.5, 1.0, 1.7], B), rng.choice([0, 1, 20, 29999, 30000, 10 ** 12, -3], B), rng.choice([0.0, 0.3, 0.9, 1.0, -1.0, 2.0], B), rng.choice([0.0, 0.01, 0.3, 1.0, 5.0], B),
+                 rng.random(B).astype(np.float32), ld=V + 7)
+    check_sample(arena, x, 1.0, 0, 0.9, 0.0, rng.random(B).astype(np.float32), ld=V + 4, off=1)
+
+
+def test_sample_ends_of_the_unit_interval(arena):
+    rng = np.random.default_rng(10)
+    x = rng.standard_normal((4, 9000))
+    for u in (0.0, 1 - 2.0 ** -24):
+        check_sample(arena, x, 1.0, 0, 1.0, 0.0, u)
+        check_sample(arena, x, 1.0, 7, 1.0, 0.0, u)
+    ids, _ = sample_rows(arena, x.astype(np.float32), None, None, None, None, np.full(4, 1.5))     # beyond it: the last token with weight
+    assert ids.tolist() == [8999] * 4
+
+
+def test_sample_ties(arena):
+    """Equal logits: prefixes end inside them, lowest indices first; more of them than the candidate list holds."""
+    for V in (8, 5000, 20000):
+        x = np.zeros((3, V), np.float32)
+        x[1, ::2] = 1.0
+        x[2] = np.arange(V) % 3
+        rng = np.random.default_rng(V)
+        for k, p in ((0, 0.5), (V // 2 + 1, 1.0), (5, 0.5), (V // 4 * 3, 0.25), (0, 1.0)):
+            for u in rng.random(4).astype(np.float32):
+                check_sample(arena, x, 1.0, k, p, 0.0, u)
+        check_sample(arena, x, 1.0, 0, 1.0, 1.0, 0.999)
+        check_sample(arena, x, 0.0, 0, 1.0, 0.0, 0.5)
+
+
+def test_sample_flat_bins(arena):
+    """Distinct logits so close together that tens of thousands fall into the bin that the prefix ends in."""
+    rng = np.random.default_rng(11)
+    V = 60000
+    x = (5.0 + rng.random((3, V)) * 0.01).astype(np.float32)
+    for k, p, m in ((0, 0.5, 0.0), (30001, 1.0, 0.0), (40000, 0.3, 0.0), (0, 1.0, 0.999), (20000, 0.9, 0.995)):
+        check_sample(arena, x, 1.0, k, p, m, rng.random(3).astype(np.float32))
+
+
+def test_sample_masked_logits(arena):
+    rng = np.random.default_rng(12)
+    V = 20000
+    x = rng.standard_normal((8, V)).astype(np.float32)
+    low = np.finfo(np.float32).min
+    x[0, 100:] = -np.inf
+    x[1, :] = -np.inf
+    x[2, :] = np.nan
+    x[3, ::2] = np.nan
+    x[4, :] = low
+    x[5, 1:] = low
+    x[6, [5, 17000]] = np.inf
+    x[7, :] = -np.inf
+    x[7, 12345] = -300.0
+    u = rng.random(8).astype(np.float32)
+    for k, p, m in ((0, 1.0, 0.0), (50, 0.9, 0.0), (0, 0.9, 0.1), (300, 1.0, 0.0)):
+        for T in (1.0, 0.0, 0.3):
+            check_sample(arena, x, T, k, p, m, u)
+
+
+def test_sample_large_and_small_scales(arena):
+    rng = np.random.default_rng(13)
+    for std, T in ((1e4, 1e3), (1e-3, 1e-3), (1e30, 1e30), (100.0, 1e-3), (1.0, 1e6), (1e-6, 1e-4)):
+        x = (rng.standard_normal((3, 6000)) * std).astype(np.float32)
+        for k, p, m in ((0, 1.0, 0.0), (20, 0.9, 0.0), (0, 1.0, 0.1)):
+            check_sample(arena, x, T, k, p, m, rng.random(3).astype(np.float32))
+
+
+def test_sample_optional_arguments_and_streams(arena):
+    rng = np.random.default_rng(14)
+    x = rng.standard_normal((2, 3000)).astype(np.float32)
+    u = np.array([0.2, 0.7], np.float32)
+    ids, _ = sample_rows(arena, x, None, None, None, None, u, logprobs=False)
+    assert ids.tolist() == [sample(x[r], 1.0, 0, 1.0, 0.0, float(u[r]))[0] for r in range(2)]
+
+
+# ------------------------------------------------------------------------------------------------------------ scored attention
+def scored_case(arena, dtype, lengths, H, G, D, block, seed=0, scored=None, decay=0.9, bad=(), in_place=False, max_context=None, q_gap=0, qs=1.0, poison=False, mutate=None):
+    rng = np.random.default_rng(seed + sum(lengths) + H + D)
+    typed(dtype)
+    w = np.dtype(kind(dtype)).itemsize
+    table, blocks = tables(rng, lengths, block, extra=1)
+    B = len(lengths)
+    q, qb = encode(rng.standard_normal((B, H * D + q_gap)) * qs, dtype)
+    k, kb = encode(rng.standard_normal((blocks, block, G, D)), dtype)
+    v, vb = encode(rng.standard_normal((blocks, block, G, D)), dtype)
+    named = table.copy()
+    for b, i, page in bad:
+        table[b, i] = page
+    if poison:                                                     # every row that no key of a sequence has: not a number
+        free = np.ones((blocks, block), bool)
+        for b, n in enumerate(lengths):
+            for j in range(n):
+                free[named[b, j // block], j % block] = False
+        nan = {"float16": 0x7E00, "bfloat16": 0x7FC0, "float32": 0x7FC00000}[dtype]
+        kb[free], vb[free] = nan, nan
+    scores = rng.random((blocks, G, block)).astype(np.float32)
+    scale = D ** -0.5
+    ds = arena.dev(scores)
+    dn = ds if in_place else arena.space(scores.nbytes)
+    before = dn.to_numpy(scores.shape, np.float32)
+    top = max(max(lengths), 0) if max_context is None else max_context
+    m = meta(arena, lengths, table, top)
+    out = arena.space(B * H * D * w)
+    ws = arena.space(L.nvr_paged_attn_scored_workspace_bytes(B, H, G, D, top), 0xFF)
+    nvr.check(L.nvr_paged_attn_decode_scored(arena.dev(qb).ptr, H * D + q_gap, arena.dev(kb).ptr, arena.dev(vb).ptr, byref(m), H, G, D, block, blocks, scale, ds.ptr,
+                                             arena.dev(np.array(scored, np.int32)).ptr if scored is not None else None, decay, dn.ptr, out.ptr, ws.ptr, None))
+    got = decode(out.to_numpy((B, H, D), kind(dtype)), dtype)
+    new = dn.to_numpy(scores.shape, np.float32)
+    two = {"float16": 2.0 ** -21, "bfloat16": 2.0 ** -15, "float32": 0.0}[dtype]
+    touched = np.zeros(scores.shape, bool)
+    for b, n in enumerate(lengths):
+        n = min(n, top, table.shape[1] * block)
+        j = np.arange(n)
+        page = table[b, j // block]
+        j = j[(page >= 0) & (page < blocks)]
+        if len(j) == 0:
+            assert (got[b] == 0).all()
+            continue
+        page, row = table[b, j // block], j % block
+        qq, kk, vv = q[b, :H * D].reshape(H, D), k[page, row], v[page, row]
+        want, weights = attend(qq, kk, vv, scale)
+        # a score is off by (D + 4) roundings of its products' sizes, a weight by twice the largest such (numerator and sum) and the exponential's, and so on
+        size = max(float((np.abs(kk[:, g]) @ np.abs(qq[h])).max()) for h in range(H) for g in [h * G // H]) * scale
+        dw = 2 * (D + 4) * F32 * size + (n / 4 + 64) * F32
+        for h in range(H):
+            s = scale * (kk[:, h * G // H] @ qq[h])
+            e = np.exp(s - s.max())
+            tol = (2 * dw + two) * ((e / e.sum()) @ np.abs(vv[:, h * G // H]))
+            within(got[b, h], want[h], tol + HALF_STEP[dtype] * (np.abs(want[h]) + tol) + SMALLEST[dtype], "out")
+        first = (n - 1 if scored is None else scored[b])
+        for g in range(G):
+            old = np.where(j < first, np.float64(np.float32(decay)) * scores[page, g, row], 0.0)
+            within(new[page, g, row].astype(np.float64), old + weights[:, g], 2 * dw * weights[:, g] + 4 * F32 * (old + weights[:, g]) + 1e-37, "scores")
+            touched[page, g, row] = True
+    assert np.array_equal(new[~touched].view(np.uint32), before[~touched].view(np.uint32))
+    return got, new
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D", [(2, 1, 64), (16, 8, 128), (8, 8, 128), (32, 8, 128), (16, 1, 64), (3, 1, 128), (4, 2, 256)])
+def test_scored_attention(arena, dtype, H, G, D):
+    scored_case(arena, dtype, [1, 33, 130], H, G, D, 16)
+    scored_case(arena, dtype, [517], H, G, D, 256)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", [1, 7, 16, 48, 64, 256, 300])
+def test_scored_attention_blocks(arena, dtype, block):
+    """Pages that end inside a tile, and rows of the pool that no sequence has (not a number: their weight of 0 must not meet them)."""
+    scored_case(arena, dtype, [5, 31, 32, 33, 64, 100], 4, 2, 64, block, poison=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scored_attention_lengths(arena, dtype):
+    scored_case(arena, dtype, [0, 1, 0, 2, 15, 16, 17, 127, 128, 129, 255, 256, 257, 511, 513, 1025], 4, 2, 128, 64, poison=True)
+    scored_case(arena, dtype, [3000, 1, 2200], 4, 1, 64, 32)
+    scored_case(arena, dtype, [0, 0], 4, 2, 128, 64)
+
+
+def test_scored_attention_of_many_sequences(arena):
+    rng = np.random.default_rng(3)
+    scored_case(arena, "bfloat16", rng.integers(0, 700, 90).tolist(), 4, 2, 64, 64)
+
+
+def test_scored_attention_new_keys_and_in_place(arena):
+    scored_case(arena, "float16", [40, 90, 130], 4, 2, 64, 16, scored=[0, 50, 130], decay=1.0)
+    scored_case(arena, "bfloat16", [40, 90, 130], 4, 2, 64, 16, scored=[0, 50, 999], decay=0.5, in_place=True)
+    scored_case(arena, "bfloat16", [40, 90, 130], 4, 2, 64, 16, in_place=True, q_gap=3)
+    scored_case(arena, "float32", [40, 90, 130], 4, 2, 64, 16, scored=[-5, 1, 3], in_place=True, q_gap=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scored_attention_pages_outside_the_pool(arena, dtype):
+    """Keys whose page is not in the pool are not there: a whole tile, a part of one, a whole sequence."""
+    scored_case(arena, dtype, [200, 200, 10], 4, 2, 64, 16, bad=[(0, 2, -1), (0, 5, 1 << 20), (1, 8, -7), (1, 9, -7), (2, 0, -1)])
+    scored_case(arena, dtype, [200, 200], 4, 2, 64, 64, bad=[(0, 0, -1), (1, 3, 1 << 30)])
+
+
+def test_scored_attention_cuts_contexts_at_their_bound(arena):
+    scored_case(arena, "float16", [50, 500, 300], 4, 2, 64, 16, max_context=256, scored=[49, 499, 299])
+
+
+def test_scored_attention_peaked(arena):
+    """Weights of one key and of none: scores of +-hundreds."""
+    scored_case(arena, "float32", [300, 65], 4, 2, 64, 16, qs=60.0)
+    scored_case(arena, "float16", [300, 65], 4, 2, 128, 16, qs=30.0)
+
+
+def test_scored_attention_agrees_with_the_plain_one(arena):
+    rng = np.random.default_rng(4)
+    typed("float16")
+    H, G, D, block, lengths = 16, 8, 128, 256, [700, 1300]
+    table, blocks = tables(rng, lengths, block)
+    q, k, v = (rng.standard_normal(s).astype(np.float16) for s in ((2, H, D), (blocks, block, G, D), (blocks, block, G, D)))
+    dq, dk, dv, m = arena.dev(q), arena.dev(k), arena.dev(v), meta(arena, lengths, table)
+    a, b = arena.space(q.nbytes), arena.space(q.nbytes)
+    sc = arena.space(blocks * G * block * 4, 0)
+    nvr.check(L.nvr_paged_attn_decode(dq.ptr, H * D, dk.ptr, dv.ptr, byref(m), H, G, D, block, D ** -0.5, a.ptr, arena.space(L.nvr_paged_attn_workspace_bytes(2, H, D, 1300)).ptr, None))
+    nvr.check(L.nvr_paged_attn_decode_scored(dq.ptr, H * D, dk.ptr, dv.ptr, byref(m), H, G, D, block, blocks, D ** -0.5, sc.ptr, None, 1.0, sc.ptr, b.ptr,
+                                             arena.space(L.nvr_paged_attn_scored_workspace_bytes(2, H, G, D, 1300)).ptr, None))
+    x, y = a.to_numpy(q.shape, np.float16).astype(np.float64), b.to_numpy(q.shape, np.float16).astype(np.float64)
+    within(x, y, 2 * HALF_STEP["float16"] * np.abs(y) + 1e-5, "the two attentions")             # (each rounded once; 32-bit sums of 1300 keys below that)
+    total = sc.to_numpy((blocks, G, block), np.float32).sum(dtype=np.float64)
+    assert abs(total - 2 * H) < 2 * H * 1e-5                                                   # a head's weights sum to 1
+
+
+# ------------------------------------------------------------------------------------------------------------ eviction
+def evict_case(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place, seed=0, scores=None, bad=(), kept_out=True, max_context=None):
+    rng = np.random.default_rng(seed + sum(lengths) + budget)
+    typed(dtype)
+    u = kind(dtype)
+    B = len(lengths)
+    cut = [min(n, budget) for n in lengths]
+    table, blocks = tables(rng, lengths, block)
+    to, more = tables(rng, cut, block)
+    to = np.where(to >= 0, to + blocks, -1).astype(np.int32)
+    total = blocks + (more if out_of_place else 0)
+    for b, i, page in bad:
+        table[b, i] = page
+    top = np.iinfo(u).max
+    k, v = (rng.integers(0, top, (total, block, G, D), dtype=u) for _ in range(2))
+    if scores is None:
+        s = (rng.integers(0, 50, (total, G, block)) / 8).astype(np.float32)                     # many ties
+    else:
+        s = scores((total, G, block), rng)
+    dk, dv, ds = arena.dev(k), arena.dev(v), arena.dev(s)
+    new, kept, ws = arena.space(B * 4), arena.space(B * G * budget * 4), arena.space(L.nvr_kv_evict_workspace_bytes(B, G, budget, max(lengths)))
+    m = meta(arena, lengths, table, max_context)
+    nvr.check(L.nvr_kv_evict(dk.ptr, dv.ptr, ds.ptr, byref(m), G, D, block, total, budget, first, last, arena.dev(to).ptr if out_of_place else None, to.shape[1] if out_of_place else 0, new.ptr,
+                             kept.ptr if kept_out else None, ws.ptr, None))
+    K, V, S = k.copy(), v.copy(), s.copy()
+    want_kept, want_len = np.full((B, G, budget), -1, np.int32), np.zeros(B, np.int32)
+    for b, n in enumerate(lengths):
+        n = min(n, max_context) if max_context is not None else n
+        j = np.arange(n)
+        if n and ((table[b, j // block] < 0) | (table[b, j // block] >= total)).any():
+            want_len[b] = -1
+            continue
+        want_len[b] = min(n, budget)
+        dest = to if out_of_place else table
+        for g in range(G):
+            mine = evict(s[table[b, j // block], g, j % block], budget, first, last)
+            want_kept[b, g, :len(mine)] = mine
+            i = np.arange(len(mine))
+            src, dst = (table[b, mine // block], mine % block), (dest[b, i // block], i % block)
+            K[dst[0], dst[1], g], V[dst[0], dst[1], g], S[dst[0], g, dst[1]] = k[src[0], src[1], g], v[src[0], src[1], g], s[src[0], g, src[1]]
+    assert np.array_equal(new.to_numpy((B,), np.int32), want_len)
+    got = (kept if kept_out else ws).to_numpy((B, G, budget), np.int32)
+    assert np.array_equal(got, want_kept)
+    assert np.array_equal(ds.to_numpy(s.shape, np.uint32), S.view(np.uint32))
+    assert np.array_equal(dk.to_numpy(k.shape, u), K) and np.array_equal(dv.to_numpy(v.shape, u), V)
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,G,D,block,budget,first,last", [
+    ([10, 1, 0, 64, 63], 2, 64, 16, 16, 2, 4), ([300, 40, 299], 8, 128, 256, 100, 4, 32), ([1000], 1, 128, 16, 999, 0, 0), ([1000], 3, 64, 7, 1, 0, 0), ([1000, 2], 2, 64, 32, 1, 0, 1),
+    ([500, 77], 2, 8, 64, 64, 64, 0), ([500, 77], 2, 8, 64, 64, 0, 64), ([257], 1, 256, 1, 256, 0, 255), ([2000, 1999], 2, 40, 48, 1500, 4, 100), ([5, 6], 2, 64, 16, 10, 1, 1)])
+def test_evict(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place):
+    evict_case(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place)
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_long_contexts(arena, out_of_place):
+    """More competing keys than LDS holds, and several steps of rows to close up."""
+    evict_case(arena, "float16", [12000, 10260, 9000], 2, 64, 256, 3000, 4, 500, out_of_place)
+    evict_case(arena, "float16", [30000], 1, 64, 64, 20001, 4, 0, out_of_place, scores=lambda s, r: r.random(s).astype(np.float32))
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_scores_that_are_alike_or_no_numbers(arena, out_of_place):
+    def odd(shape, rng):
+        s = rng.choice(np.array([0.0, -0.0, 1.0, -1.0, np.inf, -np.inf, np.nan, 1e-40, -1e-40], np.float32), shape)
+        return s
+    evict_case(arena, "bfloat16", [700, 90], 2, 64, 16, 80, 3, 5, out_of_place, scores=odd)
+    evict_case(arena, "bfloat16", [700, 90], 2, 64, 16, 80, 0, 0, out_of_place, scores=lambda s, r: np.zeros(s, np.float32))
+    evict_case(arena, "bfloat16", [700, 90], 2, 64, 16, 80, 0, 0, out_of_place, scores=lambda s, r: np.full(s, np.nan, np.float32))
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_leaves_sequences_with_bad_pages(arena, out_of_place):
+    evict_case(arena, "float16", [100, 100, 20, 100], 2, 64, 16, 40, 2, 8, out_of_place, bad=[(1, 3, -1), (2, 0, 1 << 20)], kept_out=False)
+
+
+def test_evict_cuts_contexts_at_their_bound(arena):
+    evict_case(arena, "float16", [100, 300], 2, 64, 16, 40, 2, 8, False, max_context=200)
+    evict_case(arena, "float16", [100, 300], 2, 64, 16, 40, 2, 8, False, max_context=40)
+
+
+def test_evict_refuses_tables_that_are_too_short_on_the_device(arena):
+    """to_tables rows of one block for a budget of three: every sequence that needs more stays as it is."""
+    typed("float16")
+    lengths, block = [60, 10], 16
+    table = np.arange(5, dtype=np.int32)
+    t = np.array([[0, 1, 2, 3], [4, -1, -1, -1]], np.int32)
+    k = np.random.default_rng(0).integers(0, 60000, (8, block, 1, 8), dtype=np.uint16)
+    s = np.random.default_rng(1).random((8, 1, block)).astype(np.float32)
+    dk, dv, ds, new, kept = arena.dev(k), arena.dev(k), arena.dev(s), arena.space(8), arena.space(2 * 48 * 4)
+    m = meta(arena, lengths, t)
+    nvr.check(L.nvr_kv_evict(dk.ptr, dv.ptr, ds.ptr, byref(m), 1, 8, block, 8, 48, 0, 0, arena.dev(np.array([[5], [6]], np.int32)).ptr, 1, new.ptr, kept.ptr, None, None))
+    assert new.to_numpy((2,), np.int32).tolist() == [-1, 10]
+    got = dk.to_numpy(k.shape, np.uint16)
+    assert np.array_equal(got[:6], k[:6]) and np.array_equal(got[6, :10], k[4, :10]) and np.array_equal(got[6, 10:], k[6, 10:]) and np.array_equal(got[7], k[7])
