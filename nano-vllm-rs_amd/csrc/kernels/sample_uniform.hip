@@ -2,11 +2,16 @@
 // (in the order of the vocabulary) whose summed weight exceeds uniform * (sum of what is left).
 //
 // With m the row's largest logit, token i has the weight w_i = exp((x_i - m) / T).  All three filters keep a prefix of the tokens in descending order (ties: ascending index), so a row's
-// answer is decided by two numbers: where the prefix ends, and the sum of its weights.  Nothing is sorted: the first launch reads the logits once and leaves, for each chunk of a row, its
-// maximum and the weights (and, for top-k, tokens) in bins of 1/24 of (x - m) / T; the second, a workgroup a row, adds the chunks' bins up, finds the bin that each filter ends in, reads the
-// chunks that have tokens there, settles the order inside the bin by a radix select over (logit, index), finds the chunk that the drawn number falls into, and walks that one.
-// A token's index is an answer that has to be right to the last bit, so weights are 64-bit numbers (exp by a polynomial of degree 10, 2e-13 off) and are summed as integers of
-// 2^-44 and less of the largest: their order, hence the atomics', changes nothing.  Tokens more than 42 T below the largest (e^-42 = 4e-19 of its weight) are left out.
+// answer is decided by two numbers: where the prefix ends, and the sum of its weights.  Nothing is sorted.  The first launch reads the logits once, a chunk of a row a workgroup, and leaves the chunk's
+// maximum, its weights (and, for top-k, tokens) in bins of 1/24 of x / T, and a list of its largest tokens.  The second, a workgroup a row, adds the chunks' bins up and finds the bin that the prefix
+// ends in.  If the lists have all tokens down to that bin and they are few (kDirect), it sorts those and is done, without the bins; else it settles the order inside the bin by a radix select over
+// (logit, index), finds the chunk that the drawn number falls into, and walks that one.
+// A token's index is an answer that has to be right to the last bit, so weights are 64-bit numbers and are summed as integers, so that the order of the atomics changes nothing: with
+// t = 24 x / T in 64 bits, a token lies in the cell of the whole number next to t and adds exp((t - cell) / 24), 0.98 to 1.02, in steps of 2^-40 to it (a polynomial of degree 5, 1e-13 off); a cell
+// counts exp(cell / 24).
+// Tokens more than 42 T below the largest (e^-42 = 4e-19 of its weight) are left out.
+// What a chunk cannot contribute is left out by one comparison a token: with top-k, whatever lies below the k-th of the chunk's maxima of 8 neighbours (there are k tokens above it), with min-p
+// alone, whatever lies below min_p of the chunk's maximum.
 #include <algorithm>
 #include "serving.h"
 #include "device_utils.h"
@@ -16,23 +21,29 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kBins = 1024, kScan = 512, kPick = 1024, kList = 3072, kRadix = 2048;
-constexpr float kPerUnit = 24.f;                                          // bins to a unit of (x - m) / T
+// (a token's place in its cell is meant with the product 24 x / T rounded, wherever it is formed)
+#pragma clang fp contract(off)
+constexpr int kBins = 1024, kPick = 1024, kList = 2048, kRadix = 2048, kNear = 1536;
+constexpr double kPerUnit = 24.;                                          // bins to a unit of x / T
+constexpr int kOne = 40;                                                  // weights inside a cell are integers of 2^-40
 
-struct ChunkNote { float max; int32_t arg; };                             // arg: first index of the maximum (greedy rows)
+// arg: first index of the maximum (greedy rows); cut: the list has every token of bins up to it (-1: there is no list); near: its length; binned: the bins are in memory (else the list has all that
+// counts); total: the weights of the bins, the chunk's maximum 1
+struct ChunkNote { float max; int32_t arg, cut, near, binned, pad; double total; };
 struct SampleParams {
     SampleArgs a;
-    int32_t V, P, chunk, bits;                                            // chunks of a row, their tokens; weights are integers of 2^-bits
+    int32_t V, P, chunk;                                                  // chunks of a row, their tokens
     ChunkNote *notes; unsigned long long *mass; unsigned int *cnt;        // [B][P], [B][P][kBins] twice
+    uint2 *near;                                                          // [B][P][kNear]: (key, index)
     bool whole;                                                           // rows in 16-byte pieces
 };
-// What a row asks for.  T of 0 (or less, or not a number, or too small to divide by): the largest logit
-struct RowAsk { float T, inv; double c; bool greedy; long long k; float p, min_p; };
+// What a row asks for.  T of 0 (or less, or not a number): the largest logit
+struct RowAsk { float T; double inv, c; bool greedy; long long k; float p, min_p; };
 __device__ __forceinline__ RowAsk row_ask(const SampleArgs &a, int row, int V) {
     RowAsk r;
     r.T = a.temperature ? a.temperature[row] : 1.f;
-    r.inv = kPerUnit / r.T;
-    r.greedy = !(r.T > 0.f) || r.inv > 1e30f;
+    r.greedy = !(r.T > 0.f);
+    r.inv = kPerUnit / (double)r.T;
     r.c = 1.4426950408889634 / (double)r.T;
     r.k = a.top_k ? a.top_k[row] : 0;
     if (r.k <= 0 || r.k >= V) r.k = 0;
@@ -42,27 +53,45 @@ __device__ __forceinline__ RowAsk row_ask(const SampleArgs &a, int row, int V) {
     r.min_p = r.min_p > 0.f ? fminf(r.min_p, 1.f) : 0.f;
     return r;
 }
-__device__ __forceinline__ float seen(float x) { return x == x ? x : -INFINITY; }        // (not a number: never chosen)
+__device__ __forceinline__ float seen(float x) { return x == x ? x + 0.f : -INFINITY; }  // (not a number: never chosen; -0 is 0)
+// t to the nearest whole number: its low bits behind 2^52 + 2^51 (|t| < 2^50; additions are four times as fast here as 64-bit rounding, conversion and scaling)
+constexpr double kWhole = 6755399441055744.0;
+__device__ __forceinline__ int low_of(double whole) { return (int)(uint32_t)__double_as_longlong(whole); }
 // 2^t for t <= 0: the series of exp(r ln 2), |r| <= 1/2
 __device__ __forceinline__ double exp2_64(double t) {
-    if (!(t > -1000.)) return 0.;
-    const double n = rint(t), r = t - n;
-    double s = 7.0549116208011233e-9;                                     // ln(2)^k / k!
-    s = fma(s, r, 1.0178086009239699e-7); s = fma(s, r, 1.3215486790144309e-6); s = fma(s, r, 1.5252733804059840e-5); s = fma(s, r, 1.5403530393381610e-4);
-    s = fma(s, r, 1.3333558146428443e-3); s = fma(s, r, 9.6181291076284771e-3); s = fma(s, r, 5.5504108664821580e-2); s = fma(s, r, 2.4022650695910071e-1);
-    s = fma(s, r, 6.9314718055994531e-1); s = fma(s, r, 1.0);
-    return ldexp(s, (int)n);
+    t = fmax(t, -1000.);
+    const double whole = t + kWhole, r = t - (whole - kWhole);
+    double s = 7.054911620801121e-9;                                      // ln(2)^k / k!
+    s = fma(s, r, 1.0178086009239696e-7); s = fma(s, r, 1.3215486790144305e-6); s = fma(s, r, 1.5252733804059838e-5); s = fma(s, r, 1.5403530393381606e-4);
+    s = fma(s, r, 1.3333558146428441e-3); s = fma(s, r, 9.618129107628477e-3); s = fma(s, r, 5.5504108664821576e-2); s = fma(s, r, 2.402265069591007e-1);
+    s = fma(s, r, 6.931471805599453e-1); s = fma(s, r, 1.0);
+    return __longlong_as_double(__double_as_longlong(s) + ((long long)low_of(whole) << 52));
 }
 __device__ __forceinline__ double weight(float x, float m, double c) { return x == m ? 1.0 : exp2_64(((double)x - (double)m) * c); }
-// bin of x below the maximum m: monotone in x; kBins - 1 and beyond: left out.  Whole numbers throughout, so bins under a chunk's maximum are a shift away from those under the row's
-__device__ __forceinline__ float cell(float x, float inv) { return floorf(x * inv); }
-__device__ __forceinline__ int bin_of(float x, float m, float inv) {
+// exp(f / 24) in steps of 2^-40, |f| <= 1/2: the series, every term 2^40 times as large, on top of 2^52: the integer is then the number's low bits
+__device__ __forceinline__ unsigned long long in_cell(double f) {
+    constexpr double one = 1099511627776.0;
+    double s = one / (120. * 24 * 24 * 24 * 24 * 24);
+    s = fma(s, f, one / (24. * 24 * 24 * 24 * 24)); s = fma(s, f, one / (6. * 24 * 24 * 24)); s = fma(s, f, one / (2. * 24 * 24)); s = fma(s, f, one / 24.);
+    s = fma(s, f, one + 4503599627370496.0);
+    return (unsigned long long)__double_as_longlong(s) & 0xfffffffffffffull;
+}
+// A maximum that nothing but its equals is near: infinite, or so large that the next number is 2^26 cells away
+__device__ __forceinline__ bool lonely(float m, double inv) { return !(fabs((double)m * inv) < 1125899906842624.); }
+// bin of x below the maximum m (kBins - 1 and beyond: left out): cells are whole numbers, so bins under a chunk's maximum are a shift away from those under the row's
+__device__ __forceinline__ int bin_of(float x, float m, double inv) {
     if (x == m) return 0;
-    const float d = cell(m, inv) - cell(x, inv);
-    return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+    if (lonely(m, inv)) return kBins - 1;
+    const double top = (double)m * inv, d = (top + kWhole) - (fmax((double)x * inv, top - 2. * kBins) + kWhole);
+    return d < (double)(kBins - 1) ? (int)d : kBins - 1;
 }
 __device__ __forceinline__ unsigned int key_of(float f) { const unsigned int u = __float_as_uint(f); return (u & 0x80000000u) ? ~u : (u | 0x80000000u); }
 __device__ __forceinline__ float of_key(unsigned int k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+// the last bin that tokens of weight min_p may lie in, and the last in which all have it: (m - x) 24 / T is less than 1 away from x's bin
+__device__ __forceinline__ void min_p_bins(float min_p, int &sure, int &last) {
+    const double e = -kPerUnit * log((double)min_p);
+    sure = (int)fmin(fmax(floor(e) - 2., -1.), (double)(kBins - 2)); last = (int)fmin(ceil(e) + 2., (double)(kBins - 2));
+}
 
 // tokens of a chunk from i on: 4 of them (those behind `end`: -inf)
 __device__ __forceinline__ float4_t four(const float *x, int i, int end, bool whole) {
@@ -75,198 +104,355 @@ __device__ __forceinline__ float4_t four(const float *x, int i, int end, bool wh
     for (int e = 0; e < 4; ++e) v[e] = seen(v[e]);
     return v;
 }
+// x of the lane that CTRL names, 0 where there is none or the row is not in ROWS (32 and 64 bits)
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T moved(T x) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+    } else {
+        const long long v = __builtin_bit_cast(long long, x);
+        const unsigned int lo = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false), hi = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (long long)(((unsigned long long)hi << 32) | lo));
+    }
+}
+template <class T>
+__device__ __forceinline__ T row_scan(T v) {                              // over the lanes of a row of 16 up to and with this one: row_shr 1, 2, 4, 8
+    v += moved<0x111, 0xf>(v); v += moved<0x112, 0xf>(v); v += moved<0x114, 0xf>(v); v += moved<0x118, 0xf>(v);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T from_lane(T x, int l) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+    else {
+        const long long v = __builtin_bit_cast(long long, x);
+        const unsigned int lo = (unsigned int)__builtin_amdgcn_readlane((int)v, l), hi = (unsigned int)__builtin_amdgcn_readlane((int)(v >> 32), l);
+        return __builtin_bit_cast(T, (long long)(((unsigned long long)hi << 32) | lo));
+    }
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {                             // ... of the wave: the rows' last lanes to the rows behind (row_bcast 15 and 31)
+    v = row_scan(v);
+    v += moved<0x142, 0xa>(v); v += moved<0x143, 0xc>(v);
+    return v;
+}
+// sum over the threads up to and with this one; `waves`: one of LDS a wave (16 at most)
+template <class T>
+__device__ __forceinline__ T scan(T v, T *waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) waves[wave] = v;
+    __syncthreads();
+    return from_lane(row_scan(lane < wave ? waves[lane & 15] : (T)0), 15) + v;
+}
+template <class T>
+__device__ __forceinline__ T wave_total(T v) { return from_lane(wave_scan(v), 63); }
 }  // namespace
 
-// A chunk of EPT tokens a thread, held in registers: its maximum, then its bins
-template <int EPT>
-__global__ __launch_bounds__(kScan) void sample_scan_kernel(SampleParams p) {
+// A chunk of EPT tokens a thread, held in registers: its maximum, its largest tokens, its bins
+template <int EPT, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p) {
     __shared__ unsigned long long mass[kBins];
     __shared__ unsigned int cnt[kBins];
-    __shared__ float wmax[kScan / 64];
-    __shared__ int warg[kScan / 64];
+    __shared__ uint2 near[kNear];
+    __shared__ double sums[THREADS / 64];
+    __shared__ float wmax[THREADS / 64];
+    __shared__ unsigned int wsum[THREADS / 64], listed;
+    __shared__ int cut, list_cut, first_at;
+    constexpr int NG = EPT / 4, BT = kBins / THREADS;                     // maxima of 4 tokens; bins of a thread
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const float *x = p.a.logits + (int64_t)row * p.a.ld;
     const int base = c * p.chunk, end = min(p.V, base + p.chunk);
+    auto index = [&](int j) { return base + ((j / 4) * THREADS + tid) * 4 + (j & 3); };
     float v[EPT];
 #pragma unroll
     for (int j = 0; j < EPT / 4; ++j) {
-        const float4_t f = four(x, base + (j * kScan + tid) * 4, end, p.whole);
+        const float4_t f = four(x, index(4 * j), end, p.whole);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e];
     }
     const RowAsk ask = row_ask(p.a, row, p.V);
-    for (int b = tid; b < kBins; b += kScan) { mass[b] = 0; cnt[b] = 0; }
-    float m = v[0];
+    for (int b = tid; b < kBins; b += THREADS) { mass[b] = 0; cnt[b] = 0; }
+    if (tid == 0) { cut = list_cut = kBins - 2; listed = 0; first_at = 0x7fffffff; }
+    float high[NG];
 #pragma unroll
-    for (int j = 1; j < EPT; ++j) m = fmaxf(m, v[j]);
+    for (int g = 0; g < NG; ++g) high[g] = fmaxf(fmaxf(v[4 * g], v[4 * g + 1]), fmaxf(v[4 * g + 2], v[4 * g + 3]));
+    float m = high[0];
+#pragma unroll
+    for (int g = 1; g < NG; ++g) m = fmaxf(m, high[g]);
     m = wave_max(m);
     if ((tid & 63) == 0) wmax[wave] = m;
     __syncthreads();
     m = wmax[0];
 #pragma unroll
-    for (int w = 1; w < kScan / 64; ++w) m = fmaxf(m, wmax[w]);
+    for (int w = 1; w < THREADS / 64; ++w) m = fmaxf(m, wmax[w]);
     ChunkNote *note = p.notes + (int64_t)row * p.P + c;
     if (ask.greedy) {
         int at = 0x7fffffff;
 #pragma unroll
-        for (int j = EPT - 1; j >= 0; --j) if (v[j] == m) at = base + ((j / 4) * kScan + tid) * 4 + (j & 3);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
-        if ((tid & 63) == 0) warg[wave] = at;
+        for (int j = EPT - 1; j >= 0; --j) if (v[j] == m) at = index(j);
+        if (at < 0x7fffffff) atomicMin(&first_at, at);
         __syncthreads();
-        if (tid == 0) {
-#pragma unroll
-            for (int w = 1; w < kScan / 64; ++w) at = min(at, warg[w]);
-            *note = ChunkNote{m, at};
-        }
+        if (tid == 0) *note = ChunkNote{m, first_at, -1, 0, 0, 0, 0.};
         return;
     }
-    if (tid == 0) *note = ChunkNote{m, 0};
-    if (m == -INFINITY) return;                                           // (nothing to choose here: the bins are not looked at)
-    const double one = ldexp(1.0, p.bits);
-    const bool counted = ask.k > 0;
+    if (m == -INFINITY) {                                                 // (nothing to choose here: the bins are not looked at)
+        if (tid == 0) *note = ChunkNote{m, 0, kBins, 0, 0, 0, 0.};
+        return;
+    }
+    const bool counted = ask.k > 0, lone = lonely(m, ask.inv), filtered = counted || ask.p < 1.f || ask.min_p > 0.f;
+    double total = 0.;                                                    // weights, the chunk's maximum 1 (of rows that top-p or nothing ends)
+    auto listing = [&](int j) {
+        const unsigned int at = atomicAdd(&listed, 1u);
+        if (at < kNear) near[at] = make_uint2(key_of(v[j]), (unsigned int)index(j));
+    };
+    int list_end = kBins, bins_end = kBins;                               // tokens of bins up to these go into the list, into the bins
+    bool binned = false;
+    if (lone) {                                                           // (only the equals of the maximum count)
 #pragma unroll
-    for (int j = 0; j < EPT; ++j) {
-        if (v[j] == -INFINITY) continue;
-        const int b = bin_of(v[j], m, ask.inv);
-        if (b >= kBins - 1) continue;
-        atomicAdd(&mass[b], (unsigned long long)(weight(v[j], m, ask.c) * one + 0.5));
-        if (counted) atomicAdd(&cnt[b], 1u);
+        for (int j = 0; j < EPT; ++j) if (v[j] == m) { listing(j); total += 1.; }
+        __syncthreads();
+        binned = listed > kNear;
+        if (binned) {
+            const int64_t at = ((int64_t)row * p.P + c) * kBins;
+            for (int b = tid; b < kBins - 1; b += THREADS) { p.mass[at + b] = b ? 0 : (unsigned long long)listed << kOne; if (counted) p.cnt[at + b] = b ? 0 : listed; }
+            list_end = -1;
+        }
+    } else if (!filtered) {
+        list_end = -1;
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) total += exp2_64(((double)v[j] - (double)m) * ask.c);
+    } else {
+        const double t_m = (double)m * ask.inv, whole_m = t_m + kWhole, lowest = t_m - 1.5 * kBins;
+        auto cell_of = [&](float x, double &f) {                          // bins below the maximum; f: the place inside the cell
+            const double t = fmax((double)x * ask.inv, lowest), whole = t + kWhole;
+            f = t - (whole - kWhole);
+            return low_of(whole_m) - low_of(whole);
+        };
+        // the bins of the k-th maximum, and of the one at the list's end: the k-th too, or, of many, three times a chunk's share of k; without top-k the 96th
+        const unsigned int want = counted ? (unsigned int)min(ask.k, 0x7fffffffll) : 96, want_list = want <= 96 ? want : max(96u, (unsigned int)min(3ll * ask.k / p.P, (long long)kNear));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) { double f; const int b = cell_of(high[g], f); if (b < kBins - 1) atomicAdd(&cnt[b], 1u); }
+        __syncthreads();
+        unsigned int own[BT], n = 0;
+#pragma unroll
+        for (int i = 0; i < BT; ++i) { own[i] = cnt[BT * tid + i]; n += own[i]; }
+        n = scan<unsigned int>(n, wsum) - n;
+#pragma unroll
+        for (int i = 0; i < BT; ++i) {
+            if (n < want && n + own[i] >= want) cut = BT * tid + i;       // (one thread)
+            if (n < want_list && n + own[i] >= want_list) list_cut = BT * tid + i;
+            n += own[i];
+            cnt[BT * tid + i] = 0;
+        }
+        __syncthreads();
+        bins_end = counted ? cut : kBins - 2;
+        if (ask.min_p > 0.f && ask.k == 0 && ask.p == 1.f) {
+            int sure, last;
+            min_p_bins(ask.min_p, sure, last);
+            bins_end = min(bins_end, last);
+        }
+        list_end = min(list_cut, bins_end);                               // (fewer maxima than wanted: all that is near, if it fits)
+        // 24 x / T of these bins is not below that of the maximum less the bins and 1; a little less, for the roundings
+        auto least_of = [&](int bins) { const float f = (float)((t_m - bins - 1.) / ask.inv); return f - fabsf(f) * 1e-6f; };
+        const float least_listed = least_of(list_end);
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) {
+            if (v[j] < least_listed) continue;
+            double f;
+            if (cell_of(v[j], f) <= list_end) listing(j);
+        }
+        __syncthreads();
+        binned = listed > kNear || list_end < bins_end;                   // (else the list has all that counts)
+        if (listed > kNear) list_end = -1;
+        if (binned || (!counted && ask.p < 1.f)) {
+            if (bins_end == kBins - 2) {                                  // all tokens: those too far below go into the last bin, which nobody reads
+#pragma unroll
+                for (int j = 0; j < EPT; ++j) {
+                    double f;
+                    const int b = min(cell_of(v[j], f), kBins - 1);
+                    atomicAdd(&mass[b], in_cell(f));
+                    if (counted) atomicAdd(&cnt[b], 1u);
+                }
+            } else {
+                const float least = least_of(bins_end);
+#pragma unroll
+                for (int j = 0; j < EPT; ++j) {
+                    if (v[j] < least) continue;
+                    double f;
+                    const int b = cell_of(v[j], f);
+                    if (b > bins_end) continue;
+                    atomicAdd(&mass[b], in_cell(f));
+                    if (counted) atomicAdd(&cnt[b], 1u);
+                }
+            }
+            __syncthreads();
+            const int64_t at = ((int64_t)row * p.P + c) * kBins;
+            const double off = t_m - (whole_m - kWhole);
+            for (int b = tid; b < kBins - 1; b += THREADS) {
+                const unsigned long long q = mass[b];
+                if (!counted && q) total += (double)q * exp2_64(-((double)b + off) * (1.4426950408889634 / kPerUnit));
+                if (binned) { p.mass[at + b] = q; if (counted) p.cnt[at + b] = cnt[b]; }
+            }
+            total *= 0x1p-40;
+        }
+    }
+    if (!counted) {
+        total = wave_total(total);
+        if ((tid & 63) == 0) sums[wave] = total;
     }
     __syncthreads();
-    const int64_t at = ((int64_t)row * p.P + c) * kBins;
-    for (int b = tid; b < kBins; b += kScan) { p.mass[at + b] = mass[b]; if (counted) p.cnt[at + b] = cnt[b]; }
+    const unsigned int n = listed;
+    if (list_end >= 0 && n <= kNear)
+        for (unsigned int i = tid; i < n; i += THREADS) p.near[((int64_t)row * p.P + c) * kNear + i] = near[i];
+    if (tid == 0) {
+        total = 0.;
+        if (!counted) for (int w = 0; w < THREADS / 64; ++w) total += sums[w];
+        *note = ChunkNote{m, 0, list_end, list_end >= 0 ? (int)n : 0, binned, 0, total};
+    }
 }
 
 namespace {
+constexpr int kDirect = 2048, kChunks = 1024, kBinned = 0x8000;
 struct PickShared {
     double cum[kBins];                                                    // weight of the bins up to and with this one
     unsigned int cum_n[kBins];
-    unsigned long long rmass[kRadix];
+    unsigned long long rmass[kRadix];                                     // (also the tokens that are sorted, and the chunks' sums)
     unsigned int rcnt[kRadix];
     unsigned int key[kList], idx[kList];
+    uint16_t near[kChunks];                                               // tokens of a chunk's list (kBinned: its bins are in memory)
+    int16_t shift[kChunks];                                               // bins that a chunk's maximum lies under the row's (kBins: nothing of it is near)
     double wsum[16];
     unsigned long long wsum64[16];
     unsigned int wcnt[16];
-    unsigned int n, nsel;
+    unsigned int n, nsel, sel_cnt;
+    unsigned int low, high;
     int sel, found;
-    unsigned int sel_cnt;
     unsigned long long sel_mass;
     double part;
 };
-template <class T>
-__device__ __forceinline__ T up(T v, int d) { return __shfl_up(v, d); }
-// sum over the threads up to and with this one; `waves`: 16 of LDS
-template <class T>
-__device__ __forceinline__ T scan(T v, T *waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const T o = up(v, d); if (lane >= d) v += o; }
-    __syncthreads();
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    T before = 0;
-    for (int w = 0; w < wave; ++w) before += waves[w];
-    return before + v;
-}
 
 struct Row {
     const SampleParams &p;
     PickShared &sh;
     const float *x;
-    int row;
+    int row, listed, from, to;                                            // from, to: the bins that gather() went over last; listed: the chunks' lists have every token of the row's bins up to it
     RowAsk ask;
     float m;
-    double one;
-    __device__ int shift(int c) const {                                   // bins of chunk c lie this far under the row's (kBins: nothing of it is near)
-        const float mc = p.notes[(int64_t)row * p.P + c].max;
-        if (mc == -INFINITY) return kBins;
-        return bin_of(mc, m, ask.inv) >= kBins - 1 ? kBins : bin_of(mc, m, ask.inv);
-    }
-    __device__ double factor(int c) const { return weight(p.notes[(int64_t)row * p.P + c].max, m, ask.c) / one; }
-    __device__ const unsigned long long *mass(int c) const { return p.mass + ((int64_t)row * p.P + c) * kBins; }
-    // f(key, index, x) for the tokens of bins lo .. hi: all threads take part
+    double off;                                                           // the maximum's place inside its cell: a cell's weight is exp(-(bins below + off) / 24)
+    __device__ __forceinline__ const ChunkNote &note(int c) const { return p.notes[(int64_t)row * p.P + c]; }
+    __device__ __forceinline__ double cell(int b) const { return exp2_64(-((double)b + off) * (1.4426950408889634 / kPerUnit)) * 0x1p-40; }      // weight of one unit of bin b
+    __device__ __forceinline__ unsigned long long inside(float v) const { if (lonely(m, ask.inv)) return 1ull << kOne; const double t = (double)v * ask.inv; return in_cell(t - ((t + kWhole) - kWhole)); }
+    // f(key, index, x, bin) for the tokens of bins lo .. hi in the chunks' lists, a wave a chunk
     template <class F>
-    __device__ void each_of_row(int lo, int hi, F f) const {
-        for (int c = 0; c < p.P; ++c) {
-            const int s = shift(c);
-            if (s > hi) continue;
-            each_of_chunk(c, lo, hi, f);
-        }
-    }
-    template <class F>
-    __device__ void each_of_chunk(int c, int lo, int hi, F f) const {
-        const int base = c * p.chunk, end = min(p.V, base + p.chunk);
-        for (int i = base + (int)threadIdx.x * 4; i < base + p.chunk; i += kPick * 4) {
-            const float4_t v = four(x, i, end, p.whole);
+    __device__ __forceinline__ void each_listed(int lo, int hi, F f) const {
+        const int lane = threadIdx.x & 63;
+        for (int c0 = threadIdx.x >> 6; c0 < p.P; c0 += kPick / 16) {     // (the first tokens of 4 chunks together)
+            uint2 first[4];
+            int n[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (v[e] == -INFINITY) continue;
-                const int b = bin_of(v[e], m, ask.inv);
-                if (b >= lo && b <= hi && b < kBins - 1) f(key_of(v[e]), (unsigned int)(i + e), v[e]);
+                const int c = c0 + e * (kPick / 64);
+                n[e] = c < p.P && sh.shift[c] <= hi ? sh.near[c] & (kBinned - 1) : 0;
+                if (lane < n[e]) first[e] = p.near[((int64_t)row * p.P + c) * kNear + lane];
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                for (int i = lane; i < n[e]; i += 64) {
+                    const uint2 k = i == lane ? first[e] : p.near[((int64_t)row * p.P + c0 + e * (kPick / 64)) * kNear + i];
+                    const float v = of_key(k.x);
+                    const int b = bin_of(v, m, ask.inv);
+                    if (b >= lo && b <= hi) f(k.x, k.y, v, b);
+                }
         }
     }
-    // the tokens of bins lo .. hi into the list; false: they are more than it holds
-    __device__ bool gather(int lo, int hi) {
+    // ... in the row itself.  Most tokens are outside: two comparisons with the bins' ends (a little beyond, for their roundings) come first
+    template <class F>
+    __device__ __forceinline__ void each_of_row(int lo, int hi, F f) const {
+        const double top = (double)m * ask.inv;
+        const float a = (float)((top - hi - 1.) / ask.inv), z = (float)((top - lo + 1.) / ask.inv);
+        const bool lone = lonely(m, ask.inv);
+        const float least = lone ? m : a - fabsf(a) * 1e-6f, most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
+        const bool all = !(least == least && most == most);               // (1 / inv beyond float)
+        for (int i0 = threadIdx.x * 4; i0 < p.V; i0 += kPick * 16) {
+            float4_t v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = four(x, i0 + u * kPick * 4, p.V, p.whole);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = v[u][e];
+                    if (w == -INFINITY || (!all && (w < least || w > most))) continue;
+                    const int b = bin_of(w, m, ask.inv);
+                    if (b >= lo && b <= hi && b < kBins - 1) f(key_of(w), (unsigned int)(i0 + u * kPick * 4 + e), w, b);
+                }
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void each(int lo, int hi, F f) const { if (hi <= listed) each_listed(lo, hi, f); else each_of_row(lo, hi, f); }
+    // the tokens of bins lo .. hi into LDS; false: they are more than it holds
+    __device__ __forceinline__ bool gather(int lo, int hi) {
+        if (lo == from && hi == to) return sh.n <= kList;                 // (they are there)
+        from = lo; to = hi;
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
-        for (int c = 0; c < p.P; ++c) {
-            const int s = shift(c);
-            if (s > hi) continue;
-            const unsigned long long *q = mass(c);
-            bool some = false;                                            // (the same for every thread)
-            for (int b = max(lo - s, 0); b <= hi - s && !some; ++b) some = q[b] != 0;
-            if (!some) continue;
-            each_of_chunk(c, lo, hi, [&](unsigned int k, unsigned int i, float) {
-                const unsigned int at = atomicAdd(&sh.n, 1u);
-                if (at < kList) { sh.key[at] = k; sh.idx[at] = i; }
-            });
-        }
+        each(lo, hi, [&](unsigned int k, unsigned int i, float, int) {
+            const unsigned int at = atomicAdd(&sh.n, 1u);
+            if (at < kList) { sh.key[at] = k; sh.idx[at] = i; }
+        });
         __syncthreads();
         return sh.n <= kList;
     }
     template <class F>
-    __device__ void each(bool listed, int lo, int hi, F f) {
-        if (listed) { for (unsigned int i = threadIdx.x; i < sh.n; i += kPick) f(sh.key[i], sh.idx[i], of_key(sh.key[i])); }
-        else each_of_row(lo, hi, f);
+    __device__ __forceinline__ void each_gathered(bool all_here, int lo, int hi, F f) const {
+        if (all_here) { for (unsigned int i = threadIdx.x; i < sh.n; i += kPick) { const float v = of_key(sh.key[i]); f(sh.key[i], sh.idx[i], v, bin_of(v, m, ask.inv)); } }
+        else each(lo, hi, f);
     }
     // Among the tokens of bin b in descending order (ties: ascending index): the last one that is kept, when `need` of them are (need > 0) or as many as it takes until `before` plus their weights
-    // reaches `goal`.  part: the weight of the kept ones
-    __device__ void settle(int b, unsigned int need, double before, double goal, unsigned int &key, unsigned int &index, double &part) {
-        const bool listed = gather(b, b);
+    // reaches `goal`.  part: the weight of the kept ones.  A radix select over 11 bits of the logit at a time, then over 11 and 11 of the index
+    __device__ __forceinline__ void settle(int b, unsigned int need, double before, double goal, unsigned int &key, unsigned int &index, double &part) {
+        const bool here = gather(b, b);
         const int tid = threadIdx.x;
-        unsigned int prefix = 0, mask = 0, left = need;
+        const double unit = cell(b);
+        unsigned int left = need, equal = 0;
         unsigned long long done = 0;                                      // weight above the prefix
-        unsigned int equal = 0;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
+        // the tokens of a bin are alike in their upper bits: those are the first prefix
+        if (tid == 0) { sh.low = 0xffffffffu; sh.high = 0; }
+        __syncthreads();
+        {
+            unsigned int low = 0xffffffffu, high = 0;
+            each_gathered(here, b, b, [&](unsigned int k, unsigned int, float, int) { low = min(low, k); high = max(high, k); });
+            if (low <= high) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
+        }
+        __syncthreads();
+        if (sh.low > sh.high) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }      // (no token: everything is kept)
+        const int bits = sh.low == sh.high ? 0 : 32 - __clz((int)(sh.low ^ sh.high));      // that differ
+        unsigned int mask = bits >= 32 ? 0 : 0xffffffffu << bits, prefix = sh.high & mask;
+        for (int at = bits;;) {
+            const int wide = 1 << min(at, 11);
+            at = max(at - 11, 0);
             for (int i = tid; i < kRadix; i += kPick) { sh.rcnt[i] = 0; sh.rmass[i] = 0; }
-            if (tid == 0) sh.found = 0x7fffffff;
+            if (tid == 0) { sh.found = 0x7fffffff; sh.sel = -1; }
             __syncthreads();
-            each(listed, b, b, [&](unsigned int k, unsigned int, float v) {
+            each_gathered(here, b, b, [&](unsigned int k, unsigned int, float v, int) {
                 if ((k & mask) != prefix) return;
                 const int d = wide - 1 - (int)((k >> at) & (wide - 1));   // descending
                 atomicAdd(&sh.rcnt[d], 1u);
-                atomicAdd(&sh.rmass[d], (unsigned long long)(weight(v, m, ask.c) * one + 0.5));
+                atomicAdd(&sh.rmass[d], inside(v));
             });
             __syncthreads();
             const unsigned int c0 = sh.rcnt[2 * tid], c1 = sh.rcnt[2 * tid + 1];
             const unsigned long long m0 = sh.rmass[2 * tid], m1 = sh.rmass[2 * tid + 1];
-            const unsigned int nc = scan<unsigned int>(c0 + c1, sh.wcnt);
-            const unsigned long long nm = scan<unsigned long long>(m0 + m1, sh.wsum64);
+            const unsigned int u1 = scan<unsigned int>(c0 + c1, sh.wcnt), u0 = u1 - c1;
+            const unsigned long long s1 = scan<unsigned long long>(m0 + m1, sh.wsum64), s0 = s1 - m1;
             // the first digit that the end falls into (or, where rounding leaves the goal unreached, the last that has tokens)
-            const unsigned int u1 = nc, u0 = nc - c1;
-            const unsigned long long s1 = nm, s0 = nm - m1;
-            auto ends = [&](unsigned int n, unsigned long long s) { return need ? n >= left : before + (double)(done + s) / one >= goal; };
+            auto ends = [&](unsigned int n, unsigned long long s) { return need ? n >= left : before + (double)(done + s) * unit >= goal; };
             if (c0 && ends(u0, s0)) atomicMin(&sh.found, 2 * tid);
             else if (c1 && ends(u1, s1)) atomicMin(&sh.found, 2 * tid + 1);
-            if (tid == 0) sh.sel = -1;
-            __syncthreads();
-            if (sh.found == 0x7fffffff) { if (c1) atomicMax(&sh.sel, 2 * tid + 1); else if (c0) atomicMax(&sh.sel, 2 * tid); }
+            if (c0 | c1) atomicMax(&sh.sel, c1 ? 2 * tid + 1 : 2 * tid);
             __syncthreads();
             const int d = sh.found != 0x7fffffff ? sh.found : sh.sel;
-            if (d < 0) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }        // (no token: everything is kept)
             if (tid == d / 2) {
                 const bool odd = d & 1;
                 sh.sel_cnt = odd ? u0 : u0 - c0; sh.sel_mass = odd ? s0 : s0 - m0;
@@ -278,29 +464,27 @@ struct Row {
             equal = sh.nsel;
             prefix |= (unsigned int)(wide - 1 - d) << at; mask |= (unsigned int)(wide - 1) << at;
             __syncthreads();
+            if (at == 0) break;
         }
         key = prefix;
-        const double w = weight(of_key(prefix), m, ask.c);
+        const double w = (double)inside(of_key(prefix)) * unit, start = before + (double)done * unit;
         unsigned int n = left;
-        const double start = before + (double)done / one;
         if (!need) {
-            const double q = w > 0. ? ceil((goal - start) / w) : 1.;
+            const double q = ceil((goal - start) / w);
             n = q >= (double)equal ? equal : q < 1. ? 1u : (unsigned int)q;
             if (n > 1 && start + (n - 1) * w >= goal) --n;
             else if (n < equal && start + n * w < goal) ++n;
         }
-        if (n < 1) n = 1;
-        if (n > equal) n = equal;
-        part = (double)done / one + n * w;
+        n = min(max(n, 1u), equal);
+        part = (double)done * unit + n * w;
         index = 0xffffffffu;
         if (n == equal) return;
-        // which of the equal ones: the n-th smallest index
-        unsigned int at_prefix = 0, at_mask = 0, want = n;
-        for (int at = 22; at >= 0; at -= 11) {
+        unsigned int at_prefix = 0, at_mask = 0, want = n;                // which of the equal ones: the n-th smallest index
+        for (int at = 11; at >= 0; at -= 11) {
             for (int i = tid; i < kRadix; i += kPick) sh.rcnt[i] = 0;
             if (tid == 0) sh.found = 0x7fffffff;
             __syncthreads();
-            each(listed, b, b, [&](unsigned int k, unsigned int i, float) { if (k == key && (i & at_mask) == at_prefix) atomicAdd(&sh.rcnt[(i >> at) & (kRadix - 1)], 1u); });
+            each_gathered(here, b, b, [&](unsigned int k, unsigned int i, float, int) { if (k == key && (i & at_mask) == at_prefix) atomicAdd(&sh.rcnt[(i >> at) & (kRadix - 1)], 1u); });
             __syncthreads();
             const unsigned int c0 = sh.rcnt[2 * tid], c1 = sh.rcnt[2 * tid + 1], nc = scan<unsigned int>(c0 + c1, sh.wcnt);
             if (c0 && nc - c1 >= want) atomicMin(&sh.found, 2 * tid);
@@ -315,6 +499,34 @@ struct Row {
         }
         index = at_prefix;
     }
+    // v[0 .. size) ascending, size a power of two of 64 .. 2 kPick.  Pairs less than 64 apart are a wave's own (its 64 pairs lie in 128 neighbours), and its LDS requests are served in order
+    __device__ __forceinline__ void sort(unsigned long long *v, int size) {
+        const int t = threadIdx.x;
+        if (size <= 128) {                                                // few: a number's place is how many are smaller
+            const unsigned long long a = t < size ? v[t] : 0;
+            int at = 0;
+            if (t < size)
+#pragma unroll 8
+                for (int j = 0; j < size; ++j) { const unsigned long long b = v[j]; at += b < a || (b == a && j < t); }
+            __syncthreads();
+            if (t < size) v[at] = a;
+            __syncthreads();
+            return;
+        }
+        for (int k = 2; k <= size; k *= 2) {
+            for (int j = k / 2; j > 0; j /= 2) {
+                if (j >= 64) __syncthreads();
+                if (t < size / 2) {
+                    const int i = 2 * t - (t & (j - 1));                  // pair (i, i + j)
+                    const unsigned long long a = v[i], b = v[i + j];
+                    if ((a > b) == ((i & k) == 0)) { v[i] = b; v[i + j] = a; }
+                }
+                if (j >= 64) __syncthreads();
+                asm volatile("" ::: "memory");
+            }
+        }
+        __syncthreads();
+    }
 };
 }  // namespace
 
@@ -322,175 +534,289 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     __shared__ PickShared sh;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const ChunkNote *notes = p.notes + (int64_t)row * p.P;
-    Row r{p, sh, p.a.logits + (int64_t)row * p.a.ld, row, row_ask(p.a, row, p.V), -INFINITY, ldexp(1.0, p.bits)};
-    for (int c = 0; c < p.P; ++c) r.m = fmaxf(r.m, notes[c].max);
-    if (r.m == -INFINITY || r.ask.greedy) {
+    Row r{p, sh, p.a.logits + (int64_t)row * p.a.ld, row, kBins - 2, -1, -1, row_ask(p.a, row, p.V), -INFINITY, 0.};
+    const RowAsk &ask = r.ask;
+    const double u = (double)p.a.uniform[row];
+    const ChunkNote mine = tid < p.P ? notes[tid] : ChunkNote{-INFINITY, 0, kBins, 0, 0, 0, 0.};      // (up to kChunks of them)
+    {
+        float *waves = reinterpret_cast<float *>(sh.wsum);
+        const float v = wave_max(mine.max);
+        if (lane == 0) waves[wave] = v;
+        if (tid == 0) sh.found = 0x7fffffff;
+        __syncthreads();
+        for (int w = 0; w < kPick / 64; ++w) r.m = fmaxf(r.m, waves[w]);
+        __syncthreads();
+    }
+    if (r.m == -INFINITY || ask.greedy) {
+        if (mine.max == r.m && r.m != -INFINITY) atomicMin(&sh.found, mine.arg);
+        __syncthreads();
         if (tid == 0) {
-            int64_t id = -1;
-            for (int c = p.P - 1; c >= 0 && r.m != -INFINITY; --c) if (notes[c].max == r.m) id = notes[c].arg;
+            const int64_t id = r.m != -INFINITY ? sh.found : -1;
             p.a.ids[row] = id;
             if (p.a.logprobs) p.a.logprobs[row] = id < 0 ? -INFINITY : 0.f;
         }
         return;
     }
-    const RowAsk &ask = r.ask;
-    // ---- the row's bins, thread b bin b
-    double mass = 0.;
-    unsigned int cnt = 0;
-    for (int c = 0; c < p.P; ++c) {
-        const int s = r.shift(c);
-        if (tid >= s && tid - s < kBins - 1 && tid < kBins - 1) {
-            mass += (double)r.mass(c)[tid - s] * r.factor(c);
-            if (ask.k) cnt += p.cnt[((int64_t)row * p.P + c) * kBins + tid - s];
-        }
-    }
-    sh.cum[tid] = scan<double>(mass, sh.wsum);
-    sh.cum_n[tid] = ask.k ? scan<unsigned int>(cnt, sh.wcnt) : 0;
-    __syncthreads();
-    // the first bin whose sum reaches a goal (kBins: none)
-    auto first_bin = [&](bool reached) {
+    if (!lonely(r.m, ask.inv)) { const double t = (double)r.m * ask.inv; r.off = t - ((t + kWhole) - kWhole); }
+    // the first thread for which something holds (kBins: none)
+    auto first_of = [&](bool holds) {
         if (tid == 0) sh.found = kBins;
         __syncthreads();
-        if (reached) atomicMin(&sh.found, tid);
+        const unsigned long long b = __ballot(holds);
+        if (lane == 0 && b) atomicMin(&sh.found, wave * 64 + __ffsll((long long)b) - 1);
         __syncthreads();
-        const int b = sh.found;
+        const int f = sh.found;
         __syncthreads();
-        return b;
+        return f;
     };
+    // ---- the chunks: where their bins lie, how far their lists reach, the row's weight
+    double everything;
+    {
+        int s = kBins, reach = kBins - 2;
+        double t = 0.;
+        if (tid < p.P && mine.max > -INFINITY) {
+            s = bin_of(mine.max, r.m, ask.inv);
+            if (s >= kBins - 1) s = kBins;
+            else { reach = mine.cut < 0 ? -1 : min(s + mine.cut, kBins - 2); t = mine.total * weight(mine.max, r.m, ask.c); }
+        }
+        if (tid < p.P) { sh.shift[tid] = (int16_t)s; sh.near[tid] = (uint16_t)(mine.near | (mine.binned ? kBinned : 0)); }
+        if (tid == 0) sh.sel = kBins - 2;
+        t = scan<double>(t, sh.wsum);
+        atomicMin(&sh.sel, reach);
+        if (tid == kPick - 1) sh.part = t;
+        __syncthreads();
+        everything = sh.part; r.listed = sh.sel;
+    }
+    const bool filtered = ask.k || ask.p < 1.f || ask.min_p > 0.f;
+    const unsigned int k = (unsigned int)ask.k;                           // (below V)
+    int p_sure = kBins - 2, p_last = kBins - 2;                           // min-p: bins that have it throughout, and in part
+    if (ask.min_p > 0.f) min_p_bins(ask.min_p, p_sure, p_last);
+    // ---- few tokens: the lists have all that may be kept, down to the bin that the first filter ends in
+    if (filtered && r.listed >= 0) {
+        unsigned long long *bin = sh.rmass;
+        unsigned int *cnt = sh.rcnt;
+        bin[tid] = 0; cnt[tid] = 0;
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        r.each_listed(0, r.listed, [&](unsigned int key, unsigned int i, float v, int b) {
+            atomicAdd(&bin[b], r.inside(v)); atomicAdd(&cnt[b], 1u);
+            const unsigned int at = atomicAdd(&sh.n, 1u);
+            if (at < kList) { sh.key[at] = key; sh.idx[at] = i; }
+        });
+        __syncthreads();
+        const bool here = sh.n <= kList;
+        const double cum = scan<double>((double)bin[tid] * r.cell(tid), sh.wsum);
+        const unsigned int cum_n = scan<unsigned int>(cnt[tid], sh.wcnt);
+        int reach = kBins;
+        if (ask.k) reach = first_of(cum_n >= k);
+        else if (ask.p < 1.f) reach = first_of(cum >= (double)ask.p * everything && cum_n > 0);
+        if (ask.min_p > 0.f && (!ask.k || ask.p == 1.f)) reach = min(reach, p_last);      // (what top-k keeps in all is wanted for top-p)
+        if (reach > r.listed && ask.k && r.listed == kBins - 2) reach = r.listed;         // (fewer tokens than top-k would keep)
+        if (tid == min(reach, kBins - 1)) sh.nsel = cum_n;
+        __syncthreads();
+        if (reach <= r.listed && sh.nsel <= kDirect && sh.nsel > 0) {
+            unsigned long long *v = sh.rmass;
+            int size = 64;
+            while (size < (int)sh.nsel) size *= 2;
+            if (tid == 0) sh.sel = 0;
+            __syncthreads();
+            auto take = [&](unsigned int key, unsigned int i, float f, int b) { if (b <= reach) v[atomicAdd(&sh.sel, 1)] = ((unsigned long long)~key << 32) | i; };
+            if (here) { for (unsigned int i = tid; i < sh.n; i += kPick) { const float f = of_key(sh.key[i]); take(sh.key[i], sh.idx[i], f, bin_of(f, r.m, ask.inv)); } }
+            else r.each_listed(0, reach, take);
+            __syncthreads();
+            const int n = sh.sel;
+            for (int i = n + tid; i < size; i += kPick) v[i] = ~0ull;
+            __syncthreads();
+            r.sort(v, size);                                              // descending logits, ascending indices
+            auto at = [&](int i) { return i < n ? v[i] : ~0ull; };
+            const unsigned long long a0 = at(2 * tid), a1 = at(2 * tid + 1);
+            const unsigned int k0 = ~(unsigned int)(a0 >> 32), k1 = ~(unsigned int)(a1 >> 32);
+            const double w0 = 2 * tid < n ? weight(of_key(k0), r.m, ask.c) : 0., w1 = 2 * tid + 1 < n ? weight(of_key(k1), r.m, ask.c) : 0.;
+            int end = ask.k ? min((int)k, n) : n;                         // ranks that are kept
+            if (ask.p < 1.f) {
+                const double v0 = 2 * tid < end ? w0 : 0., v1 = 2 * tid + 1 < end ? w1 : 0., upto = scan<double>(v0 + v1, sh.wsum);
+                if (tid == kPick - 1) sh.part = upto;
+                __syncthreads();
+                const double goal = (double)ask.p * (ask.k ? sh.part : everything);
+                const int t = first_of(2 * tid < end && upto >= goal);
+                if (tid == t) sh.nsel = upto - v1 >= goal || 2 * tid + 1 >= end ? 1 : 2;
+                __syncthreads();
+                if (t < kBins) end = min(end, 2 * t + (int)sh.nsel);
+            }
+            const bool in0 = 2 * tid < end && !(ask.min_p > 0.f && w0 < (double)ask.min_p), in1 = 2 * tid + 1 < end && !(ask.min_p > 0.f && w1 < (double)ask.min_p);
+            __syncthreads();
+            if (2 * tid < size) { v[2 * tid] = in0 ? (a0 << 32) | k0 : ~0ull; v[2 * tid + 1] = in1 ? (a1 << 32) | k1 : ~0ull; }
+            __syncthreads();
+            r.sort(v, size);                                              // the kept ones by their indices
+            const unsigned long long b0 = at(2 * tid), b1 = at(2 * tid + 1);
+            const double x0 = b0 != ~0ull ? weight(of_key((unsigned int)b0), r.m, ask.c) : 0., x1 = b1 != ~0ull ? weight(of_key((unsigned int)b1), r.m, ask.c) : 0.;
+            const double upto = scan<double>(x0 + x1, sh.wsum);
+            if (tid == kPick - 1) sh.part = upto;
+            __syncthreads();
+            const double sum = sh.part, goal = u * sum;
+            int t = first_of(x0 + x1 > 0. && upto > goal);
+            const bool beyond = t == kBins;                               // (no goal below the sum: the last one)
+            if (beyond) {
+                if (tid == 0) sh.sel = 0;
+                __syncthreads();
+                if (x0 + x1 > 0.) atomicMax(&sh.sel, tid);
+                __syncthreads();
+                t = sh.sel;
+            }
+            if (tid == t) {
+                const bool one = beyond ? !(x1 > 0.) : x0 > 0. && upto - x1 > goal;
+                p.a.ids[row] = (int64_t)((one ? b0 : b1) >> 32);
+                if (p.a.logprobs) p.a.logprobs[row] = (float)log((one ? x0 : x1) / sum);
+            }
+            return;
+        }
+        __syncthreads();
+    }
+    // ---- many: the row's bins, thread b bin b, from the chunks' or, of the chunks that left none, from their lists
     int stop = kBins;                                                     // bins in front of it are kept whole; of this one, tokens down to (key, index)
     unsigned int key = 0, index = 0xffffffffu;
-    double total = sh.cum[kBins - 1];
-    if (ask.k) {
-        const int b = first_bin(sh.cum_n[tid] >= (unsigned int)ask.k);
-        if (b < kBins) {
-            const unsigned int before = b ? sh.cum_n[b - 1] : 0;
-            const double mass_before = b ? sh.cum[b - 1] : 0.;
-            if (sh.cum_n[b] == (unsigned int)ask.k) { stop = b + 1; total = sh.cum[b]; }
-            else {
-                double part;
-                r.settle(b, (unsigned int)ask.k - before, 0., 0., key, index, part);
-                stop = b; total = mass_before + part;
+    double unit_of_bin = 0.;
+    if (filtered) {
+        sh.rmass[tid] = 0; sh.rcnt[tid] = 0;
+        __syncthreads();
+        for (int c = wave; c < p.P; c += kPick / 64) {
+            const int s = sh.shift[c];
+            if (s >= kBins || (sh.near[c] & kBinned)) continue;
+            const uint2 *q = p.near + ((int64_t)row * p.P + c) * kNear;
+            for (int i = lane; i < sh.near[c]; i += 64) {
+                const float v = of_key(q[i].x);
+                const int b = bin_of(v, r.m, ask.inv);
+                if (b < kBins - 1) { atomicAdd(&sh.rmass[b], r.inside(v)); atomicAdd(&sh.rcnt[b], 1u); }
             }
         }
-    }
-    if (ask.p < 1.f) {
-        const double goal = (double)ask.p * total;
-        const int b = first_bin(sh.cum[tid] >= goal && sh.cum[tid] > 0. && (tid < stop || (tid == stop && stop < kBins)));
-        const bool ends_there = b < kBins && !(b == stop && total < goal);
-        if (ends_there && b <= stop) {
+        __syncthreads();
+        unsigned long long in_bin = sh.rmass[tid];
+        unsigned int cnt = sh.rcnt[tid];
+        for (int c0 = 0; c0 < p.P; c0 += 8) {                             // (8 chunks' requests together)
+            unsigned long long q[8];
+            unsigned int n[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = min(c0 + e, p.P - 1), b = tid - sh.shift[c];
+                const bool in = c0 + e < p.P && b >= 0 && tid < kBins - 1 && (sh.near[c] & kBinned);
+                const int64_t at = ((int64_t)row * p.P + c) * kBins + b;
+                q[e] = in ? p.mass[at] : 0;
+                n[e] = in && ask.k ? p.cnt[at] : 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { in_bin += q[e]; cnt += n[e]; }
+        }
+        unit_of_bin = r.cell(tid);
+        sh.cum[tid] = scan<double>((double)in_bin * unit_of_bin, sh.wsum);
+        sh.cum_n[tid] = scan<unsigned int>(cnt, sh.wcnt);
+        __syncthreads();
+        double total = ask.k ? sh.cum[kBins - 1] : everything;
+        for (int filter = 0; filter < 2; ++filter) {                      // top-k, top-p
+            if (filter == 0 ? !ask.k : ask.p == 1.f) continue;
+            const double goal = filter ? (double)ask.p * total : 0.;
+            const int b = first_of(filter ? sh.cum[tid] >= goal && sh.cum[tid] > 0. && tid < stop : sh.cum_n[tid] >= k);
+            const int bin = filter && b == kBins ? stop : b;              // (the bin that top-k ended in, or none)
+            if (bin == kBins || (filter && b == kBins && key == 0 && index == 0xffffffffu)) continue;
+            const double before = bin ? sh.cum[bin - 1] : 0.;
+            if (!filter && sh.cum_n[bin] == k) { stop = bin + 1; total = sh.cum[bin]; continue; }
             unsigned int k2, i2;
             double part;
-            const double before = b ? sh.cum[b - 1] : 0.;
-            r.settle(b, 0, before, goal, k2, i2, part);
-            // (in the bin where top-k ended, its own end may come first)
-            if (b < stop || k2 > key || (k2 == key && i2 < index)) { key = k2; index = i2; }
-            stop = b;
+            r.settle(bin, filter ? 0 : k - (bin ? sh.cum_n[bin - 1] : 0), before, goal, k2, i2, part);
+            if (bin < stop || k2 > key || (k2 == key && i2 < index)) { key = k2; index = i2; }      // (in the bin where top-k ended, its own end may come first)
+            stop = bin;
+            if (!filter) total = before + part;
         }
     }
-    // ---- min-p: tokens of weight min_p and more, by bins but for those around the border
-    int sure = stop, last = stop < kBins ? stop : -1;                     // whole bins in front of `sure`; single tokens of bins sure .. last
-    bool by_key = stop < kBins && !(key == 0 && index == 0xffffffffu);
-    if (stop < kBins && !by_key) last = stop - 1;                         // (top-k ended with a whole bin: `stop` is the first one left out)
-    const int key_bin = stop;
-    if (ask.min_p > 0.f) {
-        const float edge = (float)((double)r.m + (double)ask.T * log((double)ask.min_p)), off = 1e-6f * fmaxf(fabsf(r.m), fabsf(edge));      // off: what rounding may move it by
-        const bool far = r.m == INFINITY;
-        const int lo = far ? 0 : max(bin_of(fminf(edge + off, r.m), r.m, ask.inv) - 1, 0), hi = far ? 0 : min(bin_of(edge - off, r.m, ask.inv) + 1, kBins - 2);
-        if (lo < sure) { last = by_key && key_bin <= hi ? key_bin : min(hi, sure - 1); sure = lo; }
-    }
-    auto kept = [&](int b, unsigned int k, unsigned int i, double w) {
-        if (b < sure) return true;
+    // whole bins in front of `sure`; single tokens of bins sure .. last
+    const bool by_key = stop < kBins && !(key == 0 && index == 0xffffffffu);
+    const int key_bin = stop, sure = min(stop, p_sure + 1), last = min(min(by_key ? stop : stop - 1, p_last), kBins - 2);
+    const bool cut = filtered && last >= sure;                            // (without filters all bins are whole)
+    auto kept = [&](int b, unsigned int kk, unsigned int i, double w) {
+        if (!filtered || b < sure) return true;
         if (b > last) return false;
-        if (by_key && b == key_bin && (k < key || (k == key && i > index))) return false;
+        if (by_key && b == key_bin && (kk < key || (kk == key && i > index))) return false;
         return !(ask.min_p > 0.f) || w >= (double)ask.min_p;
     };
-    // ---- what each chunk keeps: its whole bins, a wave a chunk, and its single tokens
-    double sum = 0.;                                                      // of the chunks so far
-    const double u = p.a.uniform ? (double)p.a.uniform[row] : 0.;
-    auto chunk_sum = [&](int c) {                                         // (a wave)
-        const int s = r.shift(c);
+    // ---- what each chunk keeps: its whole bins, and its single tokens in steps of 2^-40 of the heaviest there may be
+    __syncthreads();
+    double *sums = sh.cum;                                                // (of up to kChunks)
+    unsigned long long *single = reinterpret_cast<unsigned long long *>(sh.rmass);
+    const double unit = cut ? r.cell(sure) : 0.;
+    single[tid] = 0;
+    const bool here = cut && r.gather(sure, last);
+    __syncthreads();
+    if (cut)
+        r.each_gathered(here, sure, last, [&](unsigned int kk, unsigned int i, float v, int b) {
+            const double w = weight(v, r.m, ask.c);
+            if (kept(b, kk, i, w)) atomicAdd(&single[i / p.chunk], (unsigned long long)(w / unit + 0.5));
+        });
+    __syncthreads();
+    double *units = reinterpret_cast<double *>(sh.key);                   // (kList of 4 bytes: the gathered tokens have been looked at)
+    static_assert(kList * 4 >= kBins * 8, "");
+    units[tid] = unit_of_bin;
+    __syncthreads();
+    for (int c = wave; c < p.P; c += kPick / 64) {
+        const int s = sh.shift[c];
         double v = 0.;
         if (s < kBins) {
-            const unsigned long long *q = r.mass(c);
-            for (int b = lane; b < sure - s && b < kBins - 1; b += 64) v += (double)q[b];
-            v *= r.factor(c);
-            if (last >= sure && s <= last) {
-                bool some = false;
-                for (int b = max(sure - s, 0); b <= last - s && !some; ++b) some = q[b] != 0;
-                if (some) {
-                    const int base = c * p.chunk, end = min(p.V, base + p.chunk);
-                    for (int i = base + lane * 4; i < base + p.chunk; i += 256) {
-                        const float4_t f = four(r.x, i, end, p.whole);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (f[e] == -INFINITY) continue;
-                            const int b = bin_of(f[e], r.m, ask.inv);
-                            if (b < sure || b > last) continue;
-                            const double w = weight(f[e], r.m, ask.c);
-                            if (kept(b, key_of(f[e]), (unsigned int)(i + e), w)) v += w;
-                        }
-                    }
+            if (!filtered) v = lane == 0 ? notes[c].total * weight(notes[c].max, r.m, ask.c) : 0.;
+            else if (sh.near[c] & kBinned) {
+                const unsigned long long *q = p.mass + ((int64_t)row * p.P + c) * kBins;
+                for (int b = lane; b < sure - s && b < kBins - 1; b += 64) v += (double)q[b] * units[b + s];
+            } else {
+                const uint2 *q = p.near + ((int64_t)row * p.P + c) * kNear;
+                for (int i = lane; i < sh.near[c]; i += 64) {
+                    const float f = of_key(q[i].x);
+                    const int b = bin_of(f, r.m, ask.inv);
+                    if (b < sure && b < kBins - 1) v += (double)r.inside(f) * units[b];
                 }
             }
+            v = wave_total(v) + (double)single[c] * unit;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-        return v;
-    };
-    // two walks over the chunks' sums, 16 at a time: the row's sum, then the chunk that the goal falls into.  The sums of up to kList chunks stay in LDS (a row has more only beyond 12 million tokens)
-    double *sums = reinterpret_cast<double *>(sh.rmass);                  // (free by now: kRadix of them)
-    __syncthreads();
-    for (int c0 = 0; c0 < p.P; c0 += 16) {
-        const int c = c0 + wave;
-        if (c < p.P) { const double v = chunk_sum(c); if (lane == 0) sums[c] = v; }
+        if (lane == 0) sums[c] = v;
     }
     __syncthreads();
-    for (int c = 0; c < p.P; ++c) sum += sums[c];
-    const double goal = u * sum;
-    double before = 0.;
-    int at = -1;
-    {
-        double run = 0.;
-        int lastc = -1;
-        double lastb = 0.;
-        for (int c = 0; c < p.P; ++c) {
-            if (sums[c] > 0.) { lastc = c; lastb = run; }
-            if (at < 0 && run + sums[c] > goal) { at = c; before = run; }
-            run += sums[c];
-        }
-        if (at < 0) { at = lastc; before = lastb; }
+    // the chunk that the goal falls into (thread c chunk c)
+    const double own = tid < p.P ? sums[tid] : 0., upto_c = scan<double>(own, sh.wsum);
+    if (tid == kPick - 1) sh.part = upto_c;
+    if (tid == 0) sh.sel = 0;
+    __syncthreads();
+    const double sum = sh.part, goal = u * sum;
+    int c = first_of(own > 0. && upto_c > goal);
+    if (c == kBins) {
+        if (own > 0.) atomicMax(&sh.sel, tid);
+        __syncthreads();
+        c = sh.sel;
     }
-    // ---- the token of that chunk: a thread's tokens are neighbours
-    const int per = p.chunk / kPick, base = at * p.chunk, end = min(p.V, base + p.chunk);      // 4 or 16
-    double w[16];
-    double mine = 0.;
-    for (int j = 0; j < 16; j += 4) {
-        if (j >= per) break;
-        const int i = base + tid * per + j;
-        const float4_t f = four(r.x, i, end, p.whole);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            double v = 0.;
-            if (f[e] != -INFINITY) {
-                const int b = bin_of(f[e], r.m, ask.inv);
-                if (b < kBins - 1 && (b < sure || b <= last)) { v = weight(f[e], r.m, ask.c); if (!kept(b, key_of(f[e]), (unsigned int)(i + e), v)) v = 0.; }
-            }
-            w[j + e] = v; mine += v;
-        }
-    }
-    const double upto = scan<double>(mine, sh.wsum);
+    if (tid == c) sh.part = upto_c - own;
     if (tid == 0) { sh.found = 0x7fffffff; sh.sel = -1; }
     __syncthreads();
-    {
-        double run = before + upto - mine;
+    // ---- the token of that chunk: a thread's tokens are neighbours
+    const int per = p.chunk / kPick, base = c * p.chunk + tid * per, end = min(p.V, c * p.chunk + p.chunk);      // 4 or 16
+    auto of = [&](float v, int i) {
+        if (v == -INFINITY) return 0.;
+        const int b = bin_of(v, r.m, ask.inv);
+        if (b >= kBins - 1 || (filtered && b >= sure && b > last)) return 0.;
+        const double w = weight(v, r.m, ask.c);
+        return kept(b, key_of(v), (unsigned int)i, w) ? w : 0.;
+    };
+    double here_sum = 0.;
+    for (int j = 0; j < per; j += 4) {
+        const float4_t f = four(r.x, base + j, end, p.whole);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) here_sum += of(f[e], base + j + e);
+    }
+    const double upto = scan<double>(here_sum, sh.wsum);
+    double run = sh.part + (upto - here_sum);
+    if (here_sum > 0.) {
         int hit = -1, any = -1;
-        for (int j = 0; j < 16; ++j) {
-            if (j >= per) break;
-            run += w[j];
-            if (w[j] > 0.) { any = j; if (hit < 0 && run > goal) hit = j; }
+        for (int i = base; i < base + per && i < end; ++i) {
+            const double w = of(seen(r.x[i]), i);
+            run += w;
+            if (w > 0.) { any = i; if (hit < 0 && run > goal) hit = i; }
         }
-        if (hit >= 0) atomicMin(&sh.found, base + tid * per + hit);
-        if (any >= 0) atomicMax(&sh.sel, base + tid * per + any);
+        if (hit >= 0) atomicMin(&sh.found, hit);
+        if (any >= 0) atomicMax(&sh.sel, any);
     }
     __syncthreads();
     if (tid == 0) {
@@ -500,11 +826,11 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
 }
 
-static int sample_chunk(int64_t B, int64_t V) { return B * ((V + 16383) / 16384) >= 256 ? 16384 : 4096; }   // tokens of a chunk: 12 KB of bins each, so larger ones once they fill the chip
+static int sample_chunk(int64_t B, int64_t V) { return B * ((V + 16383) / 16384) >= 256 ? 16384 : 4096; }   // tokens of a chunk (12 KB of bins each, so larger ones once they fill the chip)
 size_t sample_uniform_workspace_bytes(int64_t B, int64_t V) {
     if (B <= 0 || V <= 0) return 0;
     const int64_t P = (V + sample_chunk(B, V) - 1) / sample_chunk(B, V);
-    return (size_t)(B * P) * (kBins * 12 + sizeof(ChunkNote));
+    return (size_t)(B * P) * (kBins * 12 + kNear * 8 + sizeof(ChunkNote));
 }
 int sample_uniform(const SampleArgs &a, hipStream_t s) {
     if (a.B < 0 || a.V <= 0 || a.ld < a.V) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_sample_uniform: B=%ld V=%ld, rows %ld apart", (long)a.B, (long)a.V, (long)a.ld);
@@ -514,15 +840,12 @@ int sample_uniform(const SampleArgs &a, hipStream_t s) {
     if (((uintptr_t)a.workspace & 15) != 0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_sample_uniform: the workspace is not aligned to 16 bytes");
     SampleParams p{};
     p.a = a; p.V = (int32_t)a.V; p.chunk = sample_chunk(a.B, a.V); p.P = (int32_t)((a.V + p.chunk - 1) / p.chunk);
-    int log2v = 0;
-    while ((1ll << log2v) < a.V) ++log2v;
-    p.bits = 62 - log2v;
     const int64_t n = a.B * p.P;
-    p.mass = (unsigned long long *)a.workspace; p.cnt = (unsigned int *)(p.mass + n * kBins); p.notes = (ChunkNote *)(p.cnt + n * kBins);
+    p.mass = (unsigned long long *)a.workspace; p.near = (uint2 *)(p.mass + n * kBins); p.cnt = (unsigned int *)(p.near + n * kNear); p.notes = (ChunkNote *)(p.cnt + n * kBins);
     p.whole = ((uintptr_t)a.logits & 15) == 0 && a.ld % 4 == 0;
     const dim3 grid((unsigned)p.P, (unsigned)a.B);
-    if (p.chunk == 4096) sample_scan_kernel<8><<<grid, kScan, 0, s>>>(p);
-    else sample_scan_kernel<32><<<grid, kScan, 0, s>>>(p);
+    if (p.chunk == 4096) sample_scan_kernel<8, 512><<<grid, 512, 0, s>>>(p);
+    else sample_scan_kernel<16, 1024><<<grid, 1024, 0, s>>>(p);
     sample_pick_kernel<<<dim3((unsigned)a.B), kPick, 0, s>>>(p);
     NVR_KX_LAUNCHED("sample_uniform");
     return 0;

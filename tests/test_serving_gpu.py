@@ -300,6 +300,14 @@ def test_sample_ties(arena):
         check_sample(arena, x, 0.0, 0, 1.0, 0.0, 0.5)
 
 
+def test_sample_zeros_of_either_sign_are_alike(arena):
+    x = np.zeros((2, 300), np.float32)
+    x[:, ::3] = -0.0
+    x[1, 5] = -1.0
+    for k, p in ((0, 0.4), (100, 1.0), (7, 1.0)):
+        check_sample(arena, x, 1.0, k, p, 0.0, [0.3, 0.95])
+
+
 def test_sample_flat_bins(arena):
     """Distinct logits so close together that tens of thousands fall into the bin that the prefix ends in."""
     rng = np.random.default_rng(11)
