@@ -71,191 +71,206 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
     const int g = blockIdx.x, w = blockIdx.y;                             // (kv heads of the same keys next to each other: their rows are neighbours)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
     const int G = p.a.H / p.a.KVH;
-    // ---- this share of all sequences' units, one behind the other: units u0 .. u1 - 1, the first of them number at[1] of sequence at[0].  A thread counts those of `per` sequences
-    const int per = (p.a.B + 255) / 256, b0 = threadIdx.x * per;
-    int mine = 0;
-    for (int i = 0; i < per && b0 + i < p.a.B; ++i) mine += units_of(p.a, b0 + i);
-    int upto = mine;
+    // ---- this share of all sequences' units, one behind the other: units u0 .. u1 - 1, the first of them number `unit` of sequence b
+    int b, unit, u0, u1, shares;                                          // (a share has a unit at least: the second launch counts on it)
+    auto shared_out = [&](int all) {
+        shares = min(p.shares, all);
+        if (w >= shares) return false;
+        u0 = (int)((int64_t)w * all / shares); u1 = (int)((int64_t)(w + 1) * all / shares);
+        return true;
+    };
+    if (p.a.B <= 64) {                                                    // a lane a sequence, every wave for itself
+        const int mine = lane < p.a.B ? units_of(p.a, lane) : 0;
+        int upto = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(upto, d); if (lane >= d) upto += o; }
-    if (lane == 63) sums[wave] = upto;
-    __syncthreads();
-    int all = 0;
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(upto, d); if (lane >= d) upto += o; }
+        if (!shared_out(__builtin_amdgcn_readlane(upto, 63))) return;
+        b = __ffsll((long long)__ballot(upto > u0)) - 1;
+        unit = u0 - __builtin_amdgcn_readlane(upto - mine, b);
+    } else {                                                              // a thread counts those of `per` sequences
+        const int per = (p.a.B + 255) / 256, b0 = threadIdx.x * per;
+        int mine = 0;
+        for (int i = 0; i < per && b0 + i < p.a.B; ++i) mine += units_of(p.a, b0 + i);
+        int upto = mine;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { if (i < wave) upto += sums[i]; all += sums[i]; }
-    const int shares = min(p.shares, all);                                // (each has a unit at least: the second launch counts on it)
-    if (w >= shares) return;
-    const int u0 = (int)((int64_t)w * all / shares), u1 = (int)((int64_t)(w + 1) * all / shares);
-    if (upto - mine <= u0 && u0 < upto) {
-        int u = upto - mine, i = b0;
-        for (int n; u + (n = units_of(p.a, i)) <= u0; ++i) u += n;
-        at[0] = i; at[1] = u0 - u;
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(upto, d); if (lane >= d) upto += o; }
+        if (lane == 63) sums[wave] = upto;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { if (i < wave) upto += sums[i]; all += sums[i]; }
+        if (!shared_out(all)) return;
+        if (upto - mine <= u0 && u0 < upto) {
+            int u = upto - mine, i = b0;
+            for (int n; u + (n = units_of(p.a, i)) <= u0; ++i) u += n;
+            at[0] = i; at[1] = u0 - u;
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(at[0]); unit = __builtin_amdgcn_readfirstlane(at[1]);
     }
-    __syncthreads();
-    int b = at[0], unit = at[1];
     const float scale2 = p.a.scale * kLog2e;
     const int64_t row_elems = (int64_t)p.a.KVH * D;
     const T *kc = (const T *)p.a.k + (int64_t)g * D, *vc = (const T *)p.a.v + (int64_t)g * D;
     char *img = smem + wave * I::BYTES;
     const int rl = lane / I::LPR, pl = lane % I::LPR;                     // this lane's row of a request and its piece
     for (int left = u1 - u0; left > 0; ++b, unit = 0) {
-    const int ctx = visible(p.a, b), units = (ctx + kUnit - 1) / kUnit, take = min(left, units - unit);
-    if (take <= 0) continue;                                              // (a sequence without keys)
-    left -= take;
-    const int first = unit * kUnit, last = min(ctx, first + take * kUnit);
-    if (g == 0 && threadIdx.x == 0) {
-        if (unit == 0) p.ends[2 * b] = w;
-        if (unit + take == units) p.ends[2 * b + 1] = w;
-    }
-    const int32_t *table = p.a.block_tables + (int64_t)b * p.a.max_blocks;
-    V qf[NKS];                                                            // column lm: head lm of the group (none behind the last: 0)
-    {
-        const T *q = (const T *)p.a.q + (int64_t)b * p.a.ldq + (int64_t)(g * G + min(lm, G - 1)) * D + lq * E::W;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) qf[ks] = lm < G ? load16<E>(q + ks * E::KS, p.qw) : zero16<E>();
-    }
-    // key `lane` of a tile: its page is asked for two tiles ahead, its row (< 0: not in the pool) formed one tile ahead.  Keys that are not there take another's row: their scores are -inf, their values 0
-    auto page_of = [&](int tile) {
-        const int j = min(first + tile * I::TK + (lane & (I::TK - 1)), last - 1);
-        return table[(unsigned)j / (unsigned)p.a.block_size];
-    };
-    auto rows_of = [&](int tile, int page, unsigned int &mask) {
-        const int j = first + tile * I::TK + (lane & (I::TK - 1));
-        const bool in = j < last && page >= 0 && page < p.a.num_blocks;
-        const int r = in ? page * p.a.block_size + (int)((unsigned)j % (unsigned)p.a.block_size) : -1;
-        mask = (unsigned int)__ballot(in && lane < I::TK);
-        return in ? r : mask ? __shfl(r, __ffs(mask) - 1) : -1;
-    };
-    V kx[I::NI], vx[I::NI];
-    auto request = [&](int rows) {
-#pragma unroll
-        for (int u = 0; u < I::NI; ++u) {
-            const int64_t o = (int64_t)__shfl(rows, u * I::RPI + rl) * row_elems + pl * E::W;
-            kx[u] = __builtin_nontemporal_load(reinterpret_cast<const V *>(kc + o));
-            vx[u] = __builtin_nontemporal_load(reinterpret_cast<const V *>(vc + o));
+        const int ctx = visible(p.a, b), units = (ctx + kUnit - 1) / kUnit, take = min(left, units - unit);
+        if (take <= 0) continue;                                              // (a sequence without keys)
+        left -= take;
+        const int first = unit * kUnit, last = min(ctx, first + take * kUnit);
+        if (g == 0 && threadIdx.x == 0) {
+            if (unit == 0) p.ends[2 * b] = w;
+            if (unit + take == units) p.ends[2 * b + 1] = w;
         }
-    };
-    const int tiles = (last - first + I::TK - 1) / I::TK;
-    float m = -INFINITY, l = 0.f;
-    float4_t o[DT];
+        const int32_t *table = p.a.block_tables + (int64_t)b * p.a.max_blocks;
+        V qf[NKS];                                                            // column lm: head lm of the group (none behind the last: 0)
+        {
+            const T *q = (const T *)p.a.q + (int64_t)b * p.a.ldq + (int64_t)(g * G + min(lm, G - 1)) * D + lq * E::W;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    constexpr unsigned int kAll = I::TK == 32 ? 0xffffffffu : 0xffffu;
-    char *vimg = img + I::KB;
-    float *sp = p.s + ((int64_t)b * p.a.H + g * G + lm) * p.lpad;
-    unsigned int mask = 0;
-    int page = 0;
-    if (wave < tiles) {
-        page = page_of(wave);
-        const int rows = rows_of(wave, page, mask);
-        page = page_of(wave + 4);
-        if (mask) request(rows);
-    }
-    constexpr int SW = I::LPR >= 16 ? 15 : I::LPR - 1;                    // K: piece c of row r at slot c ^ (r & SW)
-    for (int x = wave; x < tiles; x += 4) {
-        const int j0 = first + x * I::TK;
-        const unsigned int here = mask;
-        if (here) {
-            if (here != kAll)
-#pragma unroll
-                for (int u = 0; u < I::NI; ++u) if (!((here >> (u * I::RPI + rl)) & 1)) vx[u] = zero16<E>();
-#pragma unroll
-            for (int u = 0; u < I::NI; ++u) { const int r = u * I::RPI + rl; *reinterpret_cast<V *>(img + r * I::ROW + ((pl ^ (r & SW)) << 4)) = kx[u]; }
-#pragma unroll
-            for (int u = 0; u < I::NI; ++u) *reinterpret_cast<V *>(vimg + (u * I::RPI + rl) * I::VS + pl * 16) = vx[u];
+            for (int ks = 0; ks < NKS; ++ks) qf[ks] = lm < G ? load16<E>(q + ks * E::KS, p.qw) : zero16<E>();
         }
-        asm volatile("" ::: "memory");                                    // (a wave's LDS requests are served in order)
-        mask = 0;
-        if (x + 4 < tiles) {
-            const int rows = rows_of(x + 4, page, mask);
-            page = page_of(x + 8);
+        // key `lane` of a tile: its page is asked for two tiles ahead, its row (< 0: not in the pool) formed one tile ahead.  Keys that are not there take another's row: their scores are -inf, their values 0
+        auto page_of = [&](int tile) {
+            const int j = min(first + tile * I::TK + (lane & (I::TK - 1)), last - 1);
+            return table[(unsigned)j / (unsigned)p.a.block_size];
+        };
+        auto rows_of = [&](int tile, int page, unsigned int &mask) {
+            const int j = first + tile * I::TK + (lane & (I::TK - 1));
+            const bool in = j < last && page >= 0 && page < p.a.num_blocks;
+            const int r = in ? page * p.a.block_size + (int)((unsigned)j % (unsigned)p.a.block_size) : -1;
+            mask = (unsigned int)__ballot(in && lane < I::TK);
+            return in ? r : mask ? __shfl(r, __ffs(mask) - 1) : -1;
+        };
+        V kx[I::NI], vx[I::NI];
+        auto request = [&](int rows) {
+#pragma unroll
+            for (int u = 0; u < I::NI; ++u) {
+                const int64_t o = (int64_t)__shfl(rows, u * I::RPI + rl) * row_elems + pl * E::W;
+                kx[u] = __builtin_nontemporal_load(reinterpret_cast<const V *>(kc + o));
+                vx[u] = __builtin_nontemporal_load(reinterpret_cast<const V *>(vc + o));
+            }
+        };
+        const int tiles = (last - first + I::TK - 1) / I::TK;
+        float m = -INFINITY, l = 0.f;
+        float4_t o[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
+        constexpr unsigned int kAll = I::TK == 32 ? 0xffffffffu : 0xffffu;
+        char *vimg = img + I::KB;
+        float *sp = p.s + ((int64_t)b * p.a.H + g * G + lm) * p.lpad;
+        unsigned int mask = 0;
+        int page = 0;
+        if (wave < tiles) {
+            page = page_of(wave);
+            const int rows = rows_of(wave, page, mask);
+            page = page_of(wave + 4);
             if (mask) request(rows);
         }
-        if (!here) {                                                      // (no page of the tile is in the pool)
+        constexpr int SW = I::LPR >= 16 ? 15 : I::LPR - 1;                    // K: piece c of row r at slot c ^ (r & SW)
+        for (int x = wave; x < tiles; x += 4) {
+            const int j0 = first + x * I::TK;
+            const unsigned int here = mask;
+            if (here) {
+                if (here != kAll)
+#pragma unroll
+                    for (int u = 0; u < I::NI; ++u) if (!((here >> (u * I::RPI + rl)) & 1)) vx[u] = zero16<E>();
+#pragma unroll
+                for (int u = 0; u < I::NI; ++u) { const int r = u * I::RPI + rl; *reinterpret_cast<V *>(img + r * I::ROW + ((pl ^ (r & SW)) << 4)) = kx[u]; }
+#pragma unroll
+                for (int u = 0; u < I::NI; ++u) *reinterpret_cast<V *>(vimg + (u * I::RPI + rl) * I::VS + pl * 16) = vx[u];
+            }
+            asm volatile("" ::: "memory");                                    // (a wave's LDS requests are served in order)
+            mask = 0;
+            if (x + 4 < tiles) {
+                const int rows = rows_of(x + 4, page, mask);
+                page = page_of(x + 8);
+                if (mask) request(rows);
+            }
+            if (!here) {                                                      // (no page of the tile is in the pool)
+                if (lm < G)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t *>(sp + j0 + t * 16 + lq * 4) = (float4_t){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                continue;
+            }
+            float4_t s[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                s[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) s[t] = E::mma(*reinterpret_cast<const V *>(img + (t * 16 + lm) * I::ROW + (((ks * 4 + lq) ^ (lm & SW)) << 4)), qf[ks], s[t]);
+            }
+            float mx = -INFINITY;                                             // scores of head lm: keys j0 + 16 t + 4 lq + e
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[t][e] = ((here >> (t * 16 + lq * 4 + e)) & 1) ? s[t][e] * scale2 : -INFINITY;
+                    mx = fmaxf(mx, s[t][e]);
+                }
             if (lm < G)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t *>(sp + j0 + t * 16 + lq * 4) = (float4_t){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            continue;
-        }
-        float4_t s[MT];
+                for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t *>(sp + j0 + t * 16 + lq * 4) = s[t];
+            mx = xor32_partner_max(xor16_partner_max(mx));
+            const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ms);
+            const bool moved = mn != m;
+            m = mn;
+            float rs = 0.f;
+            V ph, pm;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            s[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) s[t] = E::mma(*reinterpret_cast<const V *>(img + (t * 16 + lm) * I::ROW + (((ks * 4 + lq) ^ (lm & SW)) << 4)), qf[ks], s[t]);
-        }
-        float mx = -INFINITY;                                             // scores of head lm: keys j0 + 16 t + 4 lq + e
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(s[t][e] - ms);
+                    rs += w;
+                    ph[t * 4 + e] = (T)w;
+                    if constexpr (!F) pm[t * 4 + e] = (T)(w - (float)ph[t * 4 + e]);
+                }
+            l = fmaf(l, alpha, rs);
+            if (__any(moved)) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] = ((here >> (t * 16 + lq * 4 + e)) & 1) ? s[t][e] * scale2 : -INFINITY;
-                mx = fmaxf(mx, s[t][e]);
+                for (int t = 0; t < DT; ++t) o[t] *= alpha;
             }
-        if (lm < G)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t *>(sp + j0 + t * 16 + lq * 4) = s[t];
-        mx = xor32_partner_max(xor16_partner_max(mx));
-        const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ms);
-        const bool moved = mn != m;
-        m = mn;
-        float rs = 0.f;
-        V ph, pm;
+            for (int t = 0; t < DT; ++t) {
+                V a;
+                if constexpr (F) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(s[t][e] - ms);
-                rs += w;
-                ph[t * 4 + e] = (T)w;
-                if constexpr (!F) pm[t * 4 + e] = (T)(w - (float)ph[t * 4 + e]);
+                    for (int e = 0; e < 4; ++e) a[e] = *reinterpret_cast<const float *>(vimg + (lq * 4 + e) * I::VS + (t * 16 + lm) * 4);
+                } else {
+                    const char *at = vimg + (lq * 4 + (lm >> 2)) * I::VS + t * 32 + (lm & 3) * 8;
+                    a = transposed<E>(at, at + 16 * I::VS);
+                }
+                o[t] = E::mma(a, ph, o[t]);
+                if constexpr (!F) o[t] = E::mma(a, pm, o[t]);
             }
-        l = fmaf(l, alpha, rs);
-        if (__any(moved)) {
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] *= alpha;
+            asm volatile("" ::: "memory");
         }
+        // ---- the waves' sums
+        l = xor32_partner_sum(xor16_partner_sum(l));
+        __syncthreads();
+        float *so = reinterpret_cast<float *>(smem);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            V a;
-            if constexpr (F) {
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<float4_t *>(so + (wave * 16 + lm) * I::OS + t * 16 + lq * 4) = o[t];
+        if (lq == 0) { ml[wave][lm][0] = m; ml[wave][lm][1] = l; }
+        __syncthreads();
+        for (int i = threadIdx.x; i < G * (D / 4); i += 256) {
+            const int h = i / (D / 4), c = (i % (D / 4)) * 4;
+            float M = ml[0][h][0], L = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = *reinterpret_cast<const float *>(vimg + (lq * 4 + e) * I::VS + (t * 16 + lm) * 4);
-            } else {
-                const char *at = vimg + (lq * 4 + (lm >> 2)) * I::VS + t * 32 + (lm & 3) * 8;
-                a = transposed<E>(at, at + 16 * I::VS);
+            for (int i = 1; i < 4; ++i) M = fmaxf(M, ml[i][h][0]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = __builtin_amdgcn_exp2f(ml[i][h][0] - Ms);
+                v += *reinterpret_cast<const float4_t *>(so + (i * 16 + h) * I::OS + c) * f;
+                L = fmaf(ml[i][h][1], f, L);
             }
-            o[t] = E::mma(a, ph, o[t]);
-            if constexpr (!F) o[t] = E::mma(a, pm, o[t]);
+            const int64_t to = (int64_t)(w + b) * p.a.H + g * G + h;
+            *reinterpret_cast<float4_t *>(p.o + to * D + c) = v;
+            if (c == 0) { p.ml[2 * to] = M; p.ml[2 * to + 1] = L; }
         }
-        asm volatile("" ::: "memory");
-    }
-    // ---- the waves' sums
-    l = xor32_partner_sum(xor16_partner_sum(l));
-    __syncthreads();
-    float *so = reinterpret_cast<float *>(smem);
-#pragma unroll
-    for (int t = 0; t < DT; ++t) *reinterpret_cast<float4_t *>(so + (wave * 16 + lm) * I::OS + t * 16 + lq * 4) = o[t];
-    if (lq == 0) { ml[wave][lm][0] = m; ml[wave][lm][1] = l; }
-    __syncthreads();
-    for (int i = threadIdx.x; i < G * (D / 4); i += 256) {
-        const int h = i / (D / 4), c = (i % (D / 4)) * 4;
-        float M = ml[0][h][0], L = 0.f;
-#pragma unroll
-        for (int i = 1; i < 4; ++i) M = fmaxf(M, ml[i][h][0]);
-        const float Ms = M == -INFINITY ? 0.f : M;
-        float4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float f = __builtin_amdgcn_exp2f(ml[i][h][0] - Ms);
-            v += *reinterpret_cast<const float4_t *>(so + (i * 16 + h) * I::OS + c) * f;
-            L = fmaf(ml[i][h][1], f, L);
-        }
-        const int64_t to = (int64_t)(w + b) * p.a.H + g * G + h;
-        *reinterpret_cast<float4_t *>(p.o + to * D + c) = v;
-        if (c == 0) { p.ml[2 * to] = M; p.ml[2 * to + 1] = L; }
-    }
-    if (left > 0) __syncthreads();
+        if (left > 0) __syncthreads();
     }
 }
 
