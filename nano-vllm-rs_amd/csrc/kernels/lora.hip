@@ -1,11 +1,12 @@
 // lora.hip — low-rank adapters of many requests beside a shared projection: y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T, a = the adapter of row t's request.
 //
-// Two products of inner sizes K and R, on the matrix cores, over TILES: up to 16 or 64 rows that share an adapter, wherever they stand in the step (up to 256 rows every workgroup finds its tile
+// Two products of inner sizes K and R, on the matrix cores, over TILES: up to 16 or 64 rows that share an adapter, wherever they stand in the step (up to 64 rows every wave finds its tile
 // itself; more are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
 //   down: v = scale x A^T, the waves of a workgroup (and `splits` workgroups of few rows) share K; partial sums stay in 32 bits in the workspace, [split][row][rank]
 //   up:   y = base + v B^T; v in two 16-bit numbers (its rounding and the rounded rest), so that the product sees it in 16 (bfloat16) or 22 bits; the sum with base is rounded once
 // Both are bound by memory for prompts (x, base and y once; 2 R flops a byte) and by their two launches for decode steps.
 #include <algorithm>
+#include <type_traits>
 #include "serving.h"
 #include "elem.h"
 #include "../common.h"
@@ -13,7 +14,7 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kSmall = 256;                                               // rows up to which a workgroup finds its tile itself
+constexpr int kSmall = 64;                                                // rows up to which a workgroup finds its tile itself
 constexpr int kMaxAdapters = 8192;                                        // counters of the grouping launch (LDS)
 
 struct LoraTile { int32_t start, count, adapter; };                       // rows order[start ..) of one adapter; adapter n: rows without one
@@ -36,39 +37,26 @@ __device__ __forceinline__ int range_of(unsigned int most) {
     return most == 0 || e == 128 ? 0 : min(max(13 - e, -100), 100);
 }
 
-// rows of tile `tile` (rows[0 .. count), LDS) and its adapter; count 0: no such tile.  256 threads, T <= 256, tiles of 16 rows: row t is number rank(t) of its adapter's rows, the rows of rank 0, 16,
-// .. lead a tile, tiles go by their leaders.
-__device__ __forceinline__ int tile_of_small(const LoraParams &p, int tile, int *rows, int *ids, int *note, int &adapter) {
-    const int t = threadIdx.x, T = (int)p.a.T;
-    const int id = t < T ? adapter_of(p, t) : -1;
-    ids[t] = id;
-    if (t < 2) note[t] = 0;
-    __syncthreads();
+// rows of tile `tile` (rows[0 .. count), LDS) and its adapter; count 0: no such tile.  T <= 64, tiles of 16 rows: row t is number rank(t) of its adapter's rows, the rows of rank 0, 16, .. lead a tile,
+// tiles go by their leaders.  Every wave for itself, a lane a row (all write the same)
+__device__ __forceinline__ int tile_of_small(const LoraParams &p, int tile, int *rows, int &adapter) {
+    const int lane = threadIdx.x & 63, id = lane < (int)p.a.T ? adapter_of(p, lane) : -1;
     int rank = 0;
-    const int4 *v = reinterpret_cast<const int4 *>(ids);
-    for (int j = 0; j < (T + 3) / 4; ++j) {
-        const int4 o = v[j];
-        rank += (o.x == id && 4 * j < t) + (o.y == id && 4 * j + 1 < t) + (o.z == id && 4 * j + 2 < t) + (o.w == id && 4 * j + 3 < t);
-    }
-    const bool lead = id >= 0 && (rank & 15) == 0;
-    const unsigned long long b = __ballot(lead);
-    int *per_wave = note + 4;
-    if ((t & 63) == 0) per_wave[t >> 6] = __popcll(b);
-    __syncthreads();
-    int before = __popcll(b & ((1ull << (t & 63)) - 1));
-    for (int w = 0; w < t >> 6; ++w) before += per_wave[w];
-    if (lead && before == tile) { note[0] = 1; note[2] = id; note[3] = rank; }
-    __syncthreads();
-    if (!note[0]) return 0;
-    adapter = note[2];
-    const int first = note[3];
-    if (id == adapter && rank >= first && rank < first + 16) { rows[rank - first] = t; atomicAdd(&note[1], 1); }
-    __syncthreads();
-    return note[1];
+    for (int j0 = 0; j0 < (int)p.a.T; j0 += 8)
+#pragma unroll
+        for (int j = j0; j < j0 + 8; ++j) rank += __builtin_amdgcn_readlane(id, j) == id && j < lane;      // (T <= 64: j < 64)
+    const unsigned long long leads = __ballot(id >= 0 && (rank & 15) == 0);
+    const unsigned long long mine = __ballot(((leads >> lane) & 1) && __popcll(leads & ((1ull << lane) - 1)) == tile);
+    if (!mine) return 0;
+    const int leader = __ffsll((long long)mine) - 1, first = __builtin_amdgcn_readlane(rank, leader);
+    adapter = __builtin_amdgcn_readlane(id, leader);
+    const bool in = id == adapter && rank >= first && rank < first + 16;
+    if (in) rows[rank - first] = lane;
+    return __popcll(__ballot(in));
 }
 template <int TR, bool GROUPED>
-__device__ __forceinline__ int tile_rows(const LoraParams &p, int tile, int *rows, int *ids, int *note, int &adapter) {
-    if constexpr (!GROUPED) return tile_of_small(p, tile, rows, ids, note, adapter);
+__device__ __forceinline__ int tile_rows(const LoraParams &p, int tile, int *rows, int &adapter) {
+    if constexpr (!GROUPED) return tile_of_small(p, tile, rows, adapter);
     if (tile >= *p.num_tiles) return 0;
     const LoraTile d = p.tiles[tile];
     adapter = d.adapter;
@@ -78,7 +66,7 @@ __device__ __forceinline__ int tile_rows(const LoraParams &p, int tile, int *row
 }
 }  // namespace
 
-// The rows of more than 256, adapter by adapter (their order inside one is of no consequence: a row's sums are its own), and the tiles they make.
+// More than 64 rows, adapter by adapter (their order inside one is of no consequence: a row's sums are its own), and the tiles they make.
 __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p, int tr, int32_t *order, LoraTile *tiles, int32_t *num_tiles) {
     extern __shared__ int32_t count[];                                    // [n + 1] rows of an adapter, then where its next row goes
     __shared__ int32_t sum_rows[16], sum_tiles[16], base_rows, base_tiles;
@@ -100,7 +88,18 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p, int tr, 
         return at;
     };
     const int64_t T = p.a.T;
-    for (int64_t c = 0; c < T; c += 1024) add(c + tid < T ? adapter_of(p, c + tid) : -1);
+    int id[8];                                                            // (8 rows a thread are asked for together, and kept where there are no more)
+    auto ask = [&](int64_t c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) id[e] = c + e * 1024 + tid < T ? p.a.ids[c + e * 1024 + tid] : -1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) id[e] = id[e] >= 0 && id[e] < (int)p.a.n ? id[e] : p.copies && c + e * 1024 + tid < T ? (int)p.a.n : -1;
+    };
+    for (int64_t c = 0; c < T; c += 8192) {
+        ask(c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) add(id[e]);
+    }
     __syncthreads();
     for (int c = 0; c < n; c += 1024) {                                   // exclusive sums of rows and tiles over the adapters
         const int i = c + tid, rows = i < n ? count[i] : 0, mine = (rows + tr - 1) / tr;
@@ -124,98 +123,117 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p, int tr, 
         __syncthreads();
     }
     if (tid == 0) *num_tiles = base_tiles;
-    for (int64_t c = 0; c < T; c += 1024) {
-        const int id = c + tid < T ? adapter_of(p, c + tid) : -1;
-        const int at = add(id);
-        if (id >= 0) order[at] = (int32_t)(c + tid);
+    for (int64_t c = 0; c < T; c += 8192) {
+        if (T > 8192) ask(c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int at = add(id[e]);
+            if (id[e] >= 0) order[at] = (int32_t)(c + e * 1024 + tid);
+        }
     }
 }
 
-// D(rank x row) = A . x^T: a lane's 4 sums are neighbours in v.  The waves take the steps of KS columns in turn; U steps are requested together.
-template <class E, int MT, int RT, bool GROUPED>
-__global__ __launch_bounds__(256) void lora_down_kernel(LoraParams p) {
+// Rows come from memory 128 bytes at a time, 8 rows a request, and pass through the wave's own LDS image into the layout of the operands (straight into that layout a request would be 16 rows of 64 bytes,
+// and each of its 64 lanes an address of its own: 26 GB/s a CU).
+template <class E>
+struct Strip {
+    static constexpr int CK = 128 / (int)sizeof(typename E::T), STEPS = CK / E::KS;      // numbers of a strip of a row, steps of the product in it
+    // piece c (16 bytes) of row r, in an image of 128-byte rows
+    static __device__ __forceinline__ int place(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+};
+
+// D(rank x row) = A . x^T: a lane's 4 sums are neighbours in v.  The waves of a workgroup take the strips of its share of K in turn; the next one is on its way.
+template <class E, int MT, int RT, bool GROUPED, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
     typedef typename E::T T; typedef typename E::V V;
-    constexpr int TR = MT * 16, U = MT == 1 ? 4 : 2;
-    __shared__ __attribute__((aligned(16))) int ids[GROUPED ? 4 : kSmall];
-    __shared__ int rows[TR], note[8];
-    __shared__ float4_t part[2][MT * RT][64];
+    typedef Strip<E> S;
+    constexpr int TR = MT * 16, XN = MT * 2, AN = RT * 2, IMAGE = (MT + RT) * 16 * 128;
+    __shared__ int rows[TR];
+    __shared__ __attribute__((aligned(16))) char smem[WAVES * IMAGE];     // (then the waves' sums)
     int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, ids, note, adapter);
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, adapter);
     if (!count || adapter >= (int)p.a.n) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4, lr = lane >> 3, lp = lane & 7;
     const int K = (int)p.a.K, R = (int)p.a.R, r0 = blockIdx.z * RT * 16;
-    const int steps = (K + E::KS - 1) / E::KS, per = (steps + p.splits - 1) / p.splits, first = blockIdx.y * per, last = min(steps, first + per);
-    const T *x[MT], *w[RT];
+    const int strips = (K + S::CK - 1) / S::CK, per = (strips + p.splits - 1) / p.splits, first = blockIdx.y * per, last = min(strips, first + per);
+    const T *x[XN], *w[AN];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) { const int t = m * 16 + lm; x[m] = (const T *)p.a.x + (int64_t)rows[t < count ? t : 0] * p.a.ldx; }
+    for (int u = 0; u < XN; ++u) { const int t = u * 8 + lr; x[u] = (const T *)p.a.x + (int64_t)rows[t < count ? t : 0] * p.a.ldx + lp * E::W; }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) w[r] = (const T *)p.a.A + ((int64_t)adapter * R + min(r0 + r * 16 + lm, R - 1)) * K;
+    for (int u = 0; u < AN; ++u) w[u] = (const T *)p.a.A + ((int64_t)adapter * R + min(r0 + u * 8 + lr, R - 1)) * K + lp * E::W;
+    char *xi = smem + wave * IMAGE, *ai = xi + MT * 16 * 128;
+    V xv[XN], wv[AN];
+    const bool aligned = p.xw && p.aw;
+    auto request = [&](int s) {
+        const int k = s * S::CK, n = K - k - lp * E::W;                   // numbers of the row from this lane's piece on
+        if (aligned && k + S::CK <= K) {
+#pragma unroll
+            for (int u = 0; u < XN; ++u) xv[u] = *reinterpret_cast<const V *>(x[u] + k);
+#pragma unroll
+            for (int u = 0; u < AN; ++u) wv[u] = *reinterpret_cast<const V *>(w[u] + k);
+        } else {
+#pragma unroll
+            for (int u = 0; u < XN; ++u) xv[u] = n > 0 ? load16<E>(x[u] + k, p.xw, n) : zero16<E>();
+#pragma unroll
+            for (int u = 0; u < AN; ++u) wv[u] = n > 0 ? load16<E>(w[u] + k, p.aw, n) : zero16<E>();
+        }
+    };
     float4_t acc[MT][RT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    int s = first + wave;
-    if (p.xw && p.aw)                                                     // whole steps: requests without a test
-        for (const int whole = min(last, K / E::KS); s + 4 * (U - 1) < whole; s += 4 * U) {
-            V xv[U][MT], wv[U][RT];
+    if (first + wave < last) request(first + wave);
+    for (int s = first + wave; s < last; s += WAVES) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = (s + 4 * u) * E::KS + lq * E::W;
+        for (int u = 0; u < XN; ++u) *reinterpret_cast<V *>(xi + S::place(u * 8 + lr, lp)) = xv[u];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) xv[u][m] = *reinterpret_cast<const V *>(x[m] + k);
+        for (int u = 0; u < AN; ++u) *reinterpret_cast<V *>(ai + S::place(u * 8 + lr, lp)) = wv[u];
+        asm volatile("" ::: "memory");                                    // (a wave's LDS requests are served in order)
+        if (s + WAVES < last) request(s + WAVES);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) wv[u][r] = *reinterpret_cast<const V *>(w[r] + k);
-            }
+        for (int st = 0; st < S::STEPS; ++st) {
+            V xf[MT], wf[RT];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int m = 0; m < MT; ++m) xf[m] = *reinterpret_cast<const V *>(xi + S::place(m * 16 + lm, st * 4 + lq));
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+            for (int r = 0; r < RT; ++r) wf[r] = *reinterpret_cast<const V *>(ai + S::place(r * 16 + lm, st * 4 + lq));
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[m][r] = E::mma(wv[u][r], xv[u][m], acc[m][r]);
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[m][r] = E::mma(wf[r], xf[m], acc[m][r]);
         }
-    for (; s < last; s += 4) {
-        const int k = s * E::KS + lq * E::W, n = K - k;                   // numbers of the row from k on (0 or fewer: this lane's part is behind the row)
-        V xv[MT], wv[RT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) xv[m] = n > 0 ? load16<E>(x[m] + k, p.xw, n) : zero16<E>();
-#pragma unroll
-        for (int r = 0; r < RT; ++r) wv[r] = n > 0 ? load16<E>(w[r] + k, p.aw, n) : zero16<E>();
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[m][r] = E::mma(wv[r], xv[m], acc[m][r]);
+        asm volatile("" ::: "memory");
     }
-    // the waves' sums in a fixed order: (0 + 2) + (1 + 3)
-    if (wave >= 2)
-#pragma unroll
-        for (int i = 0; i < MT * RT; ++i) part[wave - 2][i][lane] = acc[i / RT][i % RT];
+    // the waves' sums, one behind the other
+    static_assert(MT * RT * 1024 <= IMAGE, "");
     __syncthreads();
-    if (wave < 2)
+    float4_t *part = reinterpret_cast<float4_t *>(smem);                  // [wave][tile][lane]
 #pragma unroll
-        for (int i = 0; i < MT * RT; ++i) part[wave][i][lane] = acc[i / RT][i % RT] + part[wave][i][lane];
+    for (int i = 0; i < MT * RT; ++i) part[(wave * MT * RT + i) * 64 + lane] = acc[i / RT][i % RT];
     __syncthreads();
     const float scale = p.a.scales ? p.a.scales[adapter] : 1.f;
-    for (int i = wave; i < MT * RT; i += 4) {
+    for (int i = wave; i < MT * RT; i += WAVES) {
         const int m = i / RT, r = i % RT, t = m * 16 + lm;
-        const float4_t v = part[0][i][lane] + part[1][i][lane];
+        float4_t v = part[i * 64 + lane];
+#pragma unroll
+        for (int o = 1; o < WAVES; ++o) v += part[(o * MT * RT + i) * 64 + lane];
         if (t < count && r0 + r * 16 < p.rp) *reinterpret_cast<float4_t *>(p.v + ((int64_t)blockIdx.y * p.a.T + rows[t]) * p.rp + r0 + r * 16 + lq * 4) = v * scale;
     }
 }
 
-// D(column x row) = B . v^T: a lane's NT * 4 = W sums are neighbours in y (row m of tile i of B is column (m / 4) W + 4 i + m % 4 of the group).  A wave takes groups of NT * 16 columns.
+// D(column x row) = B . v^T: a lane's NT * 4 = W sums are neighbours in y (row m of tile i of B is column (m / 4) W + 4 i + m % 4 of the group).  A wave takes groups of NT * 16 columns, two at a time,
+// straight from and to memory: rows of 64 bytes a request, but no wait between.  (Through images as above, requests of whole rows: 93 -> 171 us for 8192 rows of 12288 columns of rank 32.)
 template <class E, int MT, bool GROUPED>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p, int groups) {
+__global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParams p, int groups) {
     typedef typename E::T T; typedef typename E::V V;
     constexpr int TR = MT * 16, W = E::W, NT = W / 4, GN = NT * 16;
-    constexpr bool F = sizeof(T) == 4;
-    constexpr bool H = __is_same(E, F16);
+    constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
     extern __shared__ __attribute__((aligned(16))) char smem[];           // v: [hi, lo] [TR][ldv]; 32 bits: [TR][ldv]
     __shared__ unsigned int high[TR];                                     // float16: bits of a row's largest |v|
-    __shared__ __attribute__((aligned(16))) int ids[GROUPED ? 4 : kSmall];
-    __shared__ int rows[TR], note[8];
+    __shared__ int rows[TR];
     int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, ids, note, adapter);
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, adapter);
     if (!count) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
     const int R = (int)p.a.R, N = (int)p.a.N, ks = (R + E::KS - 1) / E::KS, ldv = ks * E::KS + W;    // (a row's stride is 16 bytes off a multiple of 64: neighbours lie in other banks)
@@ -232,7 +250,15 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p, int groups) 
             v[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
             if (i < TR * per && t < count && r < p.rp) {
                 const float *at = p.v + (int64_t)rows[t] * p.rp + r;
-                for (int s = 0; s < p.splits; ++s, at += p.a.T * p.rp) v[n] += *reinterpret_cast<const float4_t *>(at);
+                const int64_t next = p.a.T * p.rp;
+                int s = 0;
+                for (; s + 4 <= p.splits; s += 4, at += 4 * next) {
+                    float4_t q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const float4_t *>(at + e * next);
+                    v[n] += (q[0] + q[1]) + (q[2] + q[3]);
+                }
+                for (; s < p.splits; ++s, at += next) v[n] += *reinterpret_cast<const float4_t *>(at);
             }
             float most = 0.f;
 #pragma unroll
@@ -268,58 +294,91 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p, int groups) 
         back[m] = H && real ? __uint_as_float((unsigned)(127 - range_of(high[t])) << 23) : 1.f;
     }
     const T *B = (const T *)p.a.B + (int64_t)adapter * N * R;
-    for (int g = (blockIdx.x * 4 + wave) * groups, end = g + groups; g < end; ++g) {
-        const int64_t n0 = (int64_t)g * GN;
-        if (n0 >= N) return;
-        const int left = (int)min((int64_t)W, N - n0 - at0);              // columns of this lane that there are
-        V b[MT];
+    // NB neighbouring groups at a time; whole: all their columns are there, everything in aligned pieces of 16 bytes
+    auto go = [&](int64_t n0, auto nb, auto whole) {
+        constexpr int NB = decltype(nb)::value;
+        constexpr bool WH = decltype(whole)::value;
+        V b[NB][MT];
+        int left[NB];                                                     // columns of this lane that there are
 #pragma unroll
-        for (int m = 0; m < MT; ++m) b[m] = left > 0 ? load16<E>((const T *)p.a.base + row[m] * p.a.ldb + n0 + at0, p.yw, left) : zero16<E>();
-        float4_t acc[NT][MT];
+        for (int q = 0; q < NB; ++q) {
+            left[q] = WH ? W : (int)max((int64_t)0, min((int64_t)W, N - n0 - q * GN - at0));
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+            for (int m = 0; m < MT; ++m) {
+                const T *at = (const T *)p.a.base + row[m] * p.a.ldb + n0 + q * GN + at0;
+                b[q][m] = WH ? *reinterpret_cast<const V *>(at) : left[q] > 0 ? load16<E>(at, p.yw, left[q]) : zero16<E>();
+            }
+        }
+        float4_t acc[NB][NT][MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[i][m] = (float4_t){0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[q][i][m] = (float4_t){0.f, 0.f, 0.f, 0.f};
         if (real) {
-            const T *bp[NT];
+            const T *bp[NB][NT];
 #pragma unroll
-            for (int i = 0; i < NT; ++i) bp[i] = B + min(n0 + (lm >> 2) * W + 4 * i + (lm & 3), (int64_t)N - 1) * R;
+            for (int q = 0; q < NB; ++q)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const int64_t n = n0 + q * GN + (lm >> 2) * W + 4 * i + (lm & 3);
+                    bp[q][i] = B + (WH ? n : min(n, (int64_t)N - 1)) * R;
+                }
             for (int k = 0; k < ks; ++k) {
                 const int r = k * E::KS + lq * W, n = R - r;
-                V bv[NT];
+                V bv[NB][NT];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) bv[i] = n >= W && p.bw ? *reinterpret_cast<const V *>(bp[i] + r) : n > 0 ? load16<E>(bp[i] + r, false, n) : zero16<E>();
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) bv[q][i] = n >= W && (WH || p.bw) ? *reinterpret_cast<const V *>(bp[q][i] + r) : !WH && n > 0 ? load16<E>(bp[q][i] + r, false, n) : zero16<E>();
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     const V vh = *reinterpret_cast<const V *>(hi + (m * 16 + lm) * ldv + r);
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) acc[i][m] = E::mma(bv[i], vh, acc[i][m]);
+                    for (int q = 0; q < NB; ++q)
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) acc[q][i][m] = E::mma(bv[q][i], vh, acc[q][i][m]);
                     if constexpr (!F) {
                         const V vl = *reinterpret_cast<const V *>(lo + (m * 16 + lm) * ldv + r);
 #pragma unroll
-                        for (int i = 0; i < NT; ++i) acc[i][m] = E::mma(bv[i], vl, acc[i][m]);
+                        for (int q = 0; q < NB; ++q)
+#pragma unroll
+                            for (int i = 0; i < NT; ++i) acc[q][i][m] = E::mma(bv[q][i], vl, acc[q][i][m]);
                     }
                 }
             }
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (m * 16 + lm >= count || left <= 0) continue;
-            V o;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int e = 0; e < W; ++e) o[e] = real ? (T)(H ? fmaf(acc[e / 4][m][e % 4], back[m], (float)b[m][e]) : (float)b[m][e] + acc[e / 4][m][e % 4]) : b[m][e];
-            T *y = (T *)p.a.y + row[m] * p.a.ldy + n0 + at0;
-            if (left == W && p.yw) *reinterpret_cast<V *>(y) = o;
-            else
+            for (int q = 0; q < NB; ++q) {
+                if (m * 16 + lm >= count || left[q] <= 0) continue;
+                V o;
 #pragma unroll
-                for (int e = 0; e < W; ++e) if (e < left) y[e] = o[e];
-        }
+                for (int e = 0; e < W; ++e) {
+                    const float v = acc[q][e / 4][m][e % 4], x = (float)b[q][m][e];
+                    o[e] = real ? (T)(H ? fmaf(v, back[m], x) : x + v) : b[q][m][e];
+                }
+                T *y = (T *)p.a.y + row[m] * p.a.ldy + n0 + q * GN + at0;
+                if (WH || (left[q] == W && p.yw)) *reinterpret_cast<V *>(y) = o;
+                else
+#pragma unroll
+                    for (int e = 0; e < W; ++e) if (e < left[q]) y[e] = o[e];
+            }
+    };
+    const bool aligned = p.yw && p.bw;
+    for (int g = (blockIdx.x * 4 + wave) * groups, end = g + groups; g < end;) {
+        const int64_t n0 = (int64_t)g * GN;
+        if (n0 >= N) return;
+        if (aligned && g + 2 <= end && n0 + 2 * GN <= N) { go(n0, std::integral_constant<int, 2>(), std::true_type()); g += 2; }
+        else if (aligned && n0 + GN <= N) { go(n0, std::integral_constant<int, 1>(), std::true_type()); ++g; }
+        else { go(n0, std::integral_constant<int, 1>(), std::false_type()); ++g; }
     }
 }
 
-static int lora_splits_most(int64_t T, int64_t K) {                       // (a wave has two steps at least; the sums of many rows are long enough without)
-    const int64_t steps = (K + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(T <= kSmall ? 16 : 4, steps / 8));
+static int lora_splits_most(int64_t T, int64_t K) {                       // (a wave has a strip of 64 at least)
+    return (int)std::max<int64_t>(1, std::min<int64_t>(4, K / 512));
 }
 static int64_t lora_rp(int64_t R) { return (R + 15) / 16 * 16; }
 size_t lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R) {
@@ -332,9 +391,9 @@ template <class E, int MT, bool GROUPED>
 static void lora_launch(const LoraParams &p, int64_t tiles, hipStream_t s) {
     const int rt = (int)(p.rp / 16);
     const unsigned t = (unsigned)tiles, z = (unsigned)p.splits;
-    if (rt == 1) lora_down_kernel<E, MT, 1, GROUPED><<<dim3(t, z, 1), 256, 0, s>>>(p);
-    else if (rt == 2) lora_down_kernel<E, MT, 2, GROUPED><<<dim3(t, z, 1), 256, 0, s>>>(p);
-    else lora_down_kernel<E, MT, 4, GROUPED><<<dim3(t, z, (rt + 3) / 4), 256, 0, s>>>(p);
+    constexpr int WAVES = MT == 4 ? 4 : 8;                                // tiles of 16 rows: more waves of a workgroup share K, and v has fewer shares to add up again
+    if (rt == 1) lora_down_kernel<E, MT, 1, GROUPED, WAVES><<<dim3(t, z, 1), WAVES * 64, 0, s>>>(p);
+    else lora_down_kernel<E, MT, 2, GROUPED, WAVES><<<dim3(t, z, (rt + 1) / 2), WAVES * 64, 0, s>>>(p);
     constexpr int GN = E::W / 4 * 16;
     const int64_t all = (p.a.N + GN - 1) / GN;                            // groups of columns: a wave takes 1 to 4, as long as there are workgroups for two rounds of the chip
     int groups = 4;
@@ -355,8 +414,8 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
     const int64_t kinds = std::min<int64_t>(a.n + p.copies, a.T);
     const int tr = a.T > kSmall && a.T >= 32 * kinds && a.R <= 128 ? 64 : 16;   // (up: 64 rows of v in LDS, 34 KB at rank 128)
     const int64_t tiles = std::min<int64_t>(a.T, a.T / tr + kinds);
-    const int64_t zs = (p.rp / 16 + 3) / 4;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(lora_splits_most(a.T, a.K), (512 + tiles * zs - 1) / (tiles * zs)));
+    const int64_t zs = (p.rp / 16 + 1) / 2;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(lora_splits_most(a.T, a.K), ((tr == 64 ? 512 : 256) + tiles * zs - 1) / (tiles * zs)));
     p.v = (float *)a.workspace;
     if (a.T > kSmall) {
         char *at = (char *)a.workspace + (size_t)a.T * lora_splits_most(a.T, a.K) * p.rp * 4;
