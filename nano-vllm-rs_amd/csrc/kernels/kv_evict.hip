@@ -12,7 +12,7 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kPick = 1024, kHeld = 10240, kRadix = 2048;
+constexpr int kPick = 1024, kHeld = 9216, kRadix = 2048;
 struct EvictParams {
     EvictArgs a;
     int32_t *kept;                                                        // [B][KVH][budget]
@@ -39,11 +39,11 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 }  // namespace
 
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
-    __shared__ unsigned int held[kHeld], hist[kRadix];
-    __shared__ unsigned int waves[16];
+    __shared__ __attribute__((aligned(16))) float held[kHeld];            // scores of keys 0 .. kHeld - 1
+    __shared__ unsigned int hist[3][kRadix];
+    __shared__ unsigned int waves[3][16], above[3];
     __shared__ unsigned long long waves2[16];
-    __shared__ int found;
-    __shared__ unsigned int above;
+    __shared__ int found[3];
     const EvictArgs &a = p.a;
     const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = length_of(a, b), n = min(len, a.budget);
@@ -54,6 +54,9 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     for (int i = tid; i < (len + a.block_size - 1) / a.block_size; i += kPick) bad |= table[i] < 0 || table[i] >= a.num_blocks;
     if (a.to_tables && !bad)
         for (int i = tid; i < (n + a.block_size - 1) / a.block_size; i += kPick) bad |= to[i] < 0 || to[i] >= a.num_blocks;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+        for (int i = tid; i < kRadix; i += kPick) hist[q][i] = 0;
     if (__syncthreads_or(bad)) {
         if (g == 0 && tid == 0) a.new_lens[b] = -1;
         for (int i = tid; i < a.budget; i += kPick) kept[i] = -1;
@@ -61,73 +64,96 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     }
     if (g == 0 && tid == 0) a.new_lens[b] = n;
     for (int i = n + tid; i < a.budget; i += kPick) kept[i] = -1;
-    if (len <= a.budget) {
+    const bool all = len <= a.budget;
+    if (all && !a.to_tables) {                                            // (nothing moves)
         for (int i = tid; i < n; i += kPick) kept[i] = i;
-    } else {
-        const int first = a.first, end = len - a.last, count = end - first;        // the keys that compete
-        unsigned int need = a.budget - a.first - a.last;                  // < count
-        auto load = [&](int i) { return rank_of(a.scores[score_at(a, table, g, first + i)]); };
-        for (int i = tid; i < min(count, kHeld); i += kPick) held[i] = load(i);
-        auto rank = [&](int i) { return i < kHeld ? held[i] : load(i); };
-        unsigned int prefix = 0, mask = 0, want = need;
-        if (need) {
-            for (int pass = 0; pass < 3; ++pass) {
-                const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
-                for (int i = tid; i < kRadix; i += kPick) hist[i] = 0;
-                if (tid == 0) found = kRadix;
-                __syncthreads();
-                for (int i = tid; i < count; i += kPick) { const unsigned int k = rank(i); if ((k & mask) == prefix) atomicAdd(&hist[wide - 1 - ((k >> at) & (wide - 1))], 1u); }
-                __syncthreads();
-                const unsigned int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-                unsigned int v = c0 + c1;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) { const unsigned int o = __shfl_up(v, d); if (lane >= d) v += o; }
-                if (lane == 63) waves[wave] = v;
-                __syncthreads();
-                for (int w = 0; w < wave; ++w) v += waves[w];
-                if (c0 && v - c1 >= want) atomicMin(&found, 2 * tid);
-                else if (c1 && v >= want) atomicMin(&found, 2 * tid + 1);
-                __syncthreads();
-                if (tid == found / 2) above = (found & 1) ? v - c1 : v - c1 - c0;
-                __syncthreads();
-                prefix |= (unsigned int)(wide - 1 - found) << at; mask |= (unsigned int)(wide - 1) << at;
-                want -= above;
-                __syncthreads();
-            }
-        } else { prefix = 0xffffffffu; __syncthreads(); }
-        // want of the keys with rank `prefix`, the earliest, and all above it.  A thread's run of keys: its counts of both, and where they begin
-        const int per = (count + kPick - 1) / kPick, i0 = min(count, tid * per), i1 = min(count, i0 + per);
-        unsigned int more = 0, same = 0;
-        for (int i = i0; i < i1; ++i) { const unsigned int k = rank(i); more += need && k > prefix; same += need && k == prefix; }
-        unsigned long long v = ((unsigned long long)more << 32) | same;
-        const unsigned long long own = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const unsigned long long o = __shfl_up(v, d); if (lane >= d) v += o; }
-        if (lane == 63) waves2[wave] = v;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) v += waves2[w];
-        v -= own;
-        unsigned int seen = (unsigned int)v, at = first + (unsigned int)(v >> 32) + min(seen, want);
-        for (int i = i0; i < i1; ++i) {
-            const unsigned int k = rank(i);
-            const bool tie = need && k == prefix;
-            if ((need && k > prefix) || (tie && seen < want)) kept[at++] = first + i;
-            seen += tie;
-        }
-        for (int i = tid; i < a.first; i += kPick) kept[i] = i;
-        for (int i = tid; i < a.last; i += kPick) kept[a.budget - a.last + i] = end + i;
+        return;
     }
-    if (!a.to_tables && len <= a.budget) return;
+    // ---- the scores into LDS, 4 neighbours a thread where blocks are multiples of 4
+    const int here = min(len, kHeld);
+    if (a.block_size % 4 == 0 && ((uintptr_t)a.scores & 15) == 0) {
+        for (int i0 = tid * 4; i0 < here; i0 += kPick * 8) {
+            float4_t v[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) { const int i = i0 + u * kPick * 4; if (i < here) v[u] = *reinterpret_cast<const float4_t *>(a.scores + score_at(a, table, g, i)); }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) { const int i = i0 + u * kPick * 4; if (i < here) *reinterpret_cast<float4_t *>(held + i) = v[u]; }
+        }
+    } else
+        for (int i = tid; i < here; i += kPick) held[i] = a.scores[score_at(a, table, g, i)];
+    __syncthreads();
+    auto score = [&](int i) { return i < kHeld ? held[i] : a.scores[score_at(a, table, g, i)]; };
+    // ---- the rank of the last of the best: the `need` best of keys first .. end - 1, of equal ones the earliest `want`
+    const int first = a.first, end = len - a.last;
+    const unsigned int need = all ? 0 : a.budget - a.first - a.last;      // (fewer than compete)
+    unsigned int prefix = 0xffffffffu, want = 0;
+    if (need) {
+        unsigned int mask = 0;
+        prefix = 0; want = need;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
+            for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass][wide - 1 - ((k >> at) & (wide - 1))], 1u); }
+            __syncthreads();
+            const unsigned int c0 = hist[pass][2 * tid], c1 = hist[pass][2 * tid + 1];
+            unsigned int v = c0 + c1;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const unsigned int o = __shfl_up(v, d); if (lane >= d) v += o; }
+            if (lane == 63) waves[pass][wave] = v;
+            __syncthreads();
+            unsigned int before = lane < wave ? waves[pass][lane & 15] : 0;
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) before += __shfl_xor(before, d);
+            v += __builtin_amdgcn_readlane(before, 0) - c0 - c1;          // in front of this thread's two digits
+            if (v < want && v + c0 + c1 >= want) {                        // (one thread)
+                const bool odd = v + c0 < want;
+                found[pass] = 2 * tid + odd; above[pass] = odd ? v + c0 : v;
+            }
+            __syncthreads();
+            prefix |= (unsigned int)(wide - 1 - found[pass]) << at; mask |= (unsigned int)(wide - 1) << at;
+            want -= above[pass];
+        }
+    }
+    // ---- a thread's run of keys: how many of them are kept, and where they begin
+    const int per = (len + kPick - 1) / kPick, i0 = min(len, tid * per), i1 = min(len, i0 + per);
+    unsigned int more = 0, same = 0;
+    for (int i = i0; i < i1; ++i) {
+        const bool always = all || i < first || i >= end;
+        const unsigned int k = always ? 0 : rank_of(score(i));
+        more += always || (need && k > prefix); same += !always && need && k == prefix;
+    }
+    unsigned long long v = ((unsigned long long)more << 32) | same;
+    const unsigned long long own = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const unsigned long long o = __shfl_up(v, d); if (lane >= d) v += o; }
+    if (lane == 63) waves2[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) v += waves2[w];
+    v -= own;
+    // the scores at their new places: at once where LDS has them all
+    const bool together = len <= kHeld;
+    unsigned int seen = (unsigned int)v, at = (unsigned int)(v >> 32) + min(seen, want);
+    for (int i = i0; i < i1; ++i) {
+        const bool always = all || i < first || i >= end;
+        const float f = score(i);
+        const unsigned int k = always ? 0 : rank_of(f);
+        const bool tie = !always && need && k == prefix;
+        if (always || (need && k > prefix) || (tie && seen < want)) {
+            kept[at] = i;
+            if (together) a.scores[score_at(a, to, g, (int)at)] = f;
+            ++at;
+        }
+        seen += tie;
+    }
+    if (together) return;
     __threadfence_block();
     __syncthreads();
-    // the scores, from the front: of a step all are read before any is written
-    for (int i0 = 0; i0 < n; i0 += kPick) {
-        const int i = i0 + tid;
-        float s = 0.f;
-        if (i < n) s = a.scores[score_at(a, table, g, kept[i])];
-        asm volatile("" : "+v"(s));
+    for (int j0 = 0; j0 < n; j0 += kPick) {                               // from the front: of a step all are read before any is written
+        const int i = j0 + tid;
+        float f = 0.f;
+        if (i < n) f = a.scores[score_at(a, table, g, kept[i])];
+        asm volatile("" : "+v"(f));
         __syncthreads();
-        if (i < n) a.scores[score_at(a, to, g, i)] = s;
+        if (i < n) a.scores[score_at(a, to, g, i)] = f;
     }
 }
 
