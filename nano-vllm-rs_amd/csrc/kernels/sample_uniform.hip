@@ -27,8 +27,8 @@ constexpr int kBins = 1024, kPick = 1024, kList = 2048, kRadix = 2048, kNear = 1
 constexpr double kPerUnit = 24.;                                          // bins to a unit of x / T
 constexpr int kOne = 40;                                                  // weights inside a cell are integers of 2^-40
 
-// arg: first index of the maximum (greedy rows); cut: the list has every token of bins up to it (-1: there is no list); near: its length; binned: the bins are in memory (else the list has all that
-// counts); total: the weights of the bins, the chunk's maximum 1
+// arg: first index of the maximum (greedy rows); cut: the list has every token of bins up to it (-1: there is no list); near: its length; binned: how many bins are in memory, the others are empty (0: the list
+// has all that counts); total: the weights of the bins, the chunk's maximum 1
 struct ChunkNote { float max; int32_t arg, cut, near, binned, pad; double total; };
 struct SampleParams {
     SampleArgs a;
@@ -145,6 +145,14 @@ __device__ __forceinline__ T scan(T v, T *waves) {
     __syncthreads();
     return from_lane(row_scan(lane < wave ? waves[lane & 15] : (T)0), 15) + v;
 }
+// x where every lane has the same: in scalar registers (what comes out of LDS the compiler takes for different ones, and branches on it for a branch a lane)
+template <class T>
+__device__ __forceinline__ T same(T x) { return from_lane(x, 0); }
+__device__ __forceinline__ unsigned int wave_largest(unsigned int v) {
+    v = max(v, moved<0x111, 0xf>(v)); v = max(v, moved<0x112, 0xf>(v)); v = max(v, moved<0x114, 0xf>(v)); v = max(v, moved<0x118, 0xf>(v));
+    v = max(v, moved<0x142, 0xa>(v)); v = max(v, moved<0x143, 0xc>(v));
+    return from_lane(v, 63);
+}
 template <class T>
 __device__ __forceinline__ T wave_total(T v) { return from_lane(wave_scan(v), 63); }
 }  // namespace
@@ -159,6 +167,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
     __shared__ float wmax[THREADS / 64];
     __shared__ unsigned int wsum[THREADS / 64], listed;
     __shared__ int cut, list_cut, first_at;
+    __shared__ unsigned int bins_used;
     constexpr int NG = EPT / 4, BT = kBins / THREADS;                     // maxima of 4 tokens; bins of a thread
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const float *x = p.a.logits + (int64_t)row * p.a.ld;
@@ -173,7 +182,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
     }
     const RowAsk ask = row_ask(p.a, row, p.V);
     for (int b = tid; b < kBins; b += THREADS) { mass[b] = 0; cnt[b] = 0; }
-    if (tid == 0) { cut = list_cut = kBins - 2; listed = 0; first_at = 0x7fffffff; }
+    if (tid == 0) { cut = list_cut = kBins - 2; listed = 0; first_at = 0x7fffffff; bins_used = 0; }
     float high[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) high[g] = fmaxf(fmaxf(v[4 * g], v[4 * g + 1]), fmaxf(v[4 * g + 2], v[4 * g + 3]));
@@ -207,16 +216,15 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
         if (at < kNear) near[at] = make_uint2(key_of(v[j]), (unsigned int)index(j));
     };
     int list_end = kBins, bins_end = kBins;                               // tokens of bins up to these go into the list, into the bins
-    bool binned = false;
+    int binned = 0;
     if (lone) {                                                           // (only the equals of the maximum count)
 #pragma unroll
         for (int j = 0; j < EPT; ++j) if (v[j] == m) { listing(j); total += 1.; }
         __syncthreads();
-        binned = listed > kNear;
-        if (binned) {
+        if (listed > kNear) {
             const int64_t at = ((int64_t)row * p.P + c) * kBins;
-            for (int b = tid; b < kBins - 1; b += THREADS) { p.mass[at + b] = b ? 0 : (unsigned long long)listed << kOne; if (counted) p.cnt[at + b] = b ? 0 : listed; }
-            list_end = -1;
+            if (tid == 0) { p.mass[at] = (unsigned long long)listed << kOne; if (counted) p.cnt[at] = listed; }
+            binned = 1; list_end = -1;
         }
     } else if (!filtered) {
         list_end = -1;
@@ -263,9 +271,9 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
             if (cell_of(v[j], f) <= list_end) listing(j);
         }
         __syncthreads();
-        binned = listed > kNear || list_end < bins_end;                   // (else the list has all that counts)
+        const bool bins = listed > kNear || list_end < bins_end;          // (else the list has all that counts)
         if (listed > kNear) list_end = -1;
-        if (binned || (!counted && ask.p < 1.f)) {
+        if (bins || (!counted && ask.p < 1.f)) {
             if (bins_end == kBins - 2) {                                  // all tokens: those too far below go into the last bin, which nobody reads
 #pragma unroll
                 for (int j = 0; j < EPT; ++j) {
@@ -289,11 +297,15 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
             __syncthreads();
             const int64_t at = ((int64_t)row * p.P + c) * kBins;
             const double off = t_m - (whole_m - kWhole);
+            unsigned int used = 0;
             for (int b = tid; b < kBins - 1; b += THREADS) {
                 const unsigned long long q = mass[b];
+                if (q) used = b + 1;
                 if (!counted && q) total += (double)q * exp2_64(-((double)b + off) * (1.4426950408889634 / kPerUnit));
-                if (binned) { p.mass[at + b] = q; if (counted) p.cnt[at + b] = cnt[b]; }
+                if (bins) { p.mass[at + b] = q; if (counted) p.cnt[at + b] = cnt[b]; }
             }
+            used = wave_largest(used);
+            if (bins && (tid & 63) == 0) atomicMax(&bins_used, used);
             total *= 0x1p-40;
         }
     }
@@ -308,19 +320,19 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
     if (tid == 0) {
         total = 0.;
         if (!counted) for (int w = 0; w < THREADS / 64; ++w) total += sums[w];
-        *note = ChunkNote{m, 0, list_end, list_end >= 0 ? (int)n : 0, binned, 0, total};
+        *note = ChunkNote{m, 0, list_end, list_end >= 0 ? (int)n : 0, binned ? binned : (int)bins_used, 0, total};
     }
 }
 
 namespace {
-constexpr int kDirect = 2048, kChunks = 1024, kBinned = 0x8000;
+constexpr int kDirect = 2048, kChunks = 1024;
 struct PickShared {
     double cum[kBins];                                                    // weight of the bins up to and with this one
     unsigned int cum_n[kBins];
     unsigned long long rmass[kRadix];                                     // (also the tokens that are sorted, and the chunks' sums)
     unsigned int rcnt[kRadix];
     unsigned int key[kList], idx[kList];
-    uint16_t near[kChunks];                                               // tokens of a chunk's list (kBinned: its bins are in memory)
+    uint16_t near[kChunks], binned[kChunks];                              // tokens of a chunk's list, its bins in memory
     int16_t shift[kChunks];                                               // bins that a chunk's maximum lies under the row's (kBins: nothing of it is near)
     double wsum[16];
     unsigned long long wsum64[16];
@@ -353,7 +365,7 @@ struct Row {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = c0 + e * (kPick / 64);
-                n[e] = c < p.P && sh.shift[c] <= hi ? sh.near[c] & (kBinned - 1) : 0;
+                n[e] = c < p.P && sh.shift[c] <= hi ? sh.near[c] : 0;
                 if (lane < n[e]) first[e] = p.near[((int64_t)row * p.P + c) * kNear + lane];
             }
 #pragma unroll
@@ -378,15 +390,18 @@ struct Row {
             float4_t v[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) v[u] = four(x, i0 + u * kPick * 4, p.V, p.whole);
+            unsigned int near = 0;                                        // the few that may be meant, one a lane at a time: a wave comes here as often as its busiest lane
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int e = 0; e < 16; ++e) { const float w = v[e >> 2][e & 3]; near |= (w != -INFINITY && (all || (w >= least && w <= most)) ? 1u : 0u) << e; }
+            while (near) {
+                const int j = __ffs((int)near) - 1;
+                near &= near - 1;
+                float w = v[0][0];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = v[u][e];
-                    if (w == -INFINITY || (!all && (w < least || w > most))) continue;
-                    const int b = bin_of(w, m, ask.inv);
-                    if (b >= lo && b <= hi && b < kBins - 1) f(key_of(w), (unsigned int)(i0 + u * kPick * 4 + e), w, b);
-                }
+                for (int n = 1; n < 16; ++n) w = j == n ? v[n >> 2][n & 3] : w;
+                const int b = bin_of(w, m, ask.inv);
+                if (b >= lo && b <= hi && b < kBins - 1) f(key_of(w), (unsigned int)(i0 + (j >> 2) * kPick * 4 + (j & 3)), w, b);
+            }
         }
     }
     template <class F>
@@ -402,7 +417,7 @@ struct Row {
             if (at < kList) { sh.key[at] = k; sh.idx[at] = i; }
         });
         __syncthreads();
-        return sh.n <= kList;
+        return same(sh.n) <= kList;
     }
     template <class F>
     __device__ __forceinline__ void each_gathered(bool all_here, int lo, int hi, F f) const {
@@ -423,12 +438,13 @@ struct Row {
         {
             unsigned int low = 0xffffffffu, high = 0;
             each_gathered(here, b, b, [&](unsigned int k, unsigned int, float, int) { low = min(low, k); high = max(high, k); });
-            if (low <= high) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
+            low = ~wave_largest(~low); high = wave_largest(high);
+            if ((tid & 63) == 0) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
         }
         __syncthreads();
-        if (sh.low > sh.high) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }      // (no token: everything is kept)
-        const int bits = sh.low == sh.high ? 0 : 32 - __clz((int)(sh.low ^ sh.high));      // that differ
-        unsigned int mask = bits >= 32 ? 0 : 0xffffffffu << bits, prefix = sh.high & mask;
+        if (same(sh.low) > same(sh.high)) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }      // (no token: everything is kept)
+        const int bits = same(sh.low == sh.high ? 0 : 32 - __clz((int)(sh.low ^ sh.high)));      // that differ
+        unsigned int mask = bits >= 32 ? 0 : 0xffffffffu << bits, prefix = same(sh.high) & mask;
         for (int at = bits;;) {
             const int wide = 1 << min(at, 11);
             at = max(at - 11, 0);
@@ -450,18 +466,21 @@ struct Row {
             auto ends = [&](unsigned int n, unsigned long long s) { return need ? n >= left : before + (double)(done + s) * unit >= goal; };
             if (c0 && ends(u0, s0)) atomicMin(&sh.found, 2 * tid);
             else if (c1 && ends(u1, s1)) atomicMin(&sh.found, 2 * tid + 1);
-            if (c0 | c1) atomicMax(&sh.sel, c1 ? 2 * tid + 1 : 2 * tid);
+            {
+                const unsigned long long some = __ballot((c0 | c1) != 0);
+                if (some && (tid & 63) == 63 - __clzll((long long)some)) atomicMax(&sh.sel, c1 ? 2 * tid + 1 : 2 * tid);
+            }
             __syncthreads();
-            const int d = sh.found != 0x7fffffff ? sh.found : sh.sel;
+            const int d = same(sh.found != 0x7fffffff ? sh.found : sh.sel);
             if (tid == d / 2) {
                 const bool odd = d & 1;
                 sh.sel_cnt = odd ? u0 : u0 - c0; sh.sel_mass = odd ? s0 : s0 - m0;
                 sh.nsel = odd ? c1 : c0;
             }
             __syncthreads();
-            if (need) left -= min(left, sh.sel_cnt);
-            done += sh.sel_mass;
-            equal = sh.nsel;
+            if (need) left -= min(left, same(sh.sel_cnt));
+            done += same(sh.sel_mass);
+            equal = same(sh.nsel);
             prefix |= (unsigned int)(wide - 1 - d) << at; mask |= (unsigned int)(wide - 1) << at;
             __syncthreads();
             if (at == 0) break;
@@ -490,10 +509,10 @@ struct Row {
             if (c0 && nc - c1 >= want) atomicMin(&sh.found, 2 * tid);
             else if (c1 && nc >= want) atomicMin(&sh.found, 2 * tid + 1);
             __syncthreads();
-            const int d = sh.found;
+            const int d = same(sh.found);
             if (tid == d / 2) sh.sel_cnt = (d & 1) ? nc - c1 : nc - c1 - c0;
             __syncthreads();
-            want -= sh.sel_cnt;
+            want -= same(sh.sel_cnt);
             at_prefix |= (unsigned int)d << at; at_mask |= (unsigned int)(kRadix - 1) << at;
             __syncthreads();
         }
@@ -544,7 +563,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (lane == 0) waves[wave] = v;
         if (tid == 0) sh.found = 0x7fffffff;
         __syncthreads();
-        for (int w = 0; w < kPick / 64; ++w) r.m = fmaxf(r.m, waves[w]);
+        r.m = same(wave_max(waves[lane & 15]));
         __syncthreads();
     }
     if (r.m == -INFINITY || ask.greedy) {
@@ -565,7 +584,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         const unsigned long long b = __ballot(holds);
         if (lane == 0 && b) atomicMin(&sh.found, wave * 64 + __ffsll((long long)b) - 1);
         __syncthreads();
-        const int f = sh.found;
+        const int f = same(sh.found);
         __syncthreads();
         return f;
     };
@@ -579,13 +598,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             if (s >= kBins - 1) s = kBins;
             else { reach = mine.cut < 0 ? -1 : min(s + mine.cut, kBins - 2); t = mine.total * weight(mine.max, r.m, ask.c); }
         }
-        if (tid < p.P) { sh.shift[tid] = (int16_t)s; sh.near[tid] = (uint16_t)(mine.near | (mine.binned ? kBinned : 0)); }
+        if (tid < p.P) { sh.shift[tid] = (int16_t)s; sh.near[tid] = (uint16_t)mine.near; sh.binned[tid] = (uint16_t)mine.binned; }
         if (tid == 0) sh.sel = kBins - 2;
         t = scan<double>(t, sh.wsum);
-        atomicMin(&sh.sel, reach);
+        if (reach < kBins - 2) atomicMin(&sh.sel, reach);
         if (tid == kPick - 1) sh.part = t;
         __syncthreads();
-        everything = sh.part; r.listed = sh.sel;
+        everything = same(sh.part); r.listed = same(sh.sel);
     }
     const bool filtered = ask.k || ask.p < 1.f || ask.min_p > 0.f;
     const unsigned int k = (unsigned int)ask.k;                           // (below V)
@@ -604,7 +623,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             if (at < kList) { sh.key[at] = key; sh.idx[at] = i; }
         });
         __syncthreads();
-        const bool here = sh.n <= kList;
+        const bool here = same(sh.n) <= kList;
         const double cum = scan<double>((double)bin[tid] * r.cell(tid), sh.wsum);
         const unsigned int cum_n = scan<unsigned int>(cnt[tid], sh.wcnt);
         int reach = kBins;
@@ -614,17 +633,18 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (reach > r.listed && ask.k && r.listed == kBins - 2) reach = r.listed;         // (fewer tokens than top-k would keep)
         if (tid == min(reach, kBins - 1)) sh.nsel = cum_n;
         __syncthreads();
-        if (reach <= r.listed && sh.nsel <= kDirect && sh.nsel > 0) {
+        const int few = same((int)sh.nsel);
+        if (reach <= r.listed && few <= kDirect && few > 0) {
             unsigned long long *v = sh.rmass;
             int size = 64;
-            while (size < (int)sh.nsel) size *= 2;
+            while (size < few) size *= 2;
             if (tid == 0) sh.sel = 0;
             __syncthreads();
             auto take = [&](unsigned int key, unsigned int i, float f, int b) { if (b <= reach) v[atomicAdd(&sh.sel, 1)] = ((unsigned long long)~key << 32) | i; };
             if (here) { for (unsigned int i = tid; i < sh.n; i += kPick) { const float f = of_key(sh.key[i]); take(sh.key[i], sh.idx[i], f, bin_of(f, r.m, ask.inv)); } }
             else r.each_listed(0, reach, take);
             __syncthreads();
-            const int n = sh.sel;
+            const int n = same(sh.sel);
             for (int i = n + tid; i < size; i += kPick) v[i] = ~0ull;
             __syncthreads();
             r.sort(v, size);                                              // descending logits, ascending indices
@@ -641,7 +661,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                 const int t = first_of(2 * tid < end && upto >= goal);
                 if (tid == t) sh.nsel = upto - v1 >= goal || 2 * tid + 1 >= end ? 1 : 2;
                 __syncthreads();
-                if (t < kBins) end = min(end, 2 * t + (int)sh.nsel);
+                if (t < kBins) end = min(end, 2 * t + same((int)sh.nsel));
             }
             const bool in0 = 2 * tid < end && !(ask.min_p > 0.f && w0 < (double)ask.min_p), in1 = 2 * tid + 1 < end && !(ask.min_p > 0.f && w1 < (double)ask.min_p);
             __syncthreads();
@@ -653,7 +673,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             const double upto = scan<double>(x0 + x1, sh.wsum);
             if (tid == kPick - 1) sh.part = upto;
             __syncthreads();
-            const double sum = sh.part, goal = u * sum;
+            const double sum = same(sh.part), goal = u * sum;
             int t = first_of(x0 + x1 > 0. && upto > goal);
             const bool beyond = t == kBins;                               // (no goal below the sum: the last one)
             if (beyond) {
@@ -661,7 +681,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                 __syncthreads();
                 if (x0 + x1 > 0.) atomicMax(&sh.sel, tid);
                 __syncthreads();
-                t = sh.sel;
+                t = same(sh.sel);
             }
             if (tid == t) {
                 const bool one = beyond ? !(x1 > 0.) : x0 > 0. && upto - x1 > goal;
@@ -681,7 +701,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         __syncthreads();
         for (int c = wave; c < p.P; c += kPick / 64) {
             const int s = sh.shift[c];
-            if (s >= kBins || (sh.near[c] & kBinned)) continue;
+            if (s >= kBins || sh.binned[c]) continue;
             const uint2 *q = p.near + ((int64_t)row * p.P + c) * kNear;
             for (int i = lane; i < sh.near[c]; i += 64) {
                 const float v = of_key(q[i].x);
@@ -698,7 +718,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int c = min(c0 + e, p.P - 1), b = tid - sh.shift[c];
-                const bool in = c0 + e < p.P && b >= 0 && tid < kBins - 1 && (sh.near[c] & kBinned);
+                const bool in = c0 + e < p.P && b >= 0 && b < sh.binned[c] && tid < kBins - 1;
                 const int64_t at = ((int64_t)row * p.P + c) * kBins + b;
                 q[e] = in ? p.mass[at] : 0;
                 n[e] = in && ask.k ? p.cnt[at] : 0;
@@ -710,18 +730,18 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         sh.cum[tid] = scan<double>((double)in_bin * unit_of_bin, sh.wsum);
         sh.cum_n[tid] = scan<unsigned int>(cnt, sh.wcnt);
         __syncthreads();
-        double total = ask.k ? sh.cum[kBins - 1] : everything;
+        double total = ask.k ? same(sh.cum[kBins - 1]) : everything;
         for (int filter = 0; filter < 2; ++filter) {                      // top-k, top-p
             if (filter == 0 ? !ask.k : ask.p == 1.f) continue;
             const double goal = filter ? (double)ask.p * total : 0.;
             const int b = first_of(filter ? sh.cum[tid] >= goal && sh.cum[tid] > 0. && tid < stop : sh.cum_n[tid] >= k);
             const int bin = filter && b == kBins ? stop : b;              // (the bin that top-k ended in, or none)
             if (bin == kBins || (filter && b == kBins && key == 0 && index == 0xffffffffu)) continue;
-            const double before = bin ? sh.cum[bin - 1] : 0.;
-            if (!filter && sh.cum_n[bin] == k) { stop = bin + 1; total = sh.cum[bin]; continue; }
+            const double before = bin ? same(sh.cum[bin - 1]) : 0.;
+            if (!filter && same(sh.cum_n[bin]) == k) { stop = bin + 1; total = same(sh.cum[bin]); continue; }
             unsigned int k2, i2;
             double part;
-            r.settle(bin, filter ? 0 : k - (bin ? sh.cum_n[bin - 1] : 0), before, goal, k2, i2, part);
+            r.settle(bin, filter ? 0 : k - (bin ? same(sh.cum_n[bin - 1]) : 0), before, goal, k2, i2, part);
             if (bin < stop || k2 > key || (k2 == key && i2 < index)) { key = k2; index = i2; }      // (in the bin where top-k ended, its own end may come first)
             stop = bin;
             if (!filter) total = before + part;
@@ -760,9 +780,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         double v = 0.;
         if (s < kBins) {
             if (!filtered) v = lane == 0 ? notes[c].total * weight(notes[c].max, r.m, ask.c) : 0.;
-            else if (sh.near[c] & kBinned) {
+            else if (sh.binned[c]) {
                 const unsigned long long *q = p.mass + ((int64_t)row * p.P + c) * kBins;
-                for (int b = lane; b < sure - s && b < kBins - 1; b += 64) v += (double)q[b] * units[b + s];
+                for (int b = lane; b < min(sure - s, (int)sh.binned[c]); b += 64) v += (double)q[b] * units[b + s];
             } else {
                 const uint2 *q = p.near + ((int64_t)row * p.P + c) * kNear;
                 for (int i = lane; i < sh.near[c]; i += 64) {
@@ -781,12 +801,12 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     if (tid == kPick - 1) sh.part = upto_c;
     if (tid == 0) sh.sel = 0;
     __syncthreads();
-    const double sum = sh.part, goal = u * sum;
+    const double sum = same(sh.part), goal = u * sum;
     int c = first_of(own > 0. && upto_c > goal);
     if (c == kBins) {
         if (own > 0.) atomicMax(&sh.sel, tid);
         __syncthreads();
-        c = sh.sel;
+        c = same(sh.sel);
     }
     if (tid == c) sh.part = upto_c - own;
     if (tid == 0) { sh.found = 0x7fffffff; sh.sel = -1; }
