@@ -207,8 +207,8 @@ def test_lora_inner_products_beyond_float16(arena, amplify):
     lora_case(arena, "float16", 20, 512, 40, 16, 2, np.arange(20) % 2, amplify=amplify)
 
 
-def test_lora_rows_do_not_depend_on_their_step(arena):
-    """A row's bits are the same whatever other rows the step has, up to 256 rows and the same number of K's shares."""
+def test_lora_bits_repeat(arena):
+    """No atomics decide an order of sums: a call gives the same bits again."""
     typed("bfloat16")
     ids = np.array([0, 1, 0, 2, 1, 0])
     a = lora_case(arena, "bfloat16", 6, 64, 64, 16, 3, ids, seed=3)
@@ -581,3 +581,284 @@ def test_evict_refuses_tables_that_are_too_short_on_the_device(arena):
     assert new.to_numpy((2,), np.int32).tolist() == [-1, 10]
     got = dk.to_numpy(k.shape, np.uint16)
     assert np.array_equal(got[:6], k[:6]) and np.array_equal(got[6, :10], k[4, :10]) and np.array_equal(got[6, 10:], k[6, 10:]) and np.array_equal(got[7], k[7])
+
+
+# ------------------------------------------------------------------------------------------------------------ together, captured, on streams of their own, far into a pool
+class Step:
+    """One layer's decode step of a batch whose requests have adapters of their own and whose caches are held to a budget, then a token each: the framework's product, nvr_lora_add beside it,
+    nvr_rope_rotate_store_kv, nvr_paged_attn_decode_scored, nvr_kv_evict, nvr_linear + nvr_lora_add for the output, logits, nvr_sample_uniform."""
+
+    def __init__(self, arena, dtype, stream=None, seed=0):
+        rng = np.random.default_rng(seed)
+        self.arena, self.dtype, self.stream, self.rng = arena, dtype, stream, rng
+        typed(dtype)
+        self.W, self.H, self.G, self.D, self.R, self.n, self.V, self.block, self.budget, self.first, self.last = 256, 4, 2, 64, 8, 3, 1024, 16, 48, 2, 8
+        self.lengths = [60, 47, 30, 52, 48]
+        B, self.w = len(self.lengths), np.dtype(kind(dtype)).itemsize
+        N = (self.H + 2 * self.G) * self.D
+        self.B, self.N = B, N
+
+        def weights(*shape, std):
+            return encode(rng.standard_normal(shape) * std, dtype)
+        self.host = {"x": weights(B, self.W, std=1.0), "wqkv": weights(N, self.W, std=self.W ** -0.5), "wo": weights(self.W, self.H * self.D, std=(self.H * self.D) ** -0.5),
+                     "head": weights(self.V, self.W, std=1.5 * self.W ** -0.5), "a1": weights(self.n, self.R, self.W, std=self.W ** -0.5), "b1": weights(self.n, N, self.R, std=0.5),
+                     "a2": weights(self.n, self.R, self.H * self.D, std=(self.H * self.D) ** -0.5), "b2": weights(self.n, self.W, self.R, std=0.5)}
+        self.dev = {k: arena.dev(v[1]) for k, v in self.host.items()}
+        self.ids, self.scales = np.array([0, 2, -1, 1, 0], np.int32), np.array([0.5, 1.0, 2.0], np.float32)
+        self.table, self.blocks = tables(rng, [n + 32 for n in self.lengths], self.block)
+        k, v = (encode(rng.standard_normal((self.blocks, self.block, self.G, self.D)), dtype) for _ in range(2))
+        self.k0, self.v0 = k[1], v[1]
+        self.s0 = rng.random((self.blocks, self.G, self.block)).astype(np.float32)
+        self.turns, self.amplitude = rope_turns("bands", self.D, factor=8.0, low=1.0, high=4.0)
+        self.d = {"ids": arena.dev(self.ids), "scales": arena.dev(self.scales), "turns": arena.dev(self.turns), "table": arena.dev(self.table), "k": arena.dev(self.k0), "v": arena.dev(self.v0),
+                  "scores": arena.dev(self.s0), "qkv": arena.space(B * N * self.w), "q": arena.space(B * self.H * self.D * self.w), "out": arena.space(B * self.H * self.D * self.w),
+                  "o": arena.space(B * self.W * self.w), "logits": arena.space(B * self.V * 4), "new_lens": arena.space(B * 4), "kept": arena.space(B * self.G * self.budget * 4),
+                  "token": arena.space(B * 8), "logprob": arena.space(B * 4), "ws_lora": arena.space(L.nvr_lora_workspace_bytes(B, self.H * self.D, N, self.R)),
+                  "ws_attn": arena.space(L.nvr_paged_attn_scored_workspace_bytes(B, self.H, self.G, self.D, 128)), "ws_sample": arena.space(L.nvr_sample_uniform_workspace_bytes(B, self.V)),
+                  "T": arena.dev(np.array([0.0, 0.7, 1.0, 1.3, 0.9], np.float32)), "tk": arena.dev(np.array([0, 20, 0, 50, 0], np.int64)), "tp": arena.dev(np.array([1, 1, 0.9, 0.95, 1], np.float32)),
+                  "mp": arena.dev(np.array([0, 0, 0, 0.02, 0.05], np.float32)), "u": arena.space(B * 4), "pos": arena.space(B * 8), "slots": arena.space(B * 4), "lens": arena.space(B * 4), "scored": arena.space(B * 4)}
+        self.positions = np.array([5000, 47, 123456, 52, 300], np.int64)
+
+    def feed(self, lengths):
+        """The step's small inputs: every sequence gets a key behind its `lengths`."""
+        n = np.array(lengths, np.int32)
+        slots = (self.table[np.arange(self.B), n // self.block] * self.block + n % self.block).astype(np.int32)
+        self.uniform = self.rng.random(self.B).astype(np.float32)
+        for name, a in (("lens", n + 1), ("scored", n), ("slots", slots), ("pos", self.positions), ("u", self.uniform)):
+            a = np.ascontiguousarray(a)
+            nvr.check(L.nvr_memcpy_h2d(self.d[name].ptr, a.ctypes.data, a.nbytes))
+        self.slots = slots
+
+    def launch(self):
+        d, w, s = self.d, self.dev, self.stream
+        B, N, W, H, G, D, R = self.B, self.N, self.W, self.H, self.G, self.D, self.R
+        m = nvr.AttnMetaC(is_prefill=0, context_lens=d["lens"].ptr, block_tables=d["table"].ptr, max_blocks=self.table.shape[1], batch=B, max_context_len=128)
+        ws, q = self.w, d["qkv"].ptr
+        nvr.check(L.nvr_linear(w["x"].ptr, W, w["wqkv"].ptr, B, W, N, q, 0, s))
+        nvr.check(L.nvr_lora_add(w["x"].ptr, W, w["a1"].ptr, w["b1"].ptr, d["scales"].ptr, d["ids"].ptr, self.n, B, W, N, R, q, N, q, N, d["ws_lora"].ptr, s))
+        nvr.check(L.nvr_rope_rotate_store_kv(q, N, q + H * D * ws, N, q + (H + G) * D * ws, N, d["pos"].ptr, d["slots"].ptr, B, H, G, D, D, 0, d["turns"].ptr, self.amplitude, d["q"].ptr, H * D, None, 0,
+                                             d["k"].ptr, d["v"].ptr, self.blocks * self.block, s))
+        nvr.check(L.nvr_paged_attn_decode_scored(d["q"].ptr, H * D, d["k"].ptr, d["v"].ptr, byref(m), H, G, D, self.block, self.blocks, D ** -0.5, d["scores"].ptr, d["scored"].ptr, 0.9, d["scores"].ptr,
+                                                 d["out"].ptr, d["ws_attn"].ptr, s))
+        nvr.check(L.nvr_kv_evict(d["k"].ptr, d["v"].ptr, d["scores"].ptr, byref(m), G, D, self.block, self.blocks, self.budget, self.first, self.last, None, 0, d["new_lens"].ptr, d["kept"].ptr, None, s))
+        nvr.check(L.nvr_linear(d["out"].ptr, H * D, w["wo"].ptr, B, H * D, W, d["o"].ptr, 0, s))
+        nvr.check(L.nvr_lora_add(d["out"].ptr, H * D, w["a2"].ptr, w["b2"].ptr, d["scales"].ptr, d["ids"].ptr, self.n, B, H * D, W, R, d["o"].ptr, W, d["o"].ptr, W, d["ws_lora"].ptr, s))
+        nvr.check(L.nvr_linear(d["o"].ptr, W, w["head"].ptr, B, W, self.V, d["logits"].ptr, 1, s))
+        nvr.check(L.nvr_sample_uniform(d["logits"].ptr, self.V, B, self.V, d["T"].ptr, d["tk"].ptr, d["tp"].ptr, d["mp"].ptr, d["u"].ptr, d["token"].ptr, d["logprob"].ptr, d["ws_sample"].ptr, s))
+
+    NAMES = (("qkv", None), ("q", None), ("out", None), ("o", None), ("k", None), ("v", None), ("scores", np.uint32), ("logits", np.uint32), ("new_lens", np.int32), ("kept", np.int32),
+             ("token", np.int64), ("logprob", np.uint32))
+
+    def answers(self):
+        return {n: self.d[n].to_numpy((self.d[n].nbytes // np.dtype(t or kind(self.dtype)).itemsize,), t or kind(self.dtype)) for n, t in self.NAMES}
+
+    def restore(self):
+        for name, a in (("k", self.k0), ("v", self.v0), ("scores", self.s0)):
+            nvr.check(L.nvr_memcpy_h2d(self.d[name].ptr, a.ctypes.data, a.nbytes))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_of_all_of_them(arena, dtype):
+    """Three steps; each stage against its definition on what the stage in front of it left."""
+    st = Step(arena, dtype)
+    lengths = list(st.lengths)
+    B, N, W, H, G, D = st.B, st.N, st.W, st.H, st.G, st.D
+    cache_k, cache_v = st.k0.copy(), st.v0.copy()
+    scores = st.s0.astype(np.float64)
+    up = HALF_STEP[dtype]
+    for _ in range(3):
+        st.feed(lengths)
+        st.launch()
+        nvr.synchronize()
+        a = st.answers()
+        val = {k: decode(v, dtype) for k, v in a.items() if k in ("qkv", "q", "out", "o")}
+        x, h = st.host["x"][0], {k: v[0] for k, v in st.host.items()}
+
+        def adapted(inp, base_w, A, Bm):
+            base = inp @ base_w.T
+            add = np.zeros_like(base)
+            for b in range(B):
+                if st.ids[b] >= 0:
+                    add[b] = st.scales[st.ids[b]] * (inp[b] @ A[st.ids[b]].T) @ Bm[st.ids[b]].T
+            return base, add
+        # projection: rounded once behind the product and once behind the adapters; sums of W products in 32 bits
+        base, add = adapted(x, h["wqkv"], h["a1"], h["b1"])
+        size = np.abs(x) @ np.abs(h["wqkv"]).T
+        within(val["qkv"].reshape(B, N), base + add, up * (np.abs(base) + np.abs(base + add)) * 1.01 + (W + 32) * F32 * size * 3 + SMALLEST[dtype] * 2 + 2.0 ** -15 * np.abs(add).max() * (dtype == "bfloat16"), "projection")
+        qkv = val["qkv"].reshape(B, H + 2 * G, D)
+        want = rope(qkv[:, :H + G], st.positions, st.turns, st.amplitude, False)
+        near = up * np.abs(want) * 1.01 + 8 * F32 * np.abs(qkv).max() + SMALLEST[dtype]
+        within(val["q"].reshape(B, H, D), want[:, :H], near[:, :H], "rotated queries")
+        shape = (st.blocks, st.block, G, D)
+        got_k, got_v, got_s = a["k"].reshape(shape), a["v"].reshape(shape), a["scores"].view(np.float32).reshape(st.s0.shape)
+        for b in range(B):
+            page, row = divmod(int(st.slots[b]), st.block)
+            cache_v[page, row] = a["qkv"].reshape(B, H + 2 * G, D)[b, H + G:]
+            cache_k[page, row] = encode(want[b, H:], dtype)[1]
+        new = []
+        for b in range(B):
+            n = lengths[b] + 1
+            j = np.arange(n)
+            page, row = st.table[b, j // st.block], j % st.block
+            kk, vv = decode(cache_k[page, row], dtype), decode(cache_v[page, row], dtype)
+            out, weight = attend(val["q"].reshape(B, H, D)[b], kk, vv, D ** -0.5)
+            # a key that was rounded the other way moves its score by a step: 2^-10 of |q||k| at most in 16 bits
+            within(val["out"].reshape(B, H, D)[b], out, up * np.abs(out) * 1.01 + (4 * up + 200 * F32) * np.abs(vv).max() + SMALLEST[dtype], "attention")
+            scores[page, :, row] = np.where(j[:, None] < lengths[b], 0.9 * scores[page, :, row], 0.0) + weight
+            m = min(n, st.budget)
+            for g in range(G):
+                kept = a["kept"].reshape(B, G, st.budget)[b, g]
+                assert (kept[m:] == -1).all() and (np.diff(kept[:m]) > 0).all()
+                if n > st.budget:
+                    assert np.array_equal(kept[:st.first], np.arange(st.first)) and np.array_equal(kept[m - st.last:m], np.arange(n - st.last, n))
+                    # what was left out scores no more than what was kept, but for the tolerance of the scores
+                    out_of = np.setdiff1d(np.arange(st.first, n - st.last), kept)
+                    inside = kept[st.first:m - st.last]
+                    assert scores[page[out_of], g, row[out_of]].max() <= scores[page[inside], g, row[inside]].min() + 16 * up
+                i = np.arange(m)
+                dst, src = (st.table[b, i // st.block], i % st.block), (page[kept[:m]], row[kept[:m]])
+                assert np.array_equal(got_v[dst[0], dst[1], g], cache_v[src[0], src[1], g])
+                within(decode(got_k[dst[0], dst[1], g], dtype), decode(cache_k[src[0], src[1], g], dtype), 2.02 * up * np.abs(decode(cache_k[src[0], src[1], g], dtype)) + 16 * F32 * np.abs(qkv).max(), "keys")
+                within(got_s[dst[0], g, dst[1]].astype(np.float64), scores[src[0], g, src[1]], np.full(m, 16 * up), "scores")
+            new.append(m)
+        assert a["new_lens"].tolist() == new
+        base, add = adapted(val["out"].reshape(B, -1), h["wo"], h["a2"], h["b2"])
+        within(val["o"].reshape(B, W), base + add, up * (np.abs(base) + np.abs(base + add)) * 1.01 + 600 * F32 * (np.abs(val["out"]).max() * 20) + SMALLEST[dtype] * 2 + 2.0 ** -15 * np.abs(add).max() * (dtype == "bfloat16"), "output")
+        logits = a["logits"].view(np.float32).reshape(B, st.V)
+        T, k, p, m = ([0.0, 0.7, 1.0, 1.3, 0.9], [0, 20, 0, 50, 0], [1, 1, 0.9, 0.95, 1], [0, 0, 0, 0.02, 0.05])
+        assert a["token"].tolist() == [sample(logits[b], float(np.float32(T[b])), k[b], float(np.float32(p[b])), float(np.float32(m[b])), float(st.uniform[b]))[0] for b in range(B)]
+        # the next step goes on from what is there
+        cache_k, cache_v, scores = got_k.copy(), got_v.copy(), got_s.astype(np.float64)
+        lengths = new
+        st.positions = st.positions + 1
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_captured_step_replays(arena, dtype):
+    """The step in a graph, replayed with other inputs and eager work between: the bits of the eager step each time."""
+    stream = C.c_void_p()
+    nvr.check(L.nvr_stream_create(byref(stream)))
+    st = Step(arena, dtype, stream)
+    st.feed(st.lengths)
+    st.launch()
+    nvr.check(L.nvr_stream_synchronize(stream))
+    graph = C.c_void_p()
+    nvr.check(L.nvr_graph_capture_begin(stream))
+    st.launch()
+    nvr.check(L.nvr_graph_capture_end(stream, byref(graph)))
+    for turn in range(4):
+        lengths = [min(n + 3 * turn, 75) for n in st.lengths]
+        st.positions = st.positions + 17
+        st.restore()
+        st.feed(lengths)
+        st.launch()
+        nvr.check(L.nvr_stream_synchronize(stream))
+        eager = st.answers()
+        st.restore()
+        for name in ("qkv", "q", "out", "o", "logits", "token", "kept", "new_lens"):
+            nvr.check(L.nvr_device_memset(st.d[name].ptr, SENTINEL, st.d[name].nbytes))
+        nvr.synchronize()
+        nvr.check(L.nvr_graph_launch(graph, stream))
+        nvr.check(L.nvr_stream_synchronize(stream))
+        again = st.answers()
+        for name in eager:
+            assert np.array_equal(eager[name], again[name]), (turn, name)
+    nvr.check(L.nvr_graph_destroy(graph))
+    nvr.check(L.nvr_stream_destroy(stream))
+
+
+def test_two_streams_at_once(arena):
+    """Two steps on streams of their own, with workspaces of their own, in flight together: the bits of each alone."""
+    streams = [C.c_void_p(), C.c_void_p()]
+    for s in streams:
+        nvr.check(L.nvr_stream_create(byref(s)))
+    steps = [Step(arena, "float16", s, seed=i) for i, s in enumerate(streams)]
+    alone = []
+    for st in steps:
+        st.feed(st.lengths)
+        st.launch()
+        nvr.synchronize()
+        alone.append(st.answers())
+        st.restore()
+    nvr.synchronize()
+    for st in steps:
+        st.launch()
+    nvr.synchronize()
+    for st, want in zip(steps, alone):
+        got = st.answers()
+        for name in want:
+            assert np.array_equal(want[name], got[name]), name
+    for s in streams:
+        nvr.check(L.nvr_stream_destroy(s))
+
+
+def test_pool_beyond_32_bits_of_numbers(arena):
+    """Blocks 2^31 numbers and more into caches of 4.9 GB: stored, attended to, evicted in place and into other blocks."""
+    typed("float16")
+    G, D, block, blocks, H = 8, 128, 256, 9400, 8
+    row = G * D
+    assert blocks * block * row > 1 << 31
+    k, v, s = (nvr.DeviceBuffer(n) for n in (blocks * block * row * 2, blocks * block * row * 2, blocks * G * block * 4))
+    rng = np.random.default_rng(0)
+    table = np.array([[9399, 3, 9300, 8800]], np.int32)
+    to = np.array([[9350, 9399 - 1]], np.int32)
+    n = 900
+    hk, hv, hs = rng.standard_normal((4, block, G, D)).astype(np.float16), rng.standard_normal((4, block, G, D)).astype(np.float16), rng.random((4, G, block)).astype(np.float32)
+
+    def put():
+        for i, p in enumerate(table[0]):
+            for buf, a, size in ((k, hk, block * row * 2), (v, hv, block * row * 2), (s, hs, G * block * 4)):
+                c = np.ascontiguousarray(a[i])
+                nvr.check(L.nvr_memcpy_h2d(buf.ptr + int(p) * size, c.ctypes.data, size))
+
+    def block_of(buf, p, shape, t):
+        a = np.empty(shape, t)
+        nvr.check(L.nvr_memcpy_d2h(a.ctypes.data, buf.ptr + int(p) * a.nbytes, a.nbytes))
+        return a
+    put()
+    # the newest key by the rotation, in the far block
+    x = rng.standard_normal((1, H + 2 * G, D)).astype(np.float16)
+    turns, _ = rope_turns("plain", D)
+    page, at = table[0, (n - 1) // block], (n - 1) % block
+    dx, q = arena.dev(x), arena.space(H * D * 2)
+    nvr.check(L.nvr_rope_rotate_store_kv(dx.ptr, (H + 2 * G) * D, dx.ptr + H * D * 2, (H + 2 * G) * D, dx.ptr + (H + G) * D * 2, (H + 2 * G) * D, arena.dev(np.array([n - 1])).ptr,
+                                         arena.dev(np.array([page * block + at], np.int32)).ptr, 1, H, G, D, D, 0, arena.dev(turns).ptr, 1.0, q.ptr, H * D, None, 0, k.ptr, v.ptr, blocks * block, None))
+    want = rope(x[:, H:H + G].astype(np.float64), np.array([n - 1]), turns, 1.0, False)[0]
+    stored = block_of(k, page, (block, G, D), np.float16)
+    within(stored[at].astype(np.float64), want, HALF_STEP["float16"] * np.abs(want) + 1e-5, "stored key")
+    assert np.array_equal(block_of(v, page, (block, G, D), np.float16)[at], x[0, H + G:])
+    hk[(n - 1) // block, at], hv[(n - 1) // block, at] = stored[at], x[0, H + G:]
+    m = nvr.AttnMetaC(is_prefill=0, context_lens=arena.dev(np.array([n], np.int32)).ptr, block_tables=arena.dev(table).ptr, max_blocks=4, batch=1, max_context_len=n)
+    out = arena.space(H * D * 2)
+    nvr.check(L.nvr_paged_attn_decode_scored(q.ptr, H * D, k.ptr, v.ptr, byref(m), H, G, D, block, blocks, D ** -0.5, s.ptr, None, 1.0, s.ptr, out.ptr,
+                                             arena.space(L.nvr_paged_attn_scored_workspace_bytes(1, H, G, D, n)).ptr, None))
+    j = np.arange(n)
+    wout, weight = attend(q.to_numpy((H, D), np.float16).astype(np.float64), hk[j // block, j % block].astype(np.float64), hv[j // block, j % block].astype(np.float64), D ** -0.5)
+    within(out.to_numpy((H, D), np.float16).astype(np.float64), wout, 2 * HALF_STEP["float16"] * np.abs(wout) + 2e-5, "far attention")
+    for i in range(4):
+        hs[i] = block_of(s, table[0, i], (G, block), np.float32)
+    new, kept = arena.space(4), arena.space(G * 400 * 4)
+    for dest in (to, None):
+        put()
+        nvr.check(L.nvr_kv_evict(k.ptr, v.ptr, s.ptr, byref(m), G, D, block, blocks, 400, 4, 64, arena.dev(dest).ptr if dest is not None else None, 2 if dest is not None else 0, new.ptr, kept.ptr, None, None))
+        names = (dest if dest is not None else table)[0]
+        got_k, got_s = [block_of(k, p, (block, G, D), np.float16) for p in names[:2]], [block_of(s, p, (G, block), np.float32) for p in names[:2]]
+        for g in range(G):
+            mine = evict(hs[j // block, g, j % block], 400, 4, 64)
+            assert np.array_equal(kept.to_numpy((G, 400), np.int32)[g], mine)
+            i = np.arange(400)
+            assert np.array_equal(np.array(got_k)[i // block, i % block, g], hk[mine // block, mine % block, g])
+            assert np.array_equal(np.array(got_s)[i // block, g, i % block], hs[mine // block, g, mine % block])
+    nvr.synchronize()
+
+
+def test_lora_of_thousands_of_adapters(arena):
+    rng = np.random.default_rng(7)
+    lora_case(arena, "float16", 3000, 16, 24, 4, 8191, rng.integers(-1, 8191, 3000))
+    lora_case(arena, "bfloat16", 60, 16, 24, 4, 8191, rng.integers(-1, 8191, 60))
+
+
+def test_sample_of_many_short_rows(arena):
+    rng = np.random.default_rng(8)
+    check_sample(arena, rng.standard_normal((700, 33)) * 2, 1.0, 5, 0.9, 0.01, rng.random(700).astype(np.float32))
+    check_sample(arena, rng.standard_normal((300, 17000)) * 2, 1.0, 0, 0.9, 0.0, rng.random(300).astype(np.float32))
