@@ -93,6 +93,21 @@ __device__ __forceinline__ void min_p_bins(float min_p, int &sure, int &last) {
     sure = (int)fmin(fmax(floor(e) - 2., -1.), (double)(kBins - 2)); last = (int)fmin(ceil(e) + 2., (double)(kBins - 2));
 }
 
+// v[j] of registers, a bit of j at a time.  By masks: as conditions the compiler compares anew for each of the selections
+template <int N>
+__device__ __forceinline__ float pick_of(const float (&v)[N], int j) {
+    unsigned int t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = __float_as_uint(v[i]);
+#pragma unroll
+    for (int s = N / 2; s; s /= 2) {
+        unsigned int mask = (unsigned int)((int)((unsigned int)j * (0x80000000u / s)) >> 31);
+        asm("" : "+v"(mask));
+#pragma unroll
+        for (int i = 0; i < s; ++i) t[i] = (t[i + s] & mask) | (t[i] & ~mask);
+    }
+    return __uint_as_float(t[0]);
+}
 // tokens of a chunk from i on: 4 of them (those behind `end`: -inf)
 __device__ __forceinline__ float4_t four(const float *x, int i, int end, bool whole) {
     float4_t v;
@@ -160,7 +175,8 @@ __device__ __forceinline__ T wave_total(T v) { return from_lane(wave_scan(v), 63
 // A chunk of EPT tokens a thread, held in registers: its maximum, its largest tokens, its bins
 template <int EPT, int THREADS>
 __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p) {
-    __shared__ unsigned long long mass[kBins];
+    constexpr int COPIES = EPT == 16 ? 2 : 1;
+    __shared__ unsigned long long mass[kBins][COPIES];
     __shared__ unsigned int cnt[kBins];
     __shared__ uint2 near[kNear];
     __shared__ double sums[THREADS / 64];
@@ -181,7 +197,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
         for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e];
     }
     const RowAsk ask = row_ask(p.a, row, p.V);
-    for (int b = tid; b < kBins; b += THREADS) { mass[b] = 0; cnt[b] = 0; }
+    for (int b = tid; b < kBins; b += THREADS) { for (int e = 0; e < COPIES; ++e) mass[b][e] = 0; cnt[b] = 0; }
     if (tid == 0) { cut = list_cut = kBins - 2; listed = 0; first_at = 0x7fffffff; bins_used = 0; }
     float high[NG];
 #pragma unroll
@@ -211,15 +227,26 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
     }
     const bool counted = ask.k > 0, lone = lonely(m, ask.inv), filtered = counted || ask.p < 1.f || ask.min_p > 0.f;
     double total = 0.;                                                    // weights, the chunk's maximum 1 (of rows that top-p or nothing ends)
-    auto listing = [&](int j) {
+    auto listing = [&](float x, int j) {
         const unsigned int at = atomicAdd(&listed, 1u);
-        if (at < kNear) near[at] = make_uint2(key_of(v[j]), (unsigned int)index(j));
+        if (at < kNear) near[at] = make_uint2(key_of(x), (unsigned int)index(j));
+    };
+    // f(x, j) for the tokens not below `least`, one a lane at a time: a wave comes to f as often as its busiest lane
+    auto each_from = [&](float least, auto f) {
+        unsigned int some = 0;
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) some |= (v[j] >= least ? 1u : 0u) << j;
+        while (some) {
+            const int j = __ffs((int)some) - 1;
+            some &= some - 1;
+            f(pick_of(v, j), j);
+        }
     };
     int list_end = kBins, bins_end = kBins;                               // tokens of bins up to these go into the list, into the bins
     int binned = 0;
     if (lone) {                                                           // (only the equals of the maximum count)
 #pragma unroll
-        for (int j = 0; j < EPT; ++j) if (v[j] == m) { listing(j); total += 1.; }
+        for (int j = 0; j < EPT; ++j) if (v[j] == m) { listing(m, j); total += 1.; }
         __syncthreads();
         if (listed > kNear) {
             const int64_t at = ((int64_t)row * p.P + c) * kBins;
@@ -237,8 +264,8 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
             f = t - (whole - kWhole);
             return low_of(whole_m) - low_of(whole);
         };
-        // the bins of the k-th maximum, and of the one at the list's end: the k-th too, or, of many, three times a chunk's share of k; without top-k the 96th
-        const unsigned int want = counted ? (unsigned int)min(ask.k, 0x7fffffffll) : 96, want_list = want <= 96 ? want : max(96u, (unsigned int)min(3ll * ask.k / p.P, (long long)kNear));
+        // the bins of the k-th maximum, and of the one at the list's end: the k-th too, or, of many, three times a chunk's share of k; without top-k one of 11 maxima (96 of a chunk of 4096 tokens)
+        const unsigned int want = counted ? (unsigned int)min(ask.k, 0x7fffffffll) : NG * THREADS * 3 / 32, want_list = want <= 96 || !counted ? want : max(96u, (unsigned int)min(3ll * ask.k / p.P, (long long)kNear));
 #pragma unroll
         for (int g = 0; g < NG; ++g) { double f; const int b = cell_of(high[g], f); if (b < kBins - 1) atomicAdd(&cnt[b], 1u); }
         __syncthreads();
@@ -261,45 +288,42 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
             bins_end = min(bins_end, last);
         }
         list_end = min(list_cut, bins_end);                               // (fewer maxima than wanted: all that is near, if it fits)
-        // 24 x / T of these bins is not below that of the maximum less the bins and 1; a little less, for the roundings
-        auto least_of = [&](int bins) { const float f = (float)((t_m - bins - 1.) / ask.inv); return f - fabsf(f) * 1e-6f; };
-        const float least_listed = least_of(list_end);
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            if (v[j] < least_listed) continue;
+        // the lower end of a bin's cell, as a logit; a little less, for the roundings
+        auto least_of = [&](int bins) { const float f = (float)(((whole_m - kWhole) - bins - 0.5) / ask.inv); return f - fabsf(f) * 1e-6f; };
+        auto into = [&](int b, double f) { atomicAdd(&mass[b][tid & (COPIES - 1)], in_cell(f)); if (counted) atomicAdd(&cnt[b], 1u); };
+        bool bins = list_end < bins_end;                                  // (else the list has all that counts, if it fits)
+        const bool sparse = bins_end < kBins - 2, both = bins && sparse;
+        each_from(least_of(both ? bins_end : list_end), [&](float x, int j) {
             double f;
-            if (cell_of(v[j], f) <= list_end) listing(j);
-        }
+            const int b = cell_of(x, f);
+            if (b <= list_end) listing(x, j);
+            if (both && b <= bins_end) into(b, f);
+        });
         __syncthreads();
-        const bool bins = listed > kNear || list_end < bins_end;          // (else the list has all that counts)
-        if (listed > kNear) list_end = -1;
+        if (listed > kNear) { bins = true; list_end = -1; }
         if (bins || (!counted && ask.p < 1.f)) {
-            if (bins_end == kBins - 2) {                                  // all tokens: those too far below go into the last bin, which nobody reads
+            if (!sparse) {                                                // all tokens: those too far below go into the last bin, which nobody reads
 #pragma unroll
                 for (int j = 0; j < EPT; ++j) {
                     double f;
                     const int b = min(cell_of(v[j], f), kBins - 1);
-                    atomicAdd(&mass[b], in_cell(f));
-                    if (counted) atomicAdd(&cnt[b], 1u);
+                    into(b, f);
                 }
-            } else {
-                const float least = least_of(bins_end);
-#pragma unroll
-                for (int j = 0; j < EPT; ++j) {
-                    if (v[j] < least) continue;
+            } else if (!both) {
+                each_from(least_of(bins_end), [&](float x, int) {
                     double f;
-                    const int b = cell_of(v[j], f);
-                    if (b > bins_end) continue;
-                    atomicAdd(&mass[b], in_cell(f));
-                    if (counted) atomicAdd(&cnt[b], 1u);
-                }
+                    const int b = cell_of(x, f);
+                    if (b <= bins_end) into(b, f);
+                });
             }
             __syncthreads();
             const int64_t at = ((int64_t)row * p.P + c) * kBins;
             const double off = t_m - (whole_m - kWhole);
             unsigned int used = 0;
             for (int b = tid; b < kBins - 1; b += THREADS) {
-                const unsigned long long q = mass[b];
+                unsigned long long q = mass[b][0];
+#pragma unroll
+                for (int e = 1; e < COPIES; ++e) q += mass[b][e];
                 if (q) used = b + 1;
                 if (!counted && q) total += (double)q * exp2_64(-((double)b + off) * (1.4426950408889634 / kPerUnit));
                 if (bins) { p.mass[at + b] = q; if (counted) p.cnt[at + b] = cnt[b]; }
@@ -325,7 +349,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
 }
 
 namespace {
-constexpr int kDirect = 2048, kChunks = 1024;
+constexpr int kDirect = 128, kCount = 256, kChunks = 1024;
 struct PickShared {
     double cum[kBins];                                                    // weight of the bins up to and with this one
     unsigned int cum_n[kBins];
@@ -381,8 +405,8 @@ struct Row {
     // ... in the row itself.  Most tokens are outside: two comparisons with the bins' ends (a little beyond, for their roundings) come first
     template <class F>
     __device__ __forceinline__ void each_of_row(int lo, int hi, F f) const {
-        const double top = (double)m * ask.inv;
-        const float a = (float)((top - hi - 1.) / ask.inv), z = (float)((top - lo + 1.) / ask.inv);
+        const double top = ((double)m * ask.inv + kWhole) - kWhole;       // (the cells' ends are halves)
+        const float a = (float)((top - hi - 0.5) / ask.inv), z = (float)((top - lo + 0.5) / ask.inv);
         const bool lone = lonely(m, ask.inv);
         const float least = lone ? m : a - fabsf(a) * 1e-6f, most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
         const bool all = !(least == least && most == most);               // (1 / inv beyond float)
@@ -393,12 +417,13 @@ struct Row {
             unsigned int near = 0;                                        // the few that may be meant, one a lane at a time: a wave comes here as often as its busiest lane
 #pragma unroll
             for (int e = 0; e < 16; ++e) { const float w = v[e >> 2][e & 3]; near |= (w != -INFINITY && (all || (w >= least && w <= most)) ? 1u : 0u) << e; }
+            float flat[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) flat[e] = v[e >> 2][e & 3];
             while (near) {
                 const int j = __ffs((int)near) - 1;
                 near &= near - 1;
-                float w = v[0][0];
-#pragma unroll
-                for (int n = 1; n < 16; ++n) w = j == n ? v[n >> 2][n & 3] : w;
+                const float w = pick_of(flat, j);
                 const int b = bin_of(w, m, ask.inv);
                 if (b >= lo && b <= hi && b < kBins - 1) f(key_of(w), (unsigned int)(i0 + (j >> 2) * kPick * 4 + (j & 3)), w, b);
             }
@@ -406,9 +431,10 @@ struct Row {
     }
     template <class F>
     __device__ __forceinline__ void each(int lo, int hi, F f) const { if (hi <= listed) each_listed(lo, hi, f); else each_of_row(lo, hi, f); }
-    // the tokens of bins lo .. hi into LDS; false: they are more than it holds
+    // the tokens of bins lo .. hi (and maybe more) into LDS; false: they are more than it holds
     __device__ __forceinline__ bool gather(int lo, int hi) {
-        if (lo == from && hi == to) return sh.n <= kList;                 // (they are there)
+        if (from <= lo && hi <= to && same(sh.n) <= kList) return true;   // (they are there)
+        if (lo == from && hi == to) return false;
         from = lo; to = hi;
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
@@ -421,15 +447,49 @@ struct Row {
     }
     template <class F>
     __device__ __forceinline__ void each_gathered(bool all_here, int lo, int hi, F f) const {
-        if (all_here) { for (unsigned int i = threadIdx.x; i < sh.n; i += kPick) { const float v = of_key(sh.key[i]); f(sh.key[i], sh.idx[i], v, bin_of(v, m, ask.inv)); } }
-        else each(lo, hi, f);
+        if (!all_here) { each(lo, hi, f); return; }
+        for (unsigned int i = threadIdx.x; i < sh.n; i += kPick) {
+            const unsigned int k = sh.key[i];
+            const float v = of_key(k);
+            const int b = bin_of(v, m, ask.inv);
+            if (b >= lo && b <= hi) f(k, sh.idx[i], v, b);
+        }
     }
     // Among the tokens of bin b in descending order (ties: ascending index): the last one that is kept, when `need` of them are (need > 0) or as many as it takes until `before` plus their weights
-    // reaches `goal`.  part: the weight of the kept ones.  A radix select over 11 bits of the logit at a time, then over 11 and 11 of the index
+    // reaches `goal`.  part: the weight of the kept ones.  Of few tokens, a thread a token, each counts those in front of it; else a radix select over 11 bits of the logit at a time, then over 11
+    // and 11 of the index
     __device__ __forceinline__ void settle(int b, unsigned int need, double before, double goal, unsigned int &key, unsigned int &index, double &part) {
         const bool here = gather(b, b);
         const int tid = threadIdx.x;
         const double unit = cell(b);
+        if (here) {
+            unsigned long long *v = sh.rmass, *w = v + kCount;
+            if (tid == 0) { sh.sel_cnt = 0; sh.found = 0x7fffffff; }
+            __syncthreads();
+            each_gathered(true, b, b, [&](unsigned int k, unsigned int i, float f, int) {
+                const unsigned int at = atomicAdd(&sh.sel_cnt, 1u);
+                if (at < kCount) { v[at] = ((unsigned long long)~k << 32) | i; w[at] = inside(f); }
+            });
+            __syncthreads();
+            const int n = same((int)sh.sel_cnt);
+            if (n == 0) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }      // (no token: everything is kept)
+            if (n <= kCount) {
+                int rank = 0;
+                unsigned long long upto = 0;
+                if (tid < n) {
+                    const unsigned long long a = v[tid];
+#pragma unroll 4
+                    for (int j = 0; j < n; ++j) { const bool in = v[j] <= a; rank += in; upto += in ? w[j] : 0; }      // (no two are alike)
+                    if (need ? rank >= (int)need : before + (double)upto * unit >= goal) atomicMin(&sh.found, rank);
+                }
+                __syncthreads();
+                if (tid < n && rank == min(sh.found, n)) { sh.low = ~(unsigned int)(v[tid] >> 32); sh.high = (unsigned int)v[tid]; sh.part = (double)upto * unit; }      // (where rounding leaves the goal unreached, the last)
+                __syncthreads();
+                key = same(sh.low); index = same(sh.high); part = same(sh.part);
+                __syncthreads();
+                return;
+            }
+        }
         unsigned int left = need, equal = 0;
         unsigned long long done = 0;                                      // weight above the prefix
         // the tokens of a bin are alike in their upper bits: those are the first prefix
@@ -518,32 +578,16 @@ struct Row {
         }
         index = at_prefix;
     }
-    // v[0 .. size) ascending, size a power of two of 64 .. 2 kPick.  Pairs less than 64 apart are a wave's own (its 64 pairs lie in 128 neighbours), and its LDS requests are served in order
+    // v[0 .. size) ascending, up to kDirect of them: a number's place is how many are smaller
     __device__ __forceinline__ void sort(unsigned long long *v, int size) {
         const int t = threadIdx.x;
-        if (size <= 128) {                                                // few: a number's place is how many are smaller
-            const unsigned long long a = t < size ? v[t] : 0;
-            int at = 0;
-            if (t < size)
+        const unsigned long long a = t < size ? v[t] : 0;
+        int at = 0;
+        if (t < size)
 #pragma unroll 8
-                for (int j = 0; j < size; ++j) { const unsigned long long b = v[j]; at += b < a || (b == a && j < t); }
-            __syncthreads();
-            if (t < size) v[at] = a;
-            __syncthreads();
-            return;
-        }
-        for (int k = 2; k <= size; k *= 2) {
-            for (int j = k / 2; j > 0; j /= 2) {
-                if (j >= 64) __syncthreads();
-                if (t < size / 2) {
-                    const int i = 2 * t - (t & (j - 1));                  // pair (i, i + j)
-                    const unsigned long long a = v[i], b = v[i + j];
-                    if ((a > b) == ((i & k) == 0)) { v[i] = b; v[i + j] = a; }
-                }
-                if (j >= 64) __syncthreads();
-                asm volatile("" ::: "memory");
-            }
-        }
+            for (int j = 0; j < size; ++j) { const unsigned long long b = v[j]; at += b < a || (b == a && j < t); }
+        __syncthreads();
+        if (t < size) v[at] = a;
         __syncthreads();
     }
 };
@@ -610,7 +654,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     const unsigned int k = (unsigned int)ask.k;                           // (below V)
     int p_sure = kBins - 2, p_last = kBins - 2;                           // min-p: bins that have it throughout, and in part
     if (ask.min_p > 0.f) min_p_bins(ask.min_p, p_sure, p_last);
-    // ---- few tokens: the lists have all that may be kept, down to the bin that the first filter ends in
+    // ---- the lists have all that may be kept, down to the bin that the first filter ends in?
+    bool from_lists = false, in_lds = false;                              // ... and LDS too
     if (filtered && r.listed >= 0) {
         unsigned long long *bin = sh.rmass;
         unsigned int *cnt = sh.rcnt;
@@ -632,9 +677,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (ask.min_p > 0.f && (!ask.k || ask.p == 1.f)) reach = min(reach, p_last);      // (what top-k keeps in all is wanted for top-p)
         if (reach > r.listed && ask.k && r.listed == kBins - 2) reach = r.listed;         // (fewer tokens than top-k would keep)
         if (tid == min(reach, kBins - 1)) sh.nsel = cum_n;
+        sh.cum[tid] = cum; sh.cum_n[tid] = cum_n;
         __syncthreads();
         const int few = same((int)sh.nsel);
-        if (reach <= r.listed && few <= kDirect && few > 0) {
+        from_lists = reach <= r.listed && few > 0;
+        if (here) { r.from = 0; r.to = r.listed; }
+        if (from_lists && few > kDirect && few <= kList) in_lds = r.gather(0, reach);
+        if (from_lists && few <= kDirect) {
             unsigned long long *v = sh.rmass;
             int size = 64;
             while (size < few) size *= 2;
@@ -644,7 +693,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             if (here) { for (unsigned int i = tid; i < sh.n; i += kPick) { const float f = of_key(sh.key[i]); take(sh.key[i], sh.idx[i], f, bin_of(f, r.m, ask.inv)); } }
             else r.each_listed(0, reach, take);
             __syncthreads();
-            const int n = same(sh.sel);
+            const int n = same(sh.sel);                                   // (few)
             for (int i = n + tid; i < size; i += kPick) v[i] = ~0ull;
             __syncthreads();
             r.sort(v, size);                                              // descending logits, ascending indices
@@ -692,11 +741,12 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         }
         __syncthreads();
     }
-    // ---- many: the row's bins, thread b bin b, from the chunks' or, of the chunks that left none, from their lists
+    // ---- many: the row's bins, thread b bin b: those of the lists, or from the chunks', or, of the chunks that left none, from their lists
     int stop = kBins;                                                     // bins in front of it are kept whole; of this one, tokens down to (key, index)
     unsigned int key = 0, index = 0xffffffffu;
     double unit_of_bin = 0.;
-    if (filtered) {
+    if (filtered) unit_of_bin = r.cell(tid);
+    if (filtered && !from_lists) {
         sh.rmass[tid] = 0; sh.rcnt[tid] = 0;
         __syncthreads();
         for (int c = wave; c < p.P; c += kPick / 64) {
@@ -712,11 +762,11 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         __syncthreads();
         unsigned long long in_bin = sh.rmass[tid];
         unsigned int cnt = sh.rcnt[tid];
-        for (int c0 = 0; c0 < p.P; c0 += 8) {                             // (8 chunks' requests together)
-            unsigned long long q[8];
-            unsigned int n[8];
+        for (int c0 = 0; c0 < p.P; c0 += 16) {                            // (16 chunks' requests together)
+            unsigned long long q[16];
+            unsigned int n[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 16; ++e) {
                 const int c = min(c0 + e, p.P - 1), b = tid - sh.shift[c];
                 const bool in = c0 + e < p.P && b >= 0 && b < sh.binned[c] && tid < kBins - 1;
                 const int64_t at = ((int64_t)row * p.P + c) * kBins + b;
@@ -724,12 +774,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                 n[e] = in && ask.k ? p.cnt[at] : 0;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { in_bin += q[e]; cnt += n[e]; }
+            for (int e = 0; e < 16; ++e) { in_bin += q[e]; cnt += n[e]; }
         }
-        unit_of_bin = r.cell(tid);
         sh.cum[tid] = scan<double>((double)in_bin * unit_of_bin, sh.wsum);
         sh.cum_n[tid] = scan<unsigned int>(cnt, sh.wcnt);
         __syncthreads();
+    }
+    if (filtered) {
         double total = ask.k ? same(sh.cum[kBins - 1]) : everything;
         for (int filter = 0; filter < 2; ++filter) {                      // top-k, top-p
             if (filter == 0 ? !ask.k : ask.p == 1.f) continue;
@@ -737,6 +788,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             const int b = first_of(filter ? sh.cum[tid] >= goal && sh.cum[tid] > 0. && tid < stop : sh.cum_n[tid] >= k);
             const int bin = filter && b == kBins ? stop : b;              // (the bin that top-k ended in, or none)
             if (bin == kBins || (filter && b == kBins && key == 0 && index == 0xffffffffu)) continue;
+            if (bin > p_last && (filter || ask.p == 1.f)) { stop = bin; key = 0; index = 0xffffffffu; continue; }      // (min-p leaves less)
             const double before = bin ? same(sh.cum[bin - 1]) : 0.;
             if (!filter && same(sh.cum_n[bin]) == k) { stop = bin + 1; total = same(sh.cum[bin]); continue; }
             unsigned int k2, i2;
@@ -757,6 +809,57 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (by_key && b == key_bin && (kk < key || (kk == key && i > index))) return false;
         return !(ask.min_p > 0.f) || w >= (double)ask.min_p;
     };
+    if (in_lds) {
+        // ---- the token among up to kList in LDS (thread t has t and t + kPick): weights are whole numbers of 2^-52 (and 1 at least), summed by the upper 11 bits of the index and then by the others
+        unsigned long long q[2] = {0, 0};
+        unsigned int i[2] = {0, 0}, id = 0;
+        double w[2] = {0., 0.};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const unsigned int at = tid + e * kPick;
+            if (at >= sh.n) continue;
+            const unsigned int kk = sh.key[at];
+            const float v = of_key(kk);
+            i[e] = sh.idx[at]; w[e] = weight(v, r.m, ask.c);
+            if (kept(bin_of(v, r.m, ask.inv), kk, i[e], w[e])) q[e] = max(1ull, (unsigned long long)(w[e] * 0x1p52 + 0.5));
+        }
+        unsigned long long done = 0;
+        double sum = 0., goal = 0.;
+        const int lower = max(32 - __clz(p.V - 1) - 11, 0);               // 11 at most
+        for (int level = 0; level < (lower ? 2 : 1); ++level) {
+            sh.rmass[2 * tid] = 0; sh.rmass[2 * tid + 1] = 0;
+            if (tid == 0) { sh.found = 0x7fffffff; sh.sel = 0; }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (q[e] && (level == 0 || i[e] >> lower == id)) atomicAdd(&sh.rmass[level ? i[e] & ((1u << lower) - 1) : i[e] >> lower], q[e]);
+            __syncthreads();
+            const unsigned long long m0 = sh.rmass[2 * tid], m1 = sh.rmass[2 * tid + 1], s1 = scan<unsigned long long>(m0 + m1, sh.wsum64), s0 = s1 - m1;
+            if (level == 0) {
+                if (tid == kPick - 1) sh.sel_mass = s1;
+                __syncthreads();
+                sum = (double)same(sh.sel_mass); goal = u * sum;
+                __syncthreads();
+            }
+            if (m0 && (double)(done + s0) > goal) atomicMin(&sh.found, 2 * tid);
+            else if (m1 && (double)(done + s1) > goal) atomicMin(&sh.found, 2 * tid + 1);
+            if (m0 | m1) atomicMax(&sh.sel, m1 ? 2 * tid + 1 : 2 * tid);
+            __syncthreads();
+            const int d = same(sh.found != 0x7fffffff ? sh.found : sh.sel);      // (no goal below the sum: the last one)
+            if (tid == d / 2) sh.sel_mass = (d & 1) ? s0 : s0 - m0;
+            __syncthreads();
+            done += same(sh.sel_mass);
+            __syncthreads();
+            id = level ? id << lower | (unsigned int)d : (unsigned int)d;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (q[e] && i[e] == id) {
+                p.a.ids[row] = i[e];
+                if (p.a.logprobs) p.a.logprobs[row] = (float)log(w[e] * 0x1p52 / sum);
+            }
+        return;
+    }
     // ---- what each chunk keeps: its whole bins, and its single tokens in steps of 2^-40 of the heaviest there may be
     __syncthreads();
     double *sums = sh.cum;                                                // (of up to kChunks)
@@ -807,9 +910,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (own > 0.) atomicMax(&sh.sel, tid);
         __syncthreads();
         c = same(sh.sel);
+        __syncthreads();
     }
     if (tid == c) sh.part = upto_c - own;
-    if (tid == 0) { sh.found = 0x7fffffff; sh.sel = -1; }
+    if (tid == 0) sh.sel = -1;
     __syncthreads();
     // ---- the token of that chunk: a thread's tokens are neighbours
     const int per = p.chunk / kPick, base = c * p.chunk + tid * per, end = min(p.V, c * p.chunk + p.chunk);      // 4 or 16
@@ -820,27 +924,39 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         const double w = weight(v, r.m, ask.c);
         return kept(b, key_of(v), (unsigned int)i, w) ? w : 0.;
     };
+    float4_t f[4];
     double here_sum = 0.;
-    for (int j = 0; j < per; j += 4) {
-        const float4_t f = four(r.x, base + j, end, p.whole);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) here_sum += of(f[e], base + j + e);
+    for (int j = 0; j < 4; ++j) f[j] = four(r.x, base + 4 * j, 4 * j < per ? end : 0, p.whole);
+#pragma unroll 1
+    for (int j = 0; 4 * j < per; ++j) {                                   // (not unrolled: code that runs once costs its way from memory)
+        const float4_t g = j & 2 ? j & 1 ? f[3] : f[2] : j & 1 ? f[1] : f[0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) here_sum += of(g[e], base + 4 * j + e);
     }
     const double upto = scan<double>(here_sum, sh.wsum);
-    double run = sh.part + (upto - here_sum);
-    if (here_sum > 0.) {
-        int hit = -1, any = -1;
-        for (int i = base; i < base + per && i < end; ++i) {
-            const double w = of(seen(r.x[i]), i);
-            run += w;
-            if (w > 0.) { any = i; if (hit < 0 && run > goal) hit = i; }
-        }
-        if (hit >= 0) atomicMin(&sh.found, hit);
-        if (any >= 0) atomicMax(&sh.sel, any);
+    int t = first_of(here_sum > 0. && sh.part + upto > goal);
+    if (t == kBins) {
+        if (here_sum > 0.) atomicMax(&sh.sel, tid);
+        __syncthreads();
+        t = same(sh.sel);
+    }
+    float *values = reinterpret_cast<float *>(sh.key);                    // of thread t: the first wave looks at them, a lane a token
+    if (tid == t) {
+        sh.cum[0] = sh.part + (upto - here_sum);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4_t *>(values + 4 * j) = f[j];
+    }
+    __syncthreads();
+    if (wave == 0 && t >= 0) {
+        const double w = lane < per ? of(values[lane & 15], c * p.chunk + t * per + lane) : 0., run = sh.cum[0] + wave_scan(w);
+        const unsigned long long any = __ballot(w > 0.), hit = __ballot(w > 0. && run > goal);
+        const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)any);      // (sums in another order may end a rounding below the goal: the last one)
+        if (lane == 0) sh.found = c * p.chunk + t * per + l;
     }
     __syncthreads();
     if (tid == 0) {
-        const int id = sh.found != 0x7fffffff ? sh.found : sh.sel;         // (the sums of the chunk in another order may end a rounding below the goal: its last token)
+        const int id = t < 0 ? -1 : sh.found;
         p.a.ids[row] = id;
         if (p.a.logprobs) p.a.logprobs[row] = id < 0 ? -INFINITY : (float)log(weight(seen(r.x[id]), r.m, ask.c) / sum);
     }
