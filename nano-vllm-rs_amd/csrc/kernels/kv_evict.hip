@@ -7,6 +7,7 @@
 #include <algorithm>
 #include "serving.h"
 #include "elem.h"
+#include "scan.h"
 #include "../common.h"
 
 namespace nvr { namespace kx {
@@ -41,11 +42,11 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     __shared__ __attribute__((aligned(16))) float held[kHeld];            // scores of keys 0 .. kHeld - 1
     __shared__ unsigned int hist[3][kRadix];
-    __shared__ unsigned int waves[3][16], above[3];
+    __shared__ unsigned int waves[16], above[3];
     __shared__ unsigned long long waves2[16];
     __shared__ int found[3];
     const EvictArgs &a = p.a;
-    const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int len = length_of(a, b), n = min(len, a.budget);
     const int32_t *table = a.block_tables + (int64_t)b * a.max_blocks, *to = a.to_tables ? a.to_tables + (int64_t)b * a.to_max_blocks : table;
     int32_t *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
@@ -95,15 +96,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
             for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass][wide - 1 - ((k >> at) & (wide - 1))], 1u); }
             __syncthreads();
             const unsigned int c0 = hist[pass][2 * tid], c1 = hist[pass][2 * tid + 1];
-            unsigned int v = c0 + c1;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) { const unsigned int o = __shfl_up(v, d); if (lane >= d) v += o; }
-            if (lane == 63) waves[pass][wave] = v;
-            __syncthreads();
-            unsigned int before = lane < wave ? waves[pass][lane & 15] : 0;
-#pragma unroll
-            for (int d = 8; d > 0; d >>= 1) before += __shfl_xor(before, d);
-            v += __builtin_amdgcn_readlane(before, 0) - c0 - c1;          // in front of this thread's two digits
+            const unsigned int v = scan<unsigned int>(c0 + c1, waves) - c0 - c1;      // in front of this thread's two digits
             if (v < want && v + c0 + c1 >= want) {                        // (one thread)
                 const bool odd = v + c0 < want;
                 found[pass] = 2 * tid + odd; above[pass] = odd ? v + c0 : v;
@@ -121,14 +114,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
         const unsigned int k = always ? 0 : rank_of(score(i));
         more += always || (need && k > prefix); same += !always && need && k == prefix;
     }
-    unsigned long long v = ((unsigned long long)more << 32) | same;
-    const unsigned long long own = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const unsigned long long o = __shfl_up(v, d); if (lane >= d) v += o; }
-    if (lane == 63) waves2[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) v += waves2[w];
-    v -= own;
+    const unsigned long long own = ((unsigned long long)more << 32) | same, v = scan<unsigned long long>(own, waves2) - own;
     // the scores at their new places: at once where LDS has them all
     const bool together = len <= kHeld;
     unsigned int seen = (unsigned int)v, at = (unsigned int)(v >> 32) + min(seen, want);

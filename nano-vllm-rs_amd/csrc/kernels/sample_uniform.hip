@@ -4,8 +4,9 @@
 // With m the row's largest logit, token i has the weight w_i = exp((x_i - m) / T).  All three filters keep a prefix of the tokens in descending order (ties: ascending index), so a row's
 // answer is decided by two numbers: where the prefix ends, and the sum of its weights.  Nothing is sorted.  The first launch reads the logits once, a chunk of a row a workgroup, and leaves the chunk's
 // maximum, its weights (and, for top-k, tokens) in bins of 1/24 of x / T, and a list of its largest tokens.  The second, a workgroup a row, adds the chunks' bins up and finds the bin that the prefix
-// ends in.  If the lists have all tokens down to that bin and they are few (kDirect), it sorts those and is done, without the bins; else it settles the order inside the bin by a radix select over
-// (logit, index), finds the chunk that the drawn number falls into, and walks that one.
+// ends in.  If the lists have all tokens down to that bin, the chunks' bins are not read: of few tokens (kDirect) each counts what is in front of
+// it; up to kList of them stay in LDS, are settled inside the bin, and the drawn one is found by sums over the upper and the lower bits of the index.  Else the order inside the bin is settled by a
+// radix select over (logit, index), and the chunk that the drawn number falls into is walked.
 // A token's index is an answer that has to be right to the last bit, so weights are 64-bit numbers and are summed as integers, so that the order of the atomics changes nothing: with
 // t = 24 x / T in 64 bits, a token lies in the cell of the whole number next to t and adds exp((t - cell) / 24), 0.98 to 1.02, in steps of 2^-40 to it (a polynomial of degree 5, 1e-13 off); a cell
 // counts exp(cell / 24).
@@ -17,6 +18,7 @@
 #include "device_utils.h"
 #include "../common.h"
 #include "elem.h"
+#include "scan.h"
 
 namespace nvr { namespace kx {
 
@@ -119,50 +121,6 @@ __device__ __forceinline__ float4_t four(const float *x, int i, int end, bool wh
     for (int e = 0; e < 4; ++e) v[e] = seen(v[e]);
     return v;
 }
-// x of the lane that CTRL names, 0 where there is none or the row is not in ROWS (32 and 64 bits)
-template <int CTRL, int ROWS, class T>
-__device__ __forceinline__ T moved(T x) {
-    if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
-    } else {
-        const long long v = __builtin_bit_cast(long long, x);
-        const unsigned int lo = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false), hi = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
-        return __builtin_bit_cast(T, (long long)(((unsigned long long)hi << 32) | lo));
-    }
-}
-template <class T>
-__device__ __forceinline__ T row_scan(T v) {                              // over the lanes of a row of 16 up to and with this one: row_shr 1, 2, 4, 8
-    v += moved<0x111, 0xf>(v); v += moved<0x112, 0xf>(v); v += moved<0x114, 0xf>(v); v += moved<0x118, 0xf>(v);
-    return v;
-}
-template <class T>
-__device__ __forceinline__ T from_lane(T x, int l) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
-    else {
-        const long long v = __builtin_bit_cast(long long, x);
-        const unsigned int lo = (unsigned int)__builtin_amdgcn_readlane((int)v, l), hi = (unsigned int)__builtin_amdgcn_readlane((int)(v >> 32), l);
-        return __builtin_bit_cast(T, (long long)(((unsigned long long)hi << 32) | lo));
-    }
-}
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {                             // ... of the wave: the rows' last lanes to the rows behind (row_bcast 15 and 31)
-    v = row_scan(v);
-    v += moved<0x142, 0xa>(v); v += moved<0x143, 0xc>(v);
-    return v;
-}
-// sum over the threads up to and with this one; `waves`: one of LDS a wave (16 at most)
-template <class T>
-__device__ __forceinline__ T scan(T v, T *waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v);
-    __syncthreads();
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    return from_lane(row_scan(lane < wave ? waves[lane & 15] : (T)0), 15) + v;
-}
-// x where every lane has the same: in scalar registers (what comes out of LDS the compiler takes for different ones, and branches on it for a branch a lane)
-template <class T>
-__device__ __forceinline__ T same(T x) { return from_lane(x, 0); }
 __device__ __forceinline__ unsigned int wave_largest(unsigned int v) {
     v = max(v, moved<0x111, 0xf>(v)); v = max(v, moved<0x112, 0xf>(v)); v = max(v, moved<0x114, 0xf>(v)); v = max(v, moved<0x118, 0xf>(v));
     v = max(v, moved<0x142, 0xa>(v)); v = max(v, moved<0x143, 0xc>(v));
@@ -349,7 +307,8 @@ __global__ __launch_bounds__(THREADS, 8) void sample_scan_kernel(SampleParams p)
 }
 
 namespace {
-constexpr int kDirect = 128, kCount = 256, kChunks = 1024;
+constexpr int kDirect = 256, kCount = 256, kChunks = 1024;
+static_assert(kDirect <= 4 * 64, "waves that hold tokens");
 struct PickShared {
     double cum[kBins];                                                    // weight of the bins up to and with this one
     unsigned int cum_n[kBins];
@@ -578,18 +537,6 @@ struct Row {
         }
         index = at_prefix;
     }
-    // v[0 .. size) ascending, up to kDirect of them: a number's place is how many are smaller
-    __device__ __forceinline__ void sort(unsigned long long *v, int size) {
-        const int t = threadIdx.x;
-        const unsigned long long a = t < size ? v[t] : 0;
-        int at = 0;
-        if (t < size)
-#pragma unroll 8
-            for (int j = 0; j < size; ++j) { const unsigned long long b = v[j]; at += b < a || (b == a && j < t); }
-        __syncthreads();
-        if (t < size) v[at] = a;
-        __syncthreads();
-    }
 };
 }  // namespace
 
@@ -684,58 +631,51 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         if (here) { r.from = 0; r.to = r.listed; }
         if (from_lists && few > kDirect && few <= kList) in_lds = r.gather(0, reach);
         if (from_lists && few <= kDirect) {
-            unsigned long long *v = sh.rmass;
-            int size = 64;
-            while (size < few) size *= 2;
-            if (tid == 0) sh.sel = 0;
+            // ---- few: a thread a token, each counts what is in front of it and its weight (whole numbers of 2^-52, 1 at least), by the logits and then by the indices
+            ulonglong2 *t = reinterpret_cast<ulonglong2 *>(sh.rmass);     // (what sorts by descending logits and ascending indices, weight)
+            if (tid == 0) { sh.sel = 0; sh.low = 0xffffffffu; sh.high = 0; }
             __syncthreads();
-            auto take = [&](unsigned int key, unsigned int i, float f, int b) { if (b <= reach) v[atomicAdd(&sh.sel, 1)] = ((unsigned long long)~key << 32) | i; };
-            if (here) { for (unsigned int i = tid; i < sh.n; i += kPick) { const float f = of_key(sh.key[i]); take(sh.key[i], sh.idx[i], f, bin_of(f, r.m, ask.inv)); } }
+            auto take = [&](unsigned int key, unsigned int i, float, int b) { if (b <= reach) t[atomicAdd(&sh.sel, 1)].x = ((unsigned long long)~key << 32) | i; };
+            if (here) r.each_gathered(true, 0, reach, take);
             else r.each_listed(0, reach, take);
             __syncthreads();
-            const int n = same(sh.sel);                                   // (few)
-            for (int i = n + tid; i < size; i += kPick) v[i] = ~0ull;
+            const int n = same(sh.sel);
+            const unsigned long long mine_v = tid < n ? t[tid].x : 0;
+            const unsigned int id = (unsigned int)mine_v;
+            const double x = tid < n ? weight(of_key(~(unsigned int)(mine_v >> 32)), r.m, ask.c) : 0.;
+            unsigned long long q = tid < n ? max(1ull, (unsigned long long)(x * 0x1p52 + 0.5)) : 0, upto = 0, all = 0;
+            if (tid < n) t[tid].y = q;
             __syncthreads();
-            r.sort(v, size);                                              // descending logits, ascending indices
-            auto at = [&](int i) { return i < n ? v[i] : ~0ull; };
-            const unsigned long long a0 = at(2 * tid), a1 = at(2 * tid + 1);
-            const unsigned int k0 = ~(unsigned int)(a0 >> 32), k1 = ~(unsigned int)(a1 >> 32);
-            const double w0 = 2 * tid < n ? weight(of_key(k0), r.m, ask.c) : 0., w1 = 2 * tid + 1 < n ? weight(of_key(k1), r.m, ask.c) : 0.;
-            int end = ask.k ? min((int)k, n) : n;                         // ranks that are kept
+            int rank = 0;
+            if (tid < n)
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) { const ulonglong2 o = t[j]; const bool in = o.x <= mine_v; rank += in; upto += in ? o.y : 0; }
+            bool keep = tid < n && (!ask.k || rank <= (int)k);
             if (ask.p < 1.f) {
-                const double v0 = 2 * tid < end ? w0 : 0., v1 = 2 * tid + 1 < end ? w1 : 0., upto = scan<double>(v0 + v1, sh.wsum);
-                if (tid == kPick - 1) sh.part = upto;
-                __syncthreads();
-                const double goal = (double)ask.p * (ask.k ? sh.part : everything);
-                const int t = first_of(2 * tid < end && upto >= goal);
-                if (tid == t) sh.nsel = upto - v1 >= goal || 2 * tid + 1 >= end ? 1 : 2;
-                __syncthreads();
-                if (t < kBins) end = min(end, 2 * t + same((int)sh.nsel));
+                double total = everything * 0x1p52;
+                if (ask.k) {
+                    const unsigned long long of_wave = wave_total(keep ? q : 0);
+                    if (lane == 0) sh.wsum64[wave] = of_wave;
+                    __syncthreads();
+                    total = (double)(sh.wsum64[0] + sh.wsum64[1] + sh.wsum64[2] + sh.wsum64[3]);
+                }
+                keep = keep && (rank == 1 || (double)(upto - q) < (double)ask.p * total);
             }
-            const bool in0 = 2 * tid < end && !(ask.min_p > 0.f && w0 < (double)ask.min_p), in1 = 2 * tid + 1 < end && !(ask.min_p > 0.f && w1 < (double)ask.min_p);
+            keep = keep && !(ask.min_p > 0.f && x < (double)ask.min_p);
+            if (!keep) q = 0;
             __syncthreads();
-            if (2 * tid < size) { v[2 * tid] = in0 ? (a0 << 32) | k0 : ~0ull; v[2 * tid + 1] = in1 ? (a1 << 32) | k1 : ~0ull; }
+            if (tid < n) t[tid].y = q;
             __syncthreads();
-            r.sort(v, size);                                              // the kept ones by their indices
-            const unsigned long long b0 = at(2 * tid), b1 = at(2 * tid + 1);
-            const double x0 = b0 != ~0ull ? weight(of_key((unsigned int)b0), r.m, ask.c) : 0., x1 = b1 != ~0ull ? weight(of_key((unsigned int)b1), r.m, ask.c) : 0.;
-            const double upto = scan<double>(x0 + x1, sh.wsum);
-            if (tid == kPick - 1) sh.part = upto;
-            __syncthreads();
-            const double sum = same(sh.part), goal = u * sum;
-            int t = first_of(x0 + x1 > 0. && upto > goal);
-            const bool beyond = t == kBins;                               // (no goal below the sum: the last one)
-            if (beyond) {
-                if (tid == 0) sh.sel = 0;
-                __syncthreads();
-                if (x0 + x1 > 0.) atomicMax(&sh.sel, tid);
-                __syncthreads();
-                t = same(sh.sel);
+            upto = 0;
+            if (tid < n) {
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) { const ulonglong2 o = t[j]; all += o.y; upto += (unsigned int)o.x <= id ? o.y : 0; }
+                if (q) { if ((double)upto > u * (double)all) atomicMin(&sh.low, id); atomicMax(&sh.high, id); }
             }
-            if (tid == t) {
-                const bool one = beyond ? !(x1 > 0.) : x0 > 0. && upto - x1 > goal;
-                p.a.ids[row] = (int64_t)((one ? b0 : b1) >> 32);
-                if (p.a.logprobs) p.a.logprobs[row] = (float)log((one ? x0 : x1) / sum);
+            __syncthreads();
+            if (q && id == (sh.low != 0xffffffffu ? sh.low : sh.high)) {  // (no goal below the sum: the last one)
+                p.a.ids[row] = id;
+                if (p.a.logprobs) p.a.logprobs[row] = (float)log(x * 0x1p52 / (double)all);
             }
             return;
         }
