@@ -13,23 +13,28 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kPick = 1024, kHeld = 9216, kRadix = 2048;
+constexpr int kPick = 1024, kHeld = 9216, kRadix = 2048, kTable = 512;
 struct EvictParams {
     EvictArgs a;
     int32_t *kept;                                                        // [B][KVH][budget]
-    int32_t row_bytes, strip, rows;                                       // of a key's row of a head; bytes of it that a workgroup moves; rows of a step
+    int32_t row_bytes, strip;                                             // of a key's row of a head; bytes of it that a workgroup moves
+    uint32_t per_block;                                                   // 2^32 / block_size, rounded down
 };
+// j / block_size and what is left, without a division: the product's upper half is at most one short
+struct Slot { int block, row; };
+__device__ __forceinline__ Slot slot_of(const EvictParams &p, int j) {
+    Slot s;
+    s.block = (int)__umulhi((unsigned)j, p.per_block); s.row = j - s.block * p.a.block_size;
+    if (s.row >= p.a.block_size) { ++s.block; s.row -= p.a.block_size; }
+    return s;
+}
 __device__ __forceinline__ int length_of(const EvictArgs &a, int b) {
     const long long most = (long long)a.max_blocks * a.block_size;
     return (int)max(0ll, min((long long)min(a.ctx_lens[b], a.max_ctx), most));
 }
-__device__ __forceinline__ int row_in(const int32_t *table, int block_size, int j) {
-    const int block = (int)((unsigned)j / (unsigned)block_size);
-    return table[block] * block_size + (j - block * block_size);
-}
-__device__ __forceinline__ int64_t score_at(const EvictArgs &a, const int32_t *table, int g, int j) {
-    const int block = (int)((unsigned)j / (unsigned)a.block_size);
-    return ((int64_t)table[block] * a.KVH + g) * a.block_size + (j - block * a.block_size);
+__device__ __forceinline__ int row_in(const EvictParams &p, const int32_t *table, int j) {
+    const Slot s = slot_of(p, j);
+    return table[s.block] * p.a.block_size + s.row;
 }
 // larger score, larger number; not a number: below all
 __device__ __forceinline__ unsigned int rank_of(float f) {
@@ -41,7 +46,8 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     __shared__ __attribute__((aligned(16))) float held[kHeld];            // scores of keys 0 .. kHeld - 1
-    __shared__ unsigned int hist[3][kRadix];
+    __shared__ unsigned int hist[2 * kRadix + kRadix / 2];                // 11, 11 and 10 bits
+    __shared__ int32_t from_table[kTable], to_table[kTable];              // (the first kTable blocks of each)
     __shared__ unsigned int waves[16], above[3];
     __shared__ unsigned long long waves2[16];
     __shared__ int found[3];
@@ -52,12 +58,16 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     int32_t *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
     // a sequence whose tables name a block outside the pool, or too few, stays as it is
     int bad = a.to_tables && (long long)a.to_max_blocks * a.block_size < n;
-    for (int i = tid; i < (len + a.block_size - 1) / a.block_size; i += kPick) bad |= table[i] < 0 || table[i] >= a.num_blocks;
-    if (a.to_tables && !bad)
-        for (int i = tid; i < (n + a.block_size - 1) / a.block_size; i += kPick) bad |= to[i] < 0 || to[i] >= a.num_blocks;
-#pragma unroll
-    for (int q = 0; q < 3; ++q)
-        for (int i = tid; i < kRadix; i += kPick) hist[q][i] = 0;
+    auto look = [&](const int32_t *t, int32_t *lds, int keys) {
+        for (int i = tid; i < (keys + a.block_size - 1) / a.block_size; i += kPick) {
+            const int block = t[i];
+            bad |= block < 0 || block >= a.num_blocks;
+            if (i < kTable) lds[i] = block;
+        }
+    };
+    look(table, from_table, len);
+    if (!bad) look(to, to_table, n);
+    for (int i = tid; i < 2 * kRadix + kRadix / 2; i += kPick) hist[i] = 0;
     if (__syncthreads_or(bad)) {
         if (g == 0 && tid == 0) a.new_lens[b] = -1;
         for (int i = tid; i < a.budget; i += kPick) kept[i] = -1;
@@ -70,20 +80,26 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
         for (int i = tid; i < n; i += kPick) kept[i] = i;
         return;
     }
+    auto place = [&](const int32_t *t, const int32_t *lds, int j) {
+        const Slot s = slot_of(p, j);
+        return ((int64_t)(s.block < kTable ? lds[s.block] : t[s.block]) * a.KVH + g) * a.block_size + s.row;
+    };
+    auto from_at = [&](int j) { return place(table, from_table, j); };
+    auto to_at = [&](int j) { return place(to, to_table, j); };
     // ---- the scores into LDS, 4 neighbours a thread where blocks are multiples of 4
     const int here = min(len, kHeld);
     if (a.block_size % 4 == 0 && ((uintptr_t)a.scores & 15) == 0) {
         for (int i0 = tid * 4; i0 < here; i0 += kPick * 8) {
             float4_t v[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { const int i = i0 + u * kPick * 4; if (i < here) v[u] = *reinterpret_cast<const float4_t *>(a.scores + score_at(a, table, g, i)); }
+            for (int u = 0; u < 2; ++u) { const int i = i0 + u * kPick * 4; if (i < here) v[u] = *reinterpret_cast<const float4_t *>(a.scores + from_at(i)); }
 #pragma unroll
             for (int u = 0; u < 2; ++u) { const int i = i0 + u * kPick * 4; if (i < here) *reinterpret_cast<float4_t *>(held + i) = v[u]; }
         }
     } else
-        for (int i = tid; i < here; i += kPick) held[i] = a.scores[score_at(a, table, g, i)];
+        for (int i = tid; i < here; i += kPick) held[i] = a.scores[from_at(i)];
     __syncthreads();
-    auto score = [&](int i) { return i < kHeld ? held[i] : a.scores[score_at(a, table, g, i)]; };
+    auto score = [&](int i) { return i < kHeld ? held[i] : a.scores[from_at(i)]; };
     // ---- the rank of the last of the best: the `need` best of keys first .. end - 1, of equal ones the earliest `want`
     const int first = a.first, end = len - a.last;
     const unsigned int need = all ? 0 : a.budget - a.first - a.last;      // (fewer than compete)
@@ -93,9 +109,9 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
         prefix = 0; want = need;
         for (int pass = 0; pass < 3; ++pass) {
             const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
-            for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass][wide - 1 - ((k >> at) & (wide - 1))], 1u); }
+            for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass * kRadix + wide - 1 - ((k >> at) & (wide - 1))], 1u); }
             __syncthreads();
-            const unsigned int c0 = hist[pass][2 * tid], c1 = hist[pass][2 * tid + 1];
+            const unsigned int c0 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid] : 0, c1 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid + 1] : 0;
             const unsigned int v = scan<unsigned int>(c0 + c1, waves) - c0 - c1;      // in front of this thread's two digits
             if (v < want && v + c0 + c1 >= want) {                        // (one thread)
                 const bool odd = v + c0 < want;
@@ -125,7 +141,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
         const bool tie = !always && need && k == prefix;
         if (always || (need && k > prefix) || (tie && seen < want)) {
             kept[at] = i;
-            if (together) a.scores[score_at(a, to, g, (int)at)] = f;
+            if (together) a.scores[to_at((int)at)] = f;
             ++at;
         }
         seen += tie;
@@ -136,10 +152,10 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     for (int j0 = 0; j0 < n; j0 += kPick) {                               // from the front: of a step all are read before any is written
         const int i = j0 + tid;
         float f = 0.f;
-        if (i < n) f = a.scores[score_at(a, table, g, kept[i])];
+        if (i < n) f = a.scores[from_at(kept[i])];
         asm volatile("" : "+v"(f));
         __syncthreads();
-        if (i < n) a.scores[score_at(a, to, g, i)] = f;
+        if (i < n) a.scores[to_at(i)] = f;
     }
 }
 
@@ -160,7 +176,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
 #pragma unroll
         for (int u = 0; u < kMoves; ++u) {
             const int i = i0 + u * rows + lead;
-            if (lead < rows && i < n) { const int j = kept[i]; if (j != i) v[u] = *reinterpret_cast<const float4_t *>(pool + row_in(table, a.block_size, j) * row + off); }
+            if (lead < rows && i < n) { const int j = kept[i]; if (j != i) v[u] = *reinterpret_cast<const float4_t *>(pool + row_in(p, table, j) * row + off); }
         }
     };
     request(0);
@@ -173,7 +189,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
 #pragma unroll
         for (int u = 0; u < kMoves; ++u) {
             const int i = i0 + u * rows + lead;
-            if (lead < rows && i < n && kept[i] != i) *reinterpret_cast<float4_t *>(pool + row_in(table, a.block_size, i) * row + off) = w[u];
+            if (lead < rows && i < n && kept[i] != i) *reinterpret_cast<float4_t *>(pool + row_in(p, table, i) * row + off) = w[u];
         }
     }
 }
@@ -191,7 +207,7 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(EvictParams p) {
 #pragma unroll
     for (int u = 0; u < kMoves; ++u) {
         const int i = min(i0 + u * rows + lead, n - 1);
-        const int64_t at = row_in(table, a.block_size, kept[i]) * row + off;
+        const int64_t at = row_in(p, table, kept[i]) * row + off;
         k[u] = *reinterpret_cast<const float4_t *>((const char *)a.k + at);
         v[u] = *reinterpret_cast<const float4_t *>((const char *)a.v + at);
     }
@@ -199,7 +215,7 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(EvictParams p) {
     for (int u = 0; u < kMoves; ++u) {
         const int i = i0 + u * rows + lead;
         if (i >= n) break;
-        const int64_t at = row_in(to, a.block_size, i) * row + off;
+        const int64_t at = row_in(p, to, i) * row + off;
         *reinterpret_cast<float4_t *>((char *)a.k + at) = k[u];
         *reinterpret_cast<float4_t *>((char *)a.v + at) = v[u];
     }
@@ -227,6 +243,7 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     p.a = a;
     p.kept = a.kept ? a.kept : (int32_t *)a.workspace;
     p.row_bytes = (int32_t)bytes;
+    p.per_block = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / (uint64_t)a.block_size);
     p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
     const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
     kv_evict_select_kernel<<<dim3(G, B), kPick, 0, s>>>(p);
