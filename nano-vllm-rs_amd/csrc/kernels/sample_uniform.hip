@@ -14,6 +14,8 @@
 // What a chunk cannot contribute is left out by one comparison a token: with top-k, whatever lies below the k-th of the chunk's maxima of 8 neighbours (there are k tokens above it), with min-p
 // alone, whatever lies below min_p of the chunk's maximum.
 #include <algorithm>
+#include <cfloat>
+#include <type_traits>
 #include "serving.h"
 #include "device_utils.h"
 #include "../common.h"
@@ -361,28 +363,36 @@ struct Row {
                 }
         }
     }
-    // ... in the row itself.  Most tokens are outside: two comparisons with the bins' ends (a little beyond, for their roundings) come first
+    // ... in the row itself.  Most tokens are outside: the signs of x less the bins' lower end and the upper end less x (a little beyond, for their roundings) tell, four instructions a token.
+    // Numbers that are none may pass here
     template <class F>
     __device__ __forceinline__ void each_of_row(int lo, int hi, F f) const {
         const double top = ((double)m * ask.inv + kWhole) - kWhole;       // (the cells' ends are halves)
         const float a = (float)((top - hi - 0.5) / ask.inv), z = (float)((top - lo + 0.5) / ask.inv);
         const bool lone = lonely(m, ask.inv);
-        const float least = lone ? m : a - fabsf(a) * 1e-6f, most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
-        const bool all = !(least == least && most == most);               // (1 / inv beyond float)
+        float least = fminf(lone ? m : a - fabsf(a) * 1e-6f, FLT_MAX), most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
+        if (!(least == least && most == most)) { least = -INFINITY; most = INFINITY; }      // (1 / inv beyond float)
         for (int i0 = threadIdx.x * 4; i0 < p.V; i0 += kPick * 16) {
-            float4_t v[4];
+            float v[16];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = four(x, i0 + u * kPick * 4, p.V, p.whole);
-            unsigned int near = 0;                                        // the few that may be meant, one a lane at a time: a wave comes here as often as its busiest lane
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * kPick * 4;
+                float4_t w;
+                if (p.whole && i + 4 <= p.V) w = *reinterpret_cast<const float4_t *>(x + i);
+                else
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { const float w = v[e >> 2][e & 3]; near |= (w != -INFINITY && (all || (w >= least && w <= most)) ? 1u : 0u) << e; }
-            float flat[16];
+                    for (int e = 0; e < 4; ++e) w[e] = i + e < p.V ? x[i + e] : -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) flat[e] = v[e >> 2][e & 3];
+                for (int e = 0; e < 4; ++e) v[4 * u + e] = w[e];
+            }
+            unsigned int outside = 0;
+#pragma unroll
+            for (int e = 15; e >= 0; --e) outside = __builtin_amdgcn_alignbit(outside, __float_as_uint(fminf(v[e] - least, most - v[e])), 31);
+            unsigned int near = ~outside & 0xffffu;                       // one a lane at a time: a wave comes to f as often as its busiest lane
             while (near) {
                 const int j = __ffs((int)near) - 1;
                 near &= near - 1;
-                const float w = pick_of(flat, j);
+                const float w = seen(pick_of(v, j));
                 const int b = bin_of(w, m, ask.inv);
                 if (b >= lo && b <= hi && b < kBins - 1) f(key_of(w), (unsigned int)(i0 + (j >> 2) * kPick * 4 + (j & 3)), w, b);
             }
@@ -703,18 +713,20 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         unsigned long long in_bin = sh.rmass[tid];
         unsigned int cnt = sh.rcnt[tid];
         for (int c0 = 0; c0 < p.P; c0 += 16) {                            // (16 chunks' requests together)
-            unsigned long long q[16];
-            unsigned int n[16];
+            auto of_chunks = [&](const auto *table, auto &sum) {
+                auto q = std::remove_reference_t<decltype(sum)>(0);
+                std::remove_reference_t<decltype(sum)> v[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int c = min(c0 + e, p.P - 1), b = tid - sh.shift[c];
-                const bool in = c0 + e < p.P && b >= 0 && b < sh.binned[c] && tid < kBins - 1;
-                const int64_t at = ((int64_t)row * p.P + c) * kBins + b;
-                q[e] = in ? p.mass[at] : 0;
-                n[e] = in && ask.k ? p.cnt[at] : 0;
-            }
+                for (int e = 0; e < 16; ++e) {
+                    const int c = min(c0 + e, p.P - 1), b = tid - sh.shift[c];
+                    v[e] = c0 + e < p.P && b >= 0 && b < sh.binned[c] && tid < kBins - 1 ? table[((int64_t)row * p.P + c) * kBins + b] : 0;
+                }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { in_bin += q[e]; cnt += n[e]; }
+                for (int e = 0; e < 16; ++e) q += v[e];
+                sum += q;
+            };
+            of_chunks(p.mass, in_bin);
+            if (ask.k) of_chunks(p.cnt, cnt);
         }
         sh.cum[tid] = scan<double>((double)in_bin * unit_of_bin, sh.wsum);
         sh.cum_n[tid] = scan<unsigned int>(cnt, sh.wcnt);
