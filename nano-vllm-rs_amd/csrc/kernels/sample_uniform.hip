@@ -73,13 +73,13 @@ __device__ __forceinline__ double exp2_64(double t) {
 }
 __device__ __forceinline__ double weight(float x, float m, double c) { return x == m ? 1.0 : exp2_64(((double)x - (double)m) * c); }
 // exp(f / 24) in steps of 2^-40, |f| <= 1/2: the series, every term 2^40 times as large, on top of 2^52: the integer is then the number's low bits
-__device__ __forceinline__ unsigned long long in_cell(double f) {
+__device__ __forceinline__ double above_2_52(double f) {
     constexpr double one = 1099511627776.0;
     double s = one / (120. * 24 * 24 * 24 * 24 * 24);
     s = fma(s, f, one / (24. * 24 * 24 * 24 * 24)); s = fma(s, f, one / (6. * 24 * 24 * 24)); s = fma(s, f, one / (2. * 24 * 24)); s = fma(s, f, one / 24.);
-    s = fma(s, f, one + 4503599627370496.0);
-    return (unsigned long long)__double_as_longlong(s) & 0xfffffffffffffull;
+    return fma(s, f, one + 4503599627370496.0);
 }
+__device__ __forceinline__ unsigned long long in_cell(double f) { return (unsigned long long)__double_as_longlong(above_2_52(f)) & 0xfffffffffffffull; }
 // A maximum that nothing but its equals is near: infinite, or so large that the next number is 2^26 cells away
 __device__ __forceinline__ bool lonely(float m, double inv) { return !(fabs((double)m * inv) < 1125899906842624.); }
 // bin of x below the maximum m (kBins - 1 and beyond: left out): cells are whole numbers, so bins under a chunk's maximum are a shift away from those under the row's
@@ -694,8 +694,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     // ---- many: the row's bins, thread b bin b: those of the lists, or from the chunks', or, of the chunks that left none, from their lists
     int stop = kBins;                                                     // bins in front of it are kept whole; of this one, tokens down to (key, index)
     unsigned int key = 0, index = 0xffffffffu;
-    double unit_of_bin = 0.;
-    if (filtered) unit_of_bin = r.cell(tid);
+    const double unit_of_bin = r.cell(tid);
     if (filtered && !from_lists) {
         sh.rmass[tid] = 0; sh.rcnt[tid] = 0;
         __syncthreads();
@@ -840,11 +839,14 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                 for (int b = lane; b < min(sure - s, (int)sh.binned[c]); b += 64) v += (double)q[b] * units[b + s];
             } else {
                 const uint2 *q = p.near + ((int64_t)row * p.P + c) * kNear;
+                unsigned long long n = 0;                                 // (a list's order is that of its arrival: whole numbers of 2^-52, 1 at least)
                 for (int i = lane; i < sh.near[c]; i += 64) {
                     const float f = of_key(q[i].x);
                     const int b = bin_of(f, r.m, ask.inv);
-                    if (b < sure && b < kBins - 1) v += (double)r.inside(f) * units[b];
+                    if (b < sure && b < kBins - 1) n += max(1ull, (unsigned long long)((double)r.inside(f) * units[b] * 0x1p52 + 0.5));
                 }
+                const unsigned long long all = wave_total(n);
+                v = lane == 0 ? (double)all * 0x1p-52 : 0.;
             }
             v = wave_total(v) + (double)single[c] * unit;
         }
@@ -869,11 +871,14 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     __syncthreads();
     // ---- the token of that chunk: a thread's tokens are neighbours
     const int per = p.chunk / kPick, base = c * p.chunk + tid * per, end = min(p.V, c * p.chunk + p.chunk);      // 4 or 16
-    auto of = [&](float v, int i) {
-        if (v == -INFINITY) return 0.;
-        const int b = bin_of(v, r.m, ask.inv);
+    const bool lone = lonely(r.m, ask.inv);
+    const double t_m = (double)r.m * ask.inv, whole_m = t_m + kWhole;
+    auto of = [&](float v, int i) {                                       // the weight as the cell's times the place's inside: half the work of an exponential
+        if (v == -INFINITY || (lone && v != r.m)) return 0.;
+        const double at = fmax((double)v * ask.inv, t_m - 2. * kBins), whole = at + kWhole;
+        const int b = lone ? 0 : low_of(whole_m) - low_of(whole);
         if (b >= kBins - 1 || (filtered && b >= sure && b > last)) return 0.;
-        const double w = weight(v, r.m, ask.c);
+        const double w = lone ? 1. : (above_2_52(at - (whole - kWhole)) - 4503599627370496.0) * units[b];
         return kept(b, key_of(v), (unsigned int)i, w) ? w : 0.;
     };
     float4_t f[4];
@@ -893,7 +898,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         __syncthreads();
         t = same(sh.sel);
     }
-    float *values = reinterpret_cast<float *>(sh.key);                    // of thread t: the first wave looks at them, a lane a token
+    float *values = reinterpret_cast<float *>(sh.idx);                    // of thread t: the first wave looks at them, a lane a token
     if (tid == t) {
         sh.cum[0] = sh.part + (upto - here_sum);
 #pragma unroll

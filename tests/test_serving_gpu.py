@@ -862,3 +862,35 @@ def test_sample_of_many_short_rows(arena):
     rng = np.random.default_rng(8)
     check_sample(arena, rng.standard_normal((700, 33)) * 2, 1.0, 5, 0.9, 0.01, rng.random(700).astype(np.float32))
     check_sample(arena, rng.standard_normal((300, 17000)) * 2, 1.0, 0, 0.9, 0.0, rng.random(300).astype(np.float32))
+
+
+@pytest.mark.parametrize("B", [1, 256])
+def test_sample_long_prefixes(arena, B):
+    """Prefixes of hundreds to tens of thousands of tokens, alone and where chunks are large; twice, for the same bits."""
+    rng = np.random.default_rng(9)
+    V = 50257
+    x = rng.standard_normal((B, V)) * 2
+    x[:, rng.integers(0, V, 30)] += 7
+    for k, p, m in ((300, 1.0, 0.0), (1500, 0.9, 0.0), (5000, 1.0, 0.0), (20000, 0.97, 0.0), (0, 0.5, 0.0), (0, 0.99, 0.0), (0, 0.9, 0.0005), (0, 1.0, 0.0002), (2500, 0.999, 0.001)):
+        u = rng.random(B).astype(np.float32)
+        u[0] = 0 if B == 1 and k else u[0]
+        n = min(B, 24)
+        args = [np.broadcast_to(np.asarray(a, t), (B,)) for a, t in ((0.9, np.float32), (k, np.int64), (p, np.float32), (m, np.float32), (u, np.float32))]
+        ids, lp = sample_rows(arena, x.astype(np.float32), *args)
+        again = sample_rows(arena, x.astype(np.float32), *args)
+        assert np.array_equal(ids, again[0]) and np.array_equal(lp.view(np.uint32), again[1].view(np.uint32))
+        for r in range(n):
+            want = sample(x[r].astype(np.float32), float(np.float32(0.9)), k, float(np.float32(p)), float(np.float32(m)), float(u[r]))
+            assert ids[r] == want[0], (k, p, m, r)
+            assert abs(lp[r] - want[1]) <= 2.0 ** -23 * max(1, abs(want[1])), (k, p, m, r)
+
+
+def test_sample_whole_rows_of_equal_logits(arena):
+    """Every logit the same, and two values in turn: ends of prefixes are told by the index alone, in one bin of more tokens than LDS holds."""
+    rng = np.random.default_rng(10)
+    for V in (2049, 20000, 70001):
+        same = np.zeros((2, V), np.float32)
+        two = np.where(np.arange(V) % 2 == 0, 0.5, 0.5 + 1e-6).astype(np.float32)[None].repeat(2, 0)
+        for x in (same, two):
+            for k, p, m in ((0, 1.0, 0.0), (1, 1.0, 0.0), (1777, 1.0, 0.0), (0, 0.25, 0.0), (1999, 0.5, 0.0), (0, 1.0, 1.0), (V - 1, 1.0, 0.0)):
+                check_sample(arena, x, 1.0, k, p, m, rng.random(2).astype(np.float32))
