@@ -432,8 +432,8 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
 
 int lora_add(int dt, const LoraArgs &a, hipStream_t s) {
     if (a.T < 0 || a.K <= 0 || a.N <= 0 || a.R <= 0 || a.n < 0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: T=%ld K=%ld N=%ld R=%ld adapters=%ld", (long)a.T, (long)a.K, (long)a.N, (long)a.R, (long)a.n);
-    if (a.R > 256 || a.n >= kMaxAdapters || a.K > (1 << 24) || a.N > (1 << 24) || a.T > (1 << 24))
-        return nvr::fail(NVR_ERR_UNSUPPORTED, "nvr_lora_add: ranks up to 256, fewer than %d adapters, sizes up to 2^24 (T=%ld K=%ld N=%ld R=%ld adapters=%ld)", kMaxAdapters, (long)a.T, (long)a.K, (long)a.N, (long)a.R, (long)a.n);
+    if (a.R > 256 || a.n >= kMaxAdapters || a.K > (1 << 22) || a.N > (1 << 22) || a.T > (1 << 19))       // (tiles and groups of columns are grid axes of 65535)
+        return nvr::fail(NVR_ERR_UNSUPPORTED, "nvr_lora_add: ranks up to 256, fewer than %d adapters, 2^19 rows of up to 2^22 numbers (T=%ld K=%ld N=%ld R=%ld adapters=%ld)", kMaxAdapters, (long)a.T, (long)a.K, (long)a.N, (long)a.R, (long)a.n);
     if (a.T == 0) return 0;
     if (!a.x || !a.ids || !a.base || !a.y || !a.workspace || (a.n && (!a.A || !a.B))) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: null argument");
     if (((uintptr_t)a.workspace & 15) != 0) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_lora_add: the workspace is not aligned to 16 bytes");

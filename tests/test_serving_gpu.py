@@ -894,3 +894,9 @@ def test_sample_whole_rows_of_equal_logits(arena):
         for x in (same, two):
             for k, p, m in ((0, 1.0, 0.0), (1, 1.0, 0.0), (1777, 1.0, 0.0), (0, 0.25, 0.0), (1999, 0.5, 0.0), (0, 1.0, 1.0), (V - 1, 1.0, 0.0)):
                 check_sample(arena, x, 1.0, k, p, m, rng.random(2).astype(np.float32))
+
+
+@pytest.mark.parametrize("T,K,N,R,n", [(200000, 16, 16, 4, 5), (200000, 8, 16, 130, 3), (70000, 8, 40, 4, 5000)])
+def test_lora_of_many_rows(arena, T, K, N, R, n):
+    """More rows than one pass of the grouping takes, in tiles of 64 rows and of 16."""
+    lora_case(arena, "float16", T, K, N, R, n, np.random.default_rng(T + R).integers(-1, n, T))

@@ -76,6 +76,11 @@ def test_lora_refusals(change, name):
     refused("nvr_lora_add", name, *{**LORA, **change}.values())
 
 
+@pytest.mark.parametrize("change", [dict(T=(1 << 19) + 1), dict(N=(1 << 22) + 1, ldb=1 << 23, ldy=1 << 23), dict(K=(1 << 22) + 1, ldx=1 << 23)])
+def test_lora_sizes_that_no_grid_holds(change):
+    refused("nvr_lora_add", "NVR_ERR_UNSUPPORTED", *{**LORA, **change}.values())
+
+
 def test_lora_of_no_rows_or_adapters_is_nothing():
     assert nvr.lib().nvr_lora_add(*{**LORA, "T": 0}.values()) == 0
     assert nvr.lib().nvr_lora_add(*{**LORA, "n": 0, "A": None, "B": None, "y": P}.values()) == 0     # in place, no adapter: every row stays
