@@ -697,7 +697,7 @@ NVR_API int nvr_rope_rotate_store_kv(const nvr_half *q, int64_t ldq, const nvr_h
                                      void *stream);
 
 /* y[t] = base[t] + scales[a] (x[t] A_a^T) B_a^T with a = adapters[t]: what the adapter of row t's request adds to a shared projection (nvr_linear and its like wrote base; a part of a packed
- * projection is addressed by its pointer and ldb / ldy).  x [T, K], base and y [T, N] with strides ldx / ldb / ldy, base may be y itself; A [num_adapters, R, K], B [num_adapters, N, R];
+ * projection is addressed by its pointer and ldb / ldy).  x [T, K], base and y [T, N] with strides ldx / ldb / ldy, base or x may be y itself; A [num_adapters, R, K], B [num_adapters, N, R];
  * scales [num_adapters] f32, null: 1.  A row whose adapters[t] is not in 0 .. num_adapters - 1 has none: y[t] = base[t].  Rows may come in any order; ranks (R) up to 256, fewer than 8192 adapters, T up to 2^19, K and N up to 2^22.
  * The inner product stays in f32 (16-bit types: two numbers of 16 bits); y is rounded once.  workspace: nvr_lora_workspace_bytes. */
 NVR_API size_t nvr_lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R);

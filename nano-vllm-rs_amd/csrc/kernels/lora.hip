@@ -4,7 +4,8 @@
 // itself; more are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
 //   down: v = scale x A^T, the waves of a workgroup (and `splits` workgroups of few rows) share K; partial sums stay in 32 bits in the workspace, [split][row][rank]
 //   up:   y = base + v B^T; v in two 16-bit numbers (its rounding and the rounded rest), so that the product sees it in 16 (bfloat16) or 22 bits; the sum with base is rounded once
-// Both are bound by memory for prompts (x, base and y once; 2 R flops a byte) and by their two launches for decode steps.
+// Few rows of few ranks take one launch, in which every workgroup forms v anew for its columns.
+// Bound by memory for prompts (x, base and y once; 2 R flops a byte), by launches and a chain of round trips for decode steps.
 #include <algorithm>
 #include <type_traits>
 #include "serving.h"
@@ -143,19 +144,17 @@ struct Strip {
 };
 
 // D(rank x row) = A . x^T: a lane's 4 sums are neighbours in v.  The waves of a workgroup take the strips of its share of K in turn; the next one is on its way.
-template <class E, int MT, int RT, bool GROUPED, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
+// The waves' sums of ranks r0 .. r0 + 16 RT - 1 over share `split` of K are left in smem: [wave][tile of 16 rows x tile of 16 ranks][lane]
+template <int MT, int RT>
+constexpr int image_bytes() { return (MT + RT) * 16 * 128; }
+template <class E, int MT, int RT, int WAVES>
+__device__ __forceinline__ void down_sums(const LoraParams &p, const int *rows, int count, int adapter, int r0, int split, char *smem) {
     typedef typename E::T T; typedef typename E::V V;
     typedef Strip<E> S;
-    constexpr int TR = MT * 16, XN = MT * 2, AN = RT * 2, IMAGE = (MT + RT) * 16 * 128;
-    __shared__ int rows[TR];
-    __shared__ __attribute__((aligned(16))) char smem[WAVES * IMAGE];     // (then the waves' sums)
-    int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, adapter);
-    if (!count || adapter >= (int)p.a.n) return;
+    constexpr int XN = MT * 2, AN = RT * 2, IMAGE = image_bytes<MT, RT>();
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4, lr = lane >> 3, lp = lane & 7;
-    const int K = (int)p.a.K, R = (int)p.a.R, r0 = blockIdx.z * RT * 16;
-    const int strips = (K + S::CK - 1) / S::CK, per = (strips + p.splits - 1) / p.splits, first = blockIdx.y * per, last = min(strips, first + per);
+    const int K = (int)p.a.K, R = (int)p.a.R;
+    const int strips = (K + S::CK - 1) / S::CK, per = (strips + p.splits - 1) / p.splits, first = split * per, last = min(strips, first + per);
     const T *x[XN], *w[AN];
 #pragma unroll
     for (int u = 0; u < XN; ++u) { const int t = u * 8 + lr; x[u] = (const T *)p.a.x + (int64_t)rows[t < count ? t : 0] * p.a.ldx + lp * E::W; }
@@ -212,6 +211,18 @@ __global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
 #pragma unroll
     for (int i = 0; i < MT * RT; ++i) part[(wave * MT * RT + i) * 64 + lane] = acc[i / RT][i % RT];
     __syncthreads();
+}
+template <class E, int MT, int RT, bool GROUPED, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
+    constexpr int TR = MT * 16;
+    __shared__ int rows[TR];
+    __shared__ __attribute__((aligned(16))) char smem[WAVES * image_bytes<MT, RT>()];
+    int adapter = -1;
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, adapter);
+    if (!count || adapter >= (int)p.a.n) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4, r0 = blockIdx.z * RT * 16;
+    down_sums<E, MT, RT, WAVES>(p, rows, count, adapter, r0, blockIdx.y, smem);
+    const float4_t *part = reinterpret_cast<const float4_t *>(smem);
     const float scale = p.a.scales ? p.a.scales[adapter] : 1.f;
     for (int i = wave; i < MT * RT; i += WAVES) {
         const int m = i / RT, r = i % RT, t = m * 16 + lm;
@@ -224,66 +235,18 @@ __global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
 
 // D(column x row) = B . v^T: a lane's NT * 4 = W sums are neighbours in y (row m of tile i of B is column (m / 4) W + 4 i + m % 4 of the group).  A wave takes groups of NT * 16 columns, two at a time,
 // straight from and to memory: rows of 64 bytes a request, but no wait between.  (Through images as above, requests of whole rows: 93 -> 171 us for 8192 rows of 12288 columns of rank 32.)
-template <class E, int MT, bool GROUPED>
-__global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParams p, int groups) {
+// v in LDS: [hi, lo] [rows][ldv], 32 bits: [rows][ldv]; high: float16, bits of a row's largest |v|
+template <class E>
+constexpr int v_stride(int R) { return (R + E::KS - 1) / E::KS * E::KS + E::W; }      // (16 bytes off a multiple of 64: neighbours lie in other banks)
+template <class E, int MT>
+__device__ __forceinline__ void up_columns(const LoraParams &p, const int *rows, int count, int adapter, const typename E::T *hi, const unsigned int *high, int ldv, int g0, int groups) {
     typedef typename E::T T; typedef typename E::V V;
     constexpr int TR = MT * 16, W = E::W, NT = W / 4, GN = NT * 16;
     constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
-    extern __shared__ __attribute__((aligned(16))) char smem[];           // v: [hi, lo] [TR][ldv]; 32 bits: [TR][ldv]
-    __shared__ unsigned int high[TR];                                     // float16: bits of a row's largest |v|
-    __shared__ int rows[TR];
-    int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, adapter);
-    if (!count) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
-    const int R = (int)p.a.R, N = (int)p.a.N, ks = (R + E::KS - 1) / E::KS, ldv = ks * E::KS + W;    // (a row's stride is 16 bytes off a multiple of 64: neighbours lie in other banks)
+    const int lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
+    const int R = (int)p.a.R, N = (int)p.a.N, ks = (R + E::KS - 1) / E::KS;
     const bool real = adapter < (int)p.a.n;
-    T *hi = reinterpret_cast<T *>(smem), *lo = hi + TR * ldv;
-    if (real) {
-        const int per = ks * E::KS / 4;                                   // pieces of 4 sums; a thread has up to 8 (64 rows of rank 128, 16 of rank 256)
-        float4_t v[8];
-        if (H && threadIdx.x < TR) high[threadIdx.x] = 0;
-        if (H) __syncthreads();
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
-            v[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
-            if (i < TR * per && t < count && r < p.rp) {
-                const float *at = p.v + (int64_t)rows[t] * p.rp + r;
-                const int64_t next = p.a.T * p.rp;
-                int s = 0;
-                for (; s + 4 <= p.splits; s += 4, at += 4 * next) {
-                    float4_t q[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const float4_t *>(at + e * next);
-                    v[n] += (q[0] + q[1]) + (q[2] + q[3]);
-                }
-                for (; s < p.splits; ++s, at += next) v[n] += *reinterpret_cast<const float4_t *>(at);
-            }
-            float most = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (r + e >= R) v[n][e] = 0.f;                            // (behind R there are repeats of the last row of A)
-                most = fmaxf(most, fabsf(v[n][e]));
-            }
-            if (H && i < TR * per) atomicMax(&high[t], __float_as_uint(most));
-        }
-        if (H) __syncthreads();
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
-            if (i >= TR * per) break;
-            const float f = H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = v[n][e] * f;
-                const T h = (T)x;
-                hi[t * ldv + r + e] = h;
-                if constexpr (!F) lo[t * ldv + r + e] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
-            }
-        }
-    }
-    __syncthreads();
+    const T *lo = hi + TR * ldv;
     const int64_t at0 = (int64_t)lq * W;
     int64_t row[MT];
     float back[MT];                                                       // what undoes the row's range
@@ -368,13 +331,125 @@ __global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParam
             }
     };
     const bool aligned = p.yw && p.bw;
-    for (int g = (blockIdx.x * 4 + wave) * groups, end = g + groups; g < end;) {
+    for (int g = g0, end = g + groups; g < end;) {
         const int64_t n0 = (int64_t)g * GN;
         if (n0 >= N) return;
         if (aligned && g + 2 <= end && n0 + 2 * GN <= N) { go(n0, std::integral_constant<int, 2>(), std::true_type()); g += 2; }
         else if (aligned && n0 + GN <= N) { go(n0, std::integral_constant<int, 1>(), std::true_type()); ++g; }
         else { go(n0, std::integral_constant<int, 1>(), std::false_type()); ++g; }
     }
+}
+
+template <class E, int MT, bool GROUPED>
+__global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParams p, int groups) {
+    typedef typename E::T T; typedef typename E::V V;
+    constexpr int TR = MT * 16;
+    constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // v
+    __shared__ unsigned int high[TR];
+    __shared__ int rows[TR];
+    int adapter = -1;
+    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, adapter);
+    if (!count) return;
+    const int wave = threadIdx.x >> 6, R = (int)p.a.R, ldv = v_stride<E>(R);
+    const bool real = adapter < (int)p.a.n;
+    T *hi = reinterpret_cast<T *>(smem), *lo = hi + TR * ldv;
+    if (real) {
+        const int per = (ldv - E::W) / 4;                                   // pieces of 4 sums; a thread has up to 8 (64 rows of rank 128, 16 of rank 256)
+        float4_t v[8];
+        if (H && threadIdx.x < TR) high[threadIdx.x] = 0;
+        if (H) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
+            v[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            if (i < TR * per && t < count && r < p.rp) {
+                const float *at = p.v + (int64_t)rows[t] * p.rp + r;
+                const int64_t next = p.a.T * p.rp;
+                int s = 0;
+                for (; s + 4 <= p.splits; s += 4, at += 4 * next) {
+                    float4_t q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const float4_t *>(at + e * next);
+                    v[n] += (q[0] + q[1]) + (q[2] + q[3]);
+                }
+                for (; s < p.splits; ++s, at += next) v[n] += *reinterpret_cast<const float4_t *>(at);
+            }
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (r + e >= R) v[n][e] = 0.f;                            // (behind R there are repeats of the last row of A)
+                most = fmaxf(most, fabsf(v[n][e]));
+            }
+            if (H && i < TR * per) atomicMax(&high[t], __float_as_uint(most));
+        }
+        if (H) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int i = n * 256 + threadIdx.x, t = i / per, r = (i - t * per) * 4;
+            if (i >= TR * per) break;
+            const float f = H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = v[n][e] * f;
+                const T h = (T)x;
+                hi[t * ldv + r + e] = h;
+                if constexpr (!F) lo[t * ldv + r + e] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
+            }
+        }
+    }
+    __syncthreads();
+    up_columns<E, MT>(p, rows, count, adapter, hi, high, ldv, (blockIdx.x * 4 + wave) * groups, groups);
+}
+// Both in one launch, where few rows (tiles of 16) meet few ranks (R <= 16 RT): each workgroup forms v anew for its columns, 8 waves over K, and keeps it in LDS
+template <class E, int RT>
+__global__ __launch_bounds__(512) void lora_both_kernel(LoraParams p) {
+    typedef typename E::T T;
+    constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
+    constexpr int MOST = v_stride<E>(RT * 16);
+    __shared__ int rows[16];
+    __shared__ unsigned int high[16];
+    __shared__ __attribute__((aligned(16))) char smem[8 * image_bytes<1, RT>()];
+    __shared__ __attribute__((aligned(16))) T v[(F ? 1 : 2) * 16 * MOST];
+    int adapter = -1;
+    const int count = tile_of_small(p, blockIdx.y, rows, adapter);
+    if (!count) return;
+    const int tid = threadIdx.x, R = (int)p.a.R, ldv = v_stride<E>(R);
+    T *hi = v, *lo = v + 16 * ldv;
+    if (adapter < (int)p.a.n) {
+        for (int i = tid; i < (F ? 1 : 2) * 16 * ldv; i += 512) v[i] = (T)0.f;      // (what the last step of the product reads behind R)
+        if (tid < 16) high[tid] = 0;
+        down_sums<E, 1, RT, 8>(p, rows, count, adapter, 0, 0, smem);
+        const int t = tid & 15, r = (tid >> 6) * 16 + ((tid >> 4) & 3) * 4;
+        float4_t sum = {0.f, 0.f, 0.f, 0.f};
+        if (tid < RT * 64) {
+            const float4_t *part = reinterpret_cast<const float4_t *>(smem) + tid;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) sum += part[w * RT * 64];
+            sum *= p.a.scales ? p.a.scales[adapter] : 1.f;
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (r + e >= R || t >= count) sum[e] = 0.f;               // (behind them are repeats)
+                most = fmaxf(most, fabsf(sum[e]));
+            }
+            if (H) atomicMax(&high[t], __float_as_uint(most));
+        }
+        if (H) __syncthreads();
+        if (tid < RT * 64) {
+            const float f = H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (r + e >= R) break;
+                const float x = sum[e] * f;
+                const T h = (T)x;
+                hi[t * ldv + r + e] = h;
+                if constexpr (!F) lo[t * ldv + r + e] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
+            }
+        }
+    }
+    __syncthreads();
+    up_columns<E, 1>(p, rows, count, adapter, hi, high, ldv, blockIdx.x * 8 + (tid >> 6), 1);
 }
 
 static int lora_splits_most(int64_t T, int64_t K) {                       // (a wave has a strip of 64 at least)
@@ -398,8 +473,7 @@ static void lora_launch(const LoraParams &p, int64_t tiles, hipStream_t s) {
     const int64_t all = (p.a.N + GN - 1) / GN;                            // groups of columns: a wave takes 1 to 4, as long as there are workgroups for two rounds of the chip
     int groups = 4;
     while (groups > 1 && (all + 4 * groups - 1) / (4 * groups) * tiles < 512) groups /= 2;
-    const int ldv = (int)((p.a.R + E::KS - 1) / E::KS * E::KS + E::W);
-    lora_up_kernel<E, MT, GROUPED><<<dim3((unsigned)((all + 4 * groups - 1) / (4 * groups)), t), 256, (size_t)MT * 16 * ldv * 4, s>>>(p, groups);
+    lora_up_kernel<E, MT, GROUPED><<<dim3((unsigned)((all + 4 * groups - 1) / (4 * groups)), t), 256, (size_t)MT * 16 * v_stride<E>((int)p.a.R) * 4, s>>>(p, groups);
 }
 
 template <class E>
@@ -425,7 +499,21 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
         lora_group_kernel<<<dim3(1), dim3(1024), (size_t)(a.n + 1) * 4, s>>>(p, tr, order, td, nt);
         if (tr == 64) lora_launch<E, 4, true>(p, tiles, s);
         else lora_launch<E, 1, true>(p, tiles, s);
-    } else lora_launch<E, 1, false>(p, tiles, s);
+    } else {
+        constexpr int GN = E::W / 4 * 16;
+        const int64_t columns = (a.N + 8 * GN - 1) / (8 * GN);
+        // One launch, as long as what its workgroups read again from the L2 caches, and one workgroup's way along K, take less than a launch: x and A of a tile for every 8 GN columns up to 64 MB in
+        // all, rows of up to 8 KB.  32 rows of 32 adapters of rank 16, 1024 -> 2048: 9.0 -> 5.3 us; 64 x 4096 -> 4096, rank 32, 57 MB: 10.8 -> 10.6; 32 x 4096 -> 4096, 134 MB: 9.6 -> 11.2;
+        // float32, one row of 4096: 6.9 -> 8.2.  (Each workgroup reads x while others write y: they must not overlap.)
+        const char *x0 = (const char *)a.x, *y0 = (const char *)a.y;
+        const int64_t row = a.K * (int64_t)sizeof(typename E::T), size = sizeof(typename E::T);
+        const bool apart = x0 + ((a.T - 1) * a.ldx + a.K) * size <= y0 || y0 + ((a.T - 1) * a.ldy + a.N) * size <= x0;
+        if (apart && a.R <= 32 && row <= 8192 && columns * tiles * (16 + p.rp) * row <= 64ll << 20) {
+            p.splits = 1;
+            if (a.R <= 16) lora_both_kernel<E, 1><<<dim3((unsigned)columns, (unsigned)tiles), 512, 0, s>>>(p);
+            else lora_both_kernel<E, 2><<<dim3((unsigned)columns, (unsigned)tiles), 512, 0, s>>>(p);
+        } else lora_launch<E, 1, false>(p, tiles, s);
+    }
     NVR_KX_LAUNCHED("lora_add");
     return 0;
 }

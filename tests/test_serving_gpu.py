@@ -900,3 +900,26 @@ def test_sample_whole_rows_of_equal_logits(arena):
 def test_lora_of_many_rows(arena, T, K, N, R, n):
     """More rows than one pass of the grouping takes, in tiles of 64 rows and of 16."""
     lora_case(arena, "float16", T, K, N, R, n, np.random.default_rng(T + R).integers(-1, n, T))
+
+
+@pytest.mark.parametrize("dtype,T,K,N,R,n", [("float32", 5, 4096, 64, 16, 2), ("float32", 5, 2048, 64, 16, 2), ("bfloat16", 64, 4096, 4104, 32, 64), ("float16", 64, 4096, 4104, 17, 2), ("bfloat16", 64, 72, 8, 32, 64),
+                                             ("float16", 1, 4097, 31, 32, 1), ("float16", 1, 4096, 31, 32, 1)])
+def test_lora_one_launch_and_two(arena, dtype, T, K, N, R, n):
+    """Sizes on either side of what one launch takes."""
+    lora_case(arena, dtype, T, K, N, R, n, np.random.default_rng(T + K).integers(-1, n, T))
+
+
+def test_lora_into_its_own_input(arena):
+    """y may be x: all of x is read before any of y is written."""
+    typed("float32")
+    rng = np.random.default_rng(3)
+    T, K, R = 24, 1024, 8
+    x, base = rng.standard_normal((2, T, K)).astype(np.float32)
+    A, B = rng.standard_normal((1, R, K)).astype(np.float32) / 32, rng.standard_normal((1, K, R)).astype(np.float32)
+    y = arena.dev(x)
+    nvr.check(L.nvr_lora_add(y.ptr, K, arena.dev(A).ptr, arena.dev(B).ptr, None, arena.dev(np.zeros(T, np.int32)).ptr, 1, T, K, K, R, arena.dev(base).ptr, K, y.ptr, K,
+                             arena.space(L.nvr_lora_workspace_bytes(T, K, K, R)).ptr, None))
+    v = x.astype(np.float64) @ A[0].T.astype(np.float64)
+    want = base + v @ B[0].T.astype(np.float64)
+    # sums of K and R products in 32 bits
+    within(y.to_numpy((T, K), np.float32).astype(np.float64), want, F32 * ((K + R) * (np.abs(x) @ np.abs(A[0]).T) @ np.abs(B[0]).T + np.abs(want)) + 1e-30, "into x")
