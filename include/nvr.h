@@ -690,7 +690,8 @@ typedef struct nvr_rope_scaling {
 NVR_API int nvr_rope_frequencies(const nvr_rope_scaling *sc, int64_t rotary_dim, double *turns_dev, float *amplitude);
 /* Rotates the first rotary_dim columns of every head of q [T, H, D] and k [T, KVH, D] (rows ldq / ldk numbers apart): pairs are columns (j, j + rotary_dim / 2), or (2j, 2j + 1) with
  * interleaved != 0; the other columns pass through.  q_out / k_out may be q / k themselves (with the same stride).  With caches [num_slots, KVH, D], the k rows (k_out may then be null) and the v
- * rows [T, KVH, D] are also stored at slot_mapping (a slot outside 0 .. num_slots - 1: not stored; two rows of one slot: either).  Caches, v and slot_mapping may be null together. */
+ * rows [T, KVH, D] are also stored at slot_mapping (a slot outside 0 .. num_slots - 1: not stored; two rows of one slot: either).  Caches, v and slot_mapping may be null together.
+ * T up to 2^23. */
 NVR_API int nvr_rope_rotate_store_kv(const nvr_half *q, int64_t ldq, const nvr_half *k, int64_t ldk, const nvr_half *v, int64_t ldv, const int64_t *positions,
                                      const int32_t *slot_mapping, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t rotary_dim, int interleaved, const double *turns,
                                      float amplitude, nvr_half *q_out, int64_t ldqo, nvr_half *k_out, int64_t ldko, nvr_half *k_cache, nvr_half *v_cache, int64_t num_slots,
@@ -716,7 +717,7 @@ NVR_API int nvr_sample_uniform(const float *logits, int64_t ld, int64_t B, int64
 /* nvr_paged_attn_decode that also scores the keys: new_scores[key] = decay * scores[key] + the key's softmax weight, summed over the H / KVH query heads of its kv head, for the keys
  * j < scored_lens[b] of sequence b, and the weight alone for the others (scored_lens null: all but the newest key have a score).  Score pools are [num_blocks, KVH, block_size] f32, addressed by the block
  * table like the caches [num_blocks, block_size, KVH, D]; new_scores may be scores itself; entries of keys that no sequence of the batch has stay as they are.  Keys whose block is not in
- * 0 .. num_blocks - 1 are not there; contexts are cut at max_context_len and at max_blocks * block_size; a sequence without keys answers 0.  head_dim 64, 128 or 256, up to 16 query heads a kv head.
+ * 0 .. num_blocks - 1 are not there; contexts are cut at max_context_len and at max_blocks * block_size; a sequence without keys answers 0.  head_dim 64, 128 or 256, up to 16 query heads a kv head, contexts up to 2^23.
  * The block of a key is one sequence's alone (two sequences that share a block would both write its scores).  workspace: nvr_paged_attn_scored_workspace_bytes (of meta's max_context_len). */
 NVR_API size_t nvr_paged_attn_scored_workspace_bytes(int64_t B, int64_t H, int64_t KVH, int64_t D, int64_t max_context_len);
 NVR_API int nvr_paged_attn_decode_scored(const nvr_half *q, int64_t ldq, const nvr_half *k_cache, const nvr_half *v_cache, const nvr_attn_meta *meta, int64_t H, int64_t KVH,

@@ -44,6 +44,10 @@ def test_rope_refusals(change):
     refused("nvr_rope_rotate_store_kv", "NVR_ERR_INVALID_ARG", *{**ROPE, **change}.values())
 
 
+def test_rope_of_more_tokens_than_a_launch_holds():
+    refused("nvr_rope_rotate_store_kv", "NVR_ERR_UNSUPPORTED", *{**ROPE, "T": (1 << 23) + 1}.values())
+
+
 def test_rope_of_no_rows_is_nothing():
     assert nvr.lib().nvr_rope_rotate_store_kv(*{**ROPE, "T": 0}.values()) == 0
 
