@@ -11,6 +11,9 @@
 // t = 24 x / T in 64 bits, a token lies in the cell of the whole number next to t and adds exp((t - cell) / 24), 0.98 to 1.02, in steps of 2^-40 to it (a polynomial of degree 5, 1e-13 off); a cell
 // counts exp(cell / 24).
 // Tokens more than 42 T below the largest (e^-42 = 4e-19 of its weight) are left out.
+// Rows of 151936 logits (their read alone: 24 us for 256 of them, 4 for one), both launches: one row 15 us with top-k 20, 35 with 1000, 60 with top-p 0.95 that keeps some ten thousand tokens; 256 rows 45, 82
+// and 137 (77 + 60), 112 with settings mixed (54 + 58).  The first is bound by 64-bit arithmetic and, for top-p, by the LDS atomics on the bins (two copies of them where a chunk is large: 95 -> 77); the
+// second, a workgroup a row, by a chain of scans and LDS round trips, and by walks over a row where the lists end too early.
 // What a chunk cannot contribute is left out by one comparison a token: with top-k, whatever lies below the k-th of the chunk's maxima of 8 neighbours (there are k tokens above it), with min-p
 // alone, whatever lies below min_p of the chunk's maximum.
 #include <algorithm>
@@ -344,34 +347,43 @@ struct Row {
     template <class F>
     __device__ __forceinline__ void each_listed(int lo, int hi, F f) const {
         const int lane = threadIdx.x & 63;
-        for (int c0 = threadIdx.x >> 6; c0 < p.P; c0 += kPick / 16) {     // (the first tokens of 4 chunks together)
-            uint2 first[4];
-            int n[4];
+        for (int c0 = threadIdx.x >> 6; c0 < p.P; c0 += kPick / 16) {     // (64 tokens of 4 chunks together)
+            int n[4], most = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = c0 + e * (kPick / 64);
-                n[e] = c < p.P && sh.shift[c] <= hi ? sh.near[c] : 0;
-                if (lane < n[e]) first[e] = p.near[((int64_t)row * p.P + c) * kNear + lane];
+                n[e] = c < p.P && sh.shift[c] <= hi ? same((int)sh.near[c]) : 0;
+                most = max(most, n[e]);
             }
+            for (int i = lane; i - lane < most; i += 64) {
+                uint2 q[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                for (int i = lane; i < n[e]; i += 64) {
-                    const uint2 k = i == lane ? first[e] : p.near[((int64_t)row * p.P + c0 + e * (kPick / 64)) * kNear + i];
+                for (int e = 0; e < 4; ++e) if (i < n[e]) q[e] = p.near[((int64_t)row * p.P + c0 + e * (kPick / 64)) * kNear + i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i >= n[e]) continue;
+                    const uint2 k = q[e];
                     const float v = of_key(k.x);
                     const int b = bin_of(v, m, ask.inv);
                     if (b >= lo && b <= hi) f(k.x, k.y, v, b);
                 }
+            }
         }
+    }
+    // logits of bins lo .. hi are not below `least` nor above `most`
+    __device__ __forceinline__ void ends_of(int lo, int hi, float &least, float &most) const {
+        const double top = ((double)m * ask.inv + kWhole) - kWhole;       // (the cells' ends are halves)
+        const float a = (float)((top - hi - 0.5) / ask.inv), z = (float)((top - lo + 0.5) / ask.inv);
+        const bool lone = lonely(m, ask.inv);
+        least = fminf(lone ? m : a - fabsf(a) * 1e-6f, FLT_MAX); most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
+        if (!(least == least && most == most)) { least = -INFINITY; most = INFINITY; }      // (1 / inv beyond float)
     }
     // ... in the row itself.  Most tokens are outside: the signs of x less the bins' lower end and the upper end less x (a little beyond, for their roundings) tell, four instructions a token.
     // Numbers that are none may pass here
     template <class F>
     __device__ __forceinline__ void each_of_row(int lo, int hi, F f) const {
-        const double top = ((double)m * ask.inv + kWhole) - kWhole;       // (the cells' ends are halves)
-        const float a = (float)((top - hi - 0.5) / ask.inv), z = (float)((top - lo + 0.5) / ask.inv);
-        const bool lone = lonely(m, ask.inv);
-        float least = fminf(lone ? m : a - fabsf(a) * 1e-6f, FLT_MAX), most = lone || lo == 0 ? INFINITY : z + fabsf(z) * 1e-6f;
-        if (!(least == least && most == most)) { least = -INFINITY; most = INFINITY; }      // (1 / inv beyond float)
+        float least, most;
+        ends_of(lo, hi, least, most);
         for (int i0 = threadIdx.x * 4; i0 < p.V; i0 += kPick * 16) {
             float v[16];
 #pragma unroll
@@ -427,8 +439,9 @@ struct Row {
     // Among the tokens of bin b in descending order (ties: ascending index): the last one that is kept, when `need` of them are (need > 0) or as many as it takes until `before` plus their weights
     // reaches `goal`.  part: the weight of the kept ones.  Of few tokens, a thread a token, each counts those in front of it; else a radix select over 11 bits of the logit at a time, then over 11
     // and 11 of the index
-    __device__ __forceinline__ void settle(int b, unsigned int need, double before, double goal, unsigned int &key, unsigned int &index, double &part) {
-        const bool here = gather(b, b);
+    // mass: the bin's.  Its tokens weigh 0.98 to 1.02 units each, so it tells whether LDS can have them, and a walk over the row for nothing is spared
+    __device__ __forceinline__ void settle(int b, double mass, unsigned int need, double before, double goal, unsigned int &key, unsigned int &index, double &part) {
+        const bool here = (b <= listed || mass <= cell(b) * (1.05 * kList * 0x1p40)) && gather(b, b);
         const int tid = threadIdx.x;
         const double unit = cell(b);
         if (here) {
@@ -462,18 +475,11 @@ struct Row {
         unsigned int left = need, equal = 0;
         unsigned long long done = 0;                                      // weight above the prefix
         // the tokens of a bin are alike in their upper bits: those are the first prefix
-        if (tid == 0) { sh.low = 0xffffffffu; sh.high = 0; }
-        __syncthreads();
-        {
-            unsigned int low = 0xffffffffu, high = 0;
-            each_gathered(here, b, b, [&](unsigned int k, unsigned int, float, int) { low = min(low, k); high = max(high, k); });
-            low = ~wave_largest(~low); high = wave_largest(high);
-            if ((tid & 63) == 0) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
-        }
-        __syncthreads();
-        if (same(sh.low) > same(sh.high)) { key = 0; index = 0xffffffffu; part = 0.; __syncthreads(); return; }      // (no token: everything is kept)
-        const int bits = same(sh.low == sh.high ? 0 : 32 - __clz((int)(sh.low ^ sh.high)));      // that differ
-        unsigned int mask = bits >= 32 ? 0 : 0xffffffffu << bits, prefix = same(sh.high) & mask;
+        float least, most;
+        ends_of(b, b, least, most);
+        const unsigned int low = key_of(least), high = key_of(fminf(most, m));
+        const int bits = low == high ? 0 : 32 - __clz((int)(low ^ high)); // that differ
+        unsigned int mask = bits >= 32 ? 0 : 0xffffffffu << bits, prefix = high & mask;
         for (int at = bits;;) {
             const int wide = 1 << min(at, 11);
             at = max(at - 11, 0);
@@ -744,7 +750,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             if (!filter && same(sh.cum_n[bin]) == k) { stop = bin + 1; total = same(sh.cum[bin]); continue; }
             unsigned int k2, i2;
             double part;
-            r.settle(bin, filter ? 0 : k - (bin ? same(sh.cum_n[bin - 1]) : 0), before, goal, k2, i2, part);
+            r.settle(bin, same(sh.cum[bin]) - before, filter ? 0 : k - (bin ? same(sh.cum_n[bin - 1]) : 0), before, goal, k2, i2, part);
             if (bin < stop || k2 > key || (k2 == key && i2 < index)) { key = k2; index = i2; }      // (in the bin where top-k ended, its own end may come first)
             stop = bin;
             if (!filter) total = before + part;
@@ -919,7 +925,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
 }
 
-static int sample_chunk(int64_t B, int64_t V) { return B * ((V + 16383) / 16384) >= 256 ? 16384 : 4096; }   // tokens of a chunk (12 KB of bins each, so larger ones once they fill the chip)
+// Tokens of a chunk.  Each has its bins and lists, which the second launch reads: large ones once they fill the chip or there would be many.  us with 4096 and 16384: 256 rows of 151936 137 114; one row of
+// 151936 with top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 22 (the walk over the drawn chunk); one of 10^6: 28 19, 64 58, 52 54, 26 25; one of 32000: 14 15, 36 42, 15 20, 14 21
+static int sample_chunk(int64_t B, int64_t V) { return V > 131072 || B * ((V + 16383) / 16384) >= 256 ? 16384 : 4096; }
 size_t sample_uniform_workspace_bytes(int64_t B, int64_t V) {
     if (B <= 0 || V <= 0) return 0;
     const int64_t P = (V + sample_chunk(B, V) - 1) / sample_chunk(B, V);
