@@ -15,11 +15,12 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kPick = 1024, kHeld = 9216, kRadix = 2048, kTable = 512;
+constexpr int kPick = 1024, kHeld = 32768, kRadix = 2048, kTable = 512;      // kHeld: scores in LDS, at most (128 of 160 KB)
 struct EvictParams {
     EvictArgs a;
     int32_t *kept;                                                        // [B][KVH][budget]
     int32_t row_bytes, strip;                                             // of a key's row of a head; bytes of it that a workgroup moves
+    int32_t held;                                                         // scores that LDS has room for
     uint32_t per_block;                                                   // 2^32 / block_size, rounded down
 };
 // j / block_size and what is left, without a division: the product's upper half is at most one short
@@ -47,7 +48,7 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 }  // namespace
 
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
-    __shared__ __attribute__((aligned(16))) float held[kHeld];            // scores of keys 0 .. kHeld - 1
+    extern __shared__ __attribute__((aligned(16))) float held[];          // scores of keys 0 .. p.held - 1
     __shared__ unsigned int hist[2 * kRadix + kRadix / 2];                // 11, 11 and 10 bits
     __shared__ int32_t from_table[kTable], to_table[kTable];              // (the first kTable blocks of each)
     __shared__ unsigned int waves[16], above[3];
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     auto from_at = [&](int j) { return place(table, from_table, j); };
     auto to_at = [&](int j) { return place(to, to_table, j); };
     // ---- the scores into LDS, 4 neighbours a thread where blocks are multiples of 4
-    const int here = min(len, kHeld);
+    const int here = min(len, p.held);
     if (a.block_size % 4 == 0 && ((uintptr_t)a.scores & 15) == 0) {
         for (int i0 = tid * 4; i0 < here; i0 += kPick * 8) {
             float4_t v[2];
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     } else
         for (int i = tid; i < here; i += kPick) held[i] = a.scores[from_at(i)];
     __syncthreads();
-    auto score = [&](int i) { return i < kHeld ? held[i] : a.scores[from_at(i)]; };
+    auto score = [&](int i) { return i < p.held ? held[i] : a.scores[from_at(i)]; };
     // ---- the rank of the last of the best: the `need` best of keys first .. end - 1, of equal ones the earliest `want`
     const int first = a.first, end = len - a.last;
     const unsigned int need = all ? 0 : a.budget - a.first - a.last;      // (fewer than compete)
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     }
     const unsigned long long own = ((unsigned long long)more << 32) | same, v = scan<unsigned long long>(own, waves2) - own;
     // the scores at their new places: at once where LDS has them all
-    const bool together = len <= kHeld;
+    const bool together = len <= p.held;
     unsigned int seen = (unsigned int)v, at = (unsigned int)(v >> 32) + min(seen, want);
     for (int i = i0; i < i1; ++i) {
         const bool always = all || i < first || i >= end;
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
 }
 
 // 16 bytes a lane, `strip` bytes of a row; the step in front of the next one's writes is on its way
-constexpr int kMoves = 4;
+constexpr int kMoves = 4;                                                 // requests on their way (32 x 8000 keys of 8 heads of 128 to 2048, float16: 2 109 us, 4 106, 8 129)
 __global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
     const EvictArgs &a = p.a;
     const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -196,31 +197,19 @@ __global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
     }
 }
 
-// Into other blocks: a lane 16 bytes of K and of V, kMoves rows on their way
+// Into other blocks: a lane 16 bytes of K and of V (of two rows 124 us where this takes 123, of four 126, of eight 131)
 __global__ __launch_bounds__(256) void kv_evict_copy_kernel(EvictParams p) {
     const EvictArgs &a = p.a;
     const int g = blockIdx.y, b = blockIdx.z;
     const int n = a.new_lens[b];
-    const int lanes = p.row_bytes / 16, rows = 256 / lanes, i0 = blockIdx.x * rows * kMoves, lead = threadIdx.x / lanes, piece = threadIdx.x % lanes;
-    if (i0 >= n || lead >= rows) return;
+    const int lanes = p.row_bytes / 16, rows = 256 / lanes, lead = threadIdx.x / lanes, piece = threadIdx.x % lanes, i = blockIdx.x * rows + lead;
+    if (i >= n || lead >= rows) return;
     const int32_t *table = a.block_tables + (int64_t)b * a.max_blocks, *to = a.to_tables + (int64_t)b * a.to_max_blocks, *kept = p.kept + ((int64_t)b * a.KVH + g) * a.budget;
     const int64_t row = (int64_t)a.KVH * p.row_bytes, off = (int64_t)g * p.row_bytes + piece * 16;
-    float4_t k[kMoves], v[kMoves];
-#pragma unroll
-    for (int u = 0; u < kMoves; ++u) {
-        const int i = min(i0 + u * rows + lead, n - 1);
-        const int64_t at = row_in(p, table, kept[i]) * row + off;
-        k[u] = *reinterpret_cast<const float4_t *>((const char *)a.k + at);
-        v[u] = *reinterpret_cast<const float4_t *>((const char *)a.v + at);
-    }
-#pragma unroll
-    for (int u = 0; u < kMoves; ++u) {
-        const int i = i0 + u * rows + lead;
-        if (i >= n) break;
-        const int64_t at = row_in(p, to, i) * row + off;
-        *reinterpret_cast<float4_t *>((char *)a.k + at) = k[u];
-        *reinterpret_cast<float4_t *>((char *)a.v + at) = v[u];
-    }
+    const int64_t from = row_in(p, table, kept[i]) * row + off, at = row_in(p, to, i) * row + off;
+    const float4_t k = *reinterpret_cast<const float4_t *>((const char *)a.k + from), v = *reinterpret_cast<const float4_t *>((const char *)a.v + from);
+    *reinterpret_cast<float4_t *>((char *)a.k + at) = k;
+    *reinterpret_cast<float4_t *>((char *)a.v + at) = v;
 }
 
 size_t kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_ctx) {
@@ -248,9 +237,12 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     p.per_block = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / (uint64_t)a.block_size);
     p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
     const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
-    kv_evict_select_kernel<<<dim3(G, B), kPick, 0, s>>>(p);
+    p.held = std::min((a.max_ctx + 3) / 4 * 4, kHeld);
+    static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv_evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
+    if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "%s: LDS of %d bytes: %s", me, kHeld * 4, hipGetErrorString(opted));
+    kv_evict_select_kernel<<<dim3(G, B), kPick, (size_t)p.held * 4, s>>>(p);
     if (a.to_tables) {
-        const int rows = 256 / (p.row_bytes / 16) * kMoves, most = std::min(a.budget, a.max_ctx);
+        const int rows = 256 / (p.row_bytes / 16), most = std::min(a.budget, a.max_ctx);
         if (most > 0) kv_evict_copy_kernel<<<dim3((unsigned)((most + rows - 1) / rows), G, B), 256, 0, s>>>(p);
     } else if (a.max_ctx > a.budget) kv_evict_close_kernel<<<dim3((unsigned)(2 * (p.row_bytes / p.strip)), G, B), kPick, 0, s>>>(p);
     NVR_KX_LAUNCHED("kv_evict");

@@ -923,3 +923,8 @@ def test_lora_into_its_own_input(arena):
     want = base + v @ B[0].T.astype(np.float64)
     # sums of K and R products in 32 bits
     within(y.to_numpy((T, K), np.float32).astype(np.float64), want, F32 * ((K + R) * (np.abs(x) @ np.abs(A[0]).T) @ np.abs(B[0]).T + np.abs(want)) + 1e-30, "into x")
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_of_more_keys_than_lds_holds(arena, out_of_place):
+    evict_case(arena, "bfloat16", [40000, 32769, 32768, 100], 1, 64, 256, 20000, 4, 700, out_of_place)
