@@ -1,22 +1,24 @@
 // lora.hip — low-rank adapters of many requests beside a shared projection: y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T, a = the adapter of row t's request.
 //
 // Two products of inner sizes K and R, on the matrix cores, over TILES: up to 16 or 64 rows that share an adapter, wherever they stand in the step (up to 64 rows every wave finds its tile
-// itself; more are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
+// itself; many are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
 //   down: v = scale x A^T, the waves of a workgroup (and `splits` workgroups of few rows) share K; partial sums stay in 32 bits in the workspace, [split][row][rank]
 //   up:   y = base + v B^T; v in two 16-bit numbers (its rounding and the rounded rest), so that the product sees it in 16 (bfloat16) or 22 bits; the sum with base is rounded once
-// Few rows of few ranks take one launch, in which every workgroup forms v anew for its columns.
+// Few rows of few ranks take one launch, in which every workgroup finds its tile and forms v anew for its columns.
 // Bound by memory for prompts (x, base and y once; 2 R flops a byte), by launches and a chain of round trips for decode steps.  bfloat16, 8192 rows 4096 -> 12288 of rank 32: 122 us (grouping 8, down
 // 24, up 91: 402 MB of base and y at 4.4 TB/s); float16, 251 rows 4096 -> 4096 of rank 64 over 7 adapters: 16 us (4, 6, 6); 32 rows 1024 -> 2048 of rank 16 over 32: 5.3 us in one launch.
 #include <algorithm>
 #include <type_traits>
 #include "serving.h"
 #include "elem.h"
+#include "scan.h"
 #include "../common.h"
 
 namespace nvr { namespace kx {
 
 namespace {
 constexpr int kSmall = 64;                                                // rows up to which a workgroup finds its tile itself (64 x 1024 -> 2048 of rank 64: 11.1 us, grouped by a launch 12.9)
+constexpr int kMany = 1024;                                               // rows up to which one launch may do
 constexpr int kMaxAdapters = 8192;                                        // counters of the grouping launch (LDS)
 
 struct LoraTile { int32_t start, count, adapter; };                       // rows order[start ..) of one adapter; adapter n: rows without one
@@ -402,51 +404,92 @@ __global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParam
     __syncthreads();
     up_columns<E, MT>(p, rows, count, adapter, hi, high, ldv, (blockIdx.x * 4 + wave) * groups, groups);
 }
-// Both in one launch, where few rows (tiles of 16) meet few ranks (R <= 16 RT): each workgroup forms v anew for its columns, 8 waves over K, and keeps it in LDS
-template <class E, int RT>
+// rows of tile `tile` (16 rows), as tile_of_small, of up to kMany rows and fewer than 1024 adapters: a workgroup of 512 counts each adapter's rows, and the rows of the tile's adapter in their order
+__device__ __forceinline__ int tile_of_many(const LoraParams &p, int tile, int *rows, int &adapter) {
+    constexpr int PER = kMany / 512;
+    __shared__ int cnt[1024], waves[8 * PER], chosen[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = (int)p.a.T;
+    int id[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) id[e] = e * 512 + tid < T ? adapter_of(p, e * 512 + tid) : -1;
+    cnt[2 * tid] = cnt[2 * tid + 1] = 0;
+    if (tid == 0) chosen[0] = -1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) if (id[e] >= 0) atomicAdd(&cnt[id[e]], 1);
+    __syncthreads();
+    const int t0 = (cnt[2 * tid] + 15) / 16, t1 = (cnt[2 * tid + 1] + 15) / 16, upto = scan<int>(t0 + t1, waves), from = upto - t0 - t1;
+    if (from <= tile && tile < upto) {                                    // (one thread)
+        const bool second = tile >= from + t0;
+        chosen[0] = 2 * tid + second; chosen[1] = (tile - from - (second ? t0 : 0)) * 16;
+    }
+    __syncthreads();
+    if (chosen[0] < 0) return 0;
+    adapter = same(chosen[0]);
+    const int first = same(chosen[1]), count = same(min(16, cnt[adapter] - first));
+    unsigned long long mine[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        mine[e] = __ballot(id[e] == adapter);
+        if (lane == 0) waves[e * 8 + wave] = __popcll(mine[e]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        int rank = __popcll(mine[e] & ((1ull << lane) - 1)) - first;
+        for (int w = 0; w < e * 8 + wave; ++w) rank += waves[w];
+        if (id[e] == adapter && rank >= 0 && rank < 16) rows[rank] = e * 512 + tid;
+    }
+    __syncthreads();
+    return count;
+}
+
+// Both in one launch, where few rows (tiles of 16) meet few ranks (up to kRanks, 16 RT at a time): each workgroup forms v anew for its columns, 8 waves over K, and keeps it in LDS
+constexpr int kRanks = 96;
+template <class E, int RT, bool MANY>
 __global__ __launch_bounds__(512) void lora_both_kernel(LoraParams p) {
     typedef typename E::T T;
     constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
-    constexpr int MOST = v_stride<E>(RT * 16);
+    constexpr int MOST = v_stride<E>(RT == 1 ? 16 : kRanks);
     __shared__ int rows[16];
     __shared__ unsigned int high[16];
     __shared__ __attribute__((aligned(16))) char smem[8 * image_bytes<1, RT>()];
     __shared__ __attribute__((aligned(16))) T v[(F ? 1 : 2) * 16 * MOST];
+    __shared__ float sums[RT == 1 ? 16 : kRanks][17];                     // [rank][row]
     int adapter = -1;
-    const int count = tile_of_small(p, blockIdx.y, rows, adapter);
+    const int count = MANY ? tile_of_many(p, blockIdx.y, rows, adapter) : tile_of_small(p, blockIdx.y, rows, adapter);
     if (!count) return;
     const int tid = threadIdx.x, R = (int)p.a.R, ldv = v_stride<E>(R);
     T *hi = v, *lo = v + 16 * ldv;
     if (adapter < (int)p.a.n) {
         for (int i = tid; i < (F ? 1 : 2) * 16 * ldv; i += 512) v[i] = (T)0.f;      // (what the last step of the product reads behind R)
         if (tid < 16) high[tid] = 0;
-        down_sums<E, 1, RT, 8>(p, rows, count, adapter, 0, 0, smem);
-        const int t = tid & 15, r = (tid >> 6) * 16 + ((tid >> 4) & 3) * 4;
-        float4_t sum = {0.f, 0.f, 0.f, 0.f};
-        if (tid < RT * 64) {
-            const float4_t *part = reinterpret_cast<const float4_t *>(smem) + tid;
+        const float scale = p.a.scales ? p.a.scales[adapter] : 1.f;
+        for (int r0 = 0; r0 < R; r0 += RT * 16) {
+            if (r0) __syncthreads();
+            down_sums<E, 1, RT, 8>(p, rows, count, adapter, r0, 0, smem);
+            if (tid < RT * 64) {
+                const int t = tid & 15, r = r0 + (tid >> 6) * 16 + ((tid >> 4) & 3) * 4;
+                const float4_t *part = reinterpret_cast<const float4_t *>(smem) + tid;
+                float4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 8; ++w) sum += part[w * RT * 64];
-            sum *= p.a.scales ? p.a.scales[adapter] : 1.f;
-            float most = 0.f;
+                for (int w = 0; w < 8; ++w) sum += part[w * RT * 64];
+                sum *= scale;
+                float most = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (r + e >= R || t >= count) sum[e] = 0.f;               // (behind them are repeats)
-                most = fmaxf(most, fabsf(sum[e]));
+                for (int e = 0; e < 4; ++e)
+                    if (r + e < R && t < count) { sums[r + e][t] = sum[e]; most = fmaxf(most, fabsf(sum[e])); }      // (behind them are repeats)
+                if (H) atomicMax(&high[t], __float_as_uint(most));
             }
-            if (H) atomicMax(&high[t], __float_as_uint(most));
         }
-        if (H) __syncthreads();
-        if (tid < RT * 64) {
-            const float f = H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (r + e >= R) break;
-                const float x = sum[e] * f;
-                const T h = (T)x;
-                hi[t * ldv + r + e] = h;
-                if constexpr (!F) lo[t * ldv + r + e] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
-            }
+        __syncthreads();
+        for (int i = tid; i < 16 * R; i += 512) {
+            const int t = i & 15, r = i >> 4;
+            if (t >= count) continue;
+            const float x = sums[r][t] * (H ? __uint_as_float((unsigned)(127 + range_of(high[t])) << 23) : 1.f);
+            const T h = (T)x;
+            hi[t * ldv + r] = h;
+            if constexpr (!F) lo[t * ldv + r] = (T)(fabsf((float)h) < INFINITY ? x - (float)h : 0.f);
         }
     }
     __syncthreads();
@@ -494,7 +537,29 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
     const int64_t zs = (p.rp / 16 + 1) / 2;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(lora_splits_most(a.T, a.K), ((tr == 64 ? 512 : 256) + tiles * zs - 1) / (tiles * zs)));
     p.v = (float *)a.workspace;
-    if (a.T > kSmall) {
+    constexpr int GN = E::W / 4 * 16;
+    const int64_t columns = (a.N + 8 * GN - 1) / (8 * GN), row = a.K * (int64_t)sizeof(typename E::T), size = sizeof(typename E::T);
+    const char *x0 = (const char *)a.x, *y0 = (const char *)a.y;
+    const bool apart = x0 + ((a.T - 1) * a.ldx + a.K) * size <= y0 || y0 + ((a.T - 1) * a.ldy + a.N) * size <= x0;
+    const int64_t tiles16 = std::min<int64_t>(a.T, a.T / 16 + kinds);
+    // One launch, as long as what its workgroups read again from the L2 caches (x and A of a tile for every 8 GN columns), and the way of one of them along K (for every 32 ranks), take less than the
+    // launches spared, one up to kSmall rows, two beyond.  us in one launch and in two or three, 16-bit types: 32 rows of 32 adapters of rank 16, 1024 -> 2048 (17 MB again) 5.3 9.0; 64 x 4096 -> 4096,
+    // rank 32 (57 MB) 10.6 10.8; 32 x 4096 -> 4096, rank 16 (134 MB) 11.2 9.6; 32 x 2048 -> 2048, rank 96 (3 x 4 KB along K) 14.2 9.6; 251 x 1024 -> 2048, rank 16 (12 MB) 6.2 13.2;
+    // 1000 x 1024 -> 4096, rank 16 (70 MB) 16.8 18.2; 512 x 1024 -> 12288, rank 16 (116 MB) 18.6 18.4; 251 x 4096 -> 4096, rank 32 (145 MB) 16.4 15.3; 200 x 4096 -> 1024, rank 96 (3 x 8 KB) 22.3 15.6.
+    // (Each workgroup reads x while others write y: they must not overlap.)
+    const int64_t rounds = a.R <= 16 ? 1 : (a.R + 31) / 32, again = rounds * columns * tiles16 * (16 + p.rp) * row;
+    const bool little = a.T <= kSmall ? rounds * row <= 8192 && again <= 64ll << 20 : a.T <= kMany && a.n < 1023 && rounds * row <= 12288 && again <= 128ll << 20;
+    if (apart && a.R <= kRanks && little) {
+        p.splits = 1;
+        const dim3 grid((unsigned)columns, (unsigned)tiles16);
+        if (a.T <= kSmall) {
+            if (a.R <= 16) lora_both_kernel<E, 1, false><<<grid, 512, 0, s>>>(p);
+            else lora_both_kernel<E, 2, false><<<grid, 512, 0, s>>>(p);
+        } else {
+            if (a.R <= 16) lora_both_kernel<E, 1, true><<<grid, 512, 0, s>>>(p);
+            else lora_both_kernel<E, 2, true><<<grid, 512, 0, s>>>(p);
+        }
+    } else if (a.T > kSmall) {
         char *at = (char *)a.workspace + (size_t)a.T * lora_splits_most(a.T, a.K) * p.rp * 4;
         LoraTile *td = (LoraTile *)at;
         int32_t *order = (int32_t *)(at + (size_t)a.T * sizeof(LoraTile)), *nt = order + a.T;
@@ -502,21 +567,7 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
         lora_group_kernel<<<dim3(1), dim3(1024), (size_t)(a.n + 1) * 4, s>>>(p, tr, order, td, nt);
         if (tr == 64) lora_launch<E, 4, true>(p, tiles, s);
         else lora_launch<E, 1, true>(p, tiles, s);
-    } else {
-        constexpr int GN = E::W / 4 * 16;
-        const int64_t columns = (a.N + 8 * GN - 1) / (8 * GN);
-        // One launch, as long as what its workgroups read again from the L2 caches, and one workgroup's way along K, take less than a launch: x and A of a tile for every 8 GN columns up to 64 MB in
-        // all, rows of up to 8 KB.  32 rows of 32 adapters of rank 16, 1024 -> 2048: 9.0 -> 5.3 us; 64 x 4096 -> 4096, rank 32, 57 MB: 10.8 -> 10.6; 32 x 4096 -> 4096, 134 MB: 9.6 -> 11.2;
-        // float32, one row of 4096: 6.9 -> 8.2.  (Each workgroup reads x while others write y: they must not overlap.)
-        const char *x0 = (const char *)a.x, *y0 = (const char *)a.y;
-        const int64_t row = a.K * (int64_t)sizeof(typename E::T), size = sizeof(typename E::T);
-        const bool apart = x0 + ((a.T - 1) * a.ldx + a.K) * size <= y0 || y0 + ((a.T - 1) * a.ldy + a.N) * size <= x0;
-        if (apart && a.R <= 32 && row <= 8192 && columns * tiles * (16 + p.rp) * row <= 64ll << 20) {
-            p.splits = 1;
-            if (a.R <= 16) lora_both_kernel<E, 1><<<dim3((unsigned)columns, (unsigned)tiles), 512, 0, s>>>(p);
-            else lora_both_kernel<E, 2><<<dim3((unsigned)columns, (unsigned)tiles), 512, 0, s>>>(p);
-        } else lora_launch<E, 1, false>(p, tiles, s);
-    }
+    } else lora_launch<E, 1, false>(p, tiles, s);
     NVR_KX_LAUNCHED("lora_add");
     return 0;
 }

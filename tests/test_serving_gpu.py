@@ -928,3 +928,14 @@ def test_lora_into_its_own_input(arena):
 @pytest.mark.parametrize("out_of_place", [False, True])
 def test_evict_of_more_keys_than_lds_holds(arena, out_of_place):
     evict_case(arena, "bfloat16", [40000, 32769, 32768, 100], 1, 64, 256, 20000, 4, 700, out_of_place)
+
+
+@pytest.mark.parametrize("dtype,T,K,N,R,n", [("float16", 65, 64, 40, 16, 1), ("bfloat16", 512, 1024, 264, 32, 7), ("float16", 513, 72, 33, 20, 1022), ("float16", 513, 72, 33, 20, 1023), ("float32", 1024, 64, 128, 8, 3),
+                                             ("bfloat16", 1024, 64, 128, 96, 40), ("bfloat16", 1025, 64, 128, 8, 3), ("float32", 1000, 16, 16, 90, 1000), ("bfloat16", 40, 1024, 72, 96, 3), ("float16", 64, 200, 1000, 49, 64)])
+def test_lora_rows_found_by_each_workgroup(arena, dtype, T, K, N, R, n):
+    rng = np.random.default_rng(T + n)
+    a = lora_case(arena, dtype, T, K, N, R, n, rng.integers(-1, n, T), seed=1)
+    rng = np.random.default_rng(T + n)
+    assert np.array_equal(a, lora_case(arena, dtype, T, K, N, R, n, rng.integers(-1, n, T), seed=1))
+    lora_case(arena, dtype, T, K, N, R, n, np.full(T, n - 1))
+    lora_case(arena, dtype, T, K, N, R, n, np.full(T, -1))
