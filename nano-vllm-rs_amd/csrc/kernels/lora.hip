@@ -1,12 +1,12 @@
 // lora.hip — low-rank adapters of many requests beside a shared projection: y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T, a = the adapter of row t's request.
 //
 // Two products of inner sizes K and R, on the matrix cores, over TILES: up to 16 or 64 rows that share an adapter, wherever they stand in the step (up to 64 rows every wave finds its tile
-// itself; many are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
+// itself, up to 1024 every workgroup; more are grouped by a launch of their own).  An adapter is so read once per tile and its rows cost no more than they are.
 //   down: v = scale x A^T, the waves of a workgroup (and `splits` workgroups of few rows) share K; partial sums stay in 32 bits in the workspace, [split][row][rank]
 //   up:   y = base + v B^T; v in two 16-bit numbers (its rounding and the rounded rest), so that the product sees it in 16 (bfloat16) or 22 bits; the sum with base is rounded once
 // Few rows of few ranks take one launch, in which every workgroup finds its tile and forms v anew for its columns.
 // Bound by memory for prompts (x, base and y once; 2 R flops a byte), by launches and a chain of round trips for decode steps.  bfloat16, 8192 rows 4096 -> 12288 of rank 32: 122 us (grouping 8, down
-// 24, up 91: 402 MB of base and y at 4.4 TB/s); float16, 251 rows 4096 -> 4096 of rank 64 over 7 adapters: 16 us (4, 6, 6); 32 rows 1024 -> 2048 of rank 16 over 32: 5.3 us in one launch.
+// 24, up 91: 402 MB of base and y at 4.4 TB/s); float16, 251 rows 4096 -> 4096 of rank 64 over 7 adapters: 15 us; 32 rows 1024 -> 2048 of rank 16 over 32: 5.3 us in one launch.
 #include <algorithm>
 #include <type_traits>
 #include "serving.h"
@@ -18,7 +18,7 @@ namespace nvr { namespace kx {
 
 namespace {
 constexpr int kSmall = 64;                                                // rows up to which a workgroup finds its tile itself (64 x 1024 -> 2048 of rank 64: 11.1 us, grouped by a launch 12.9)
-constexpr int kMany = 1024;                                               // rows up to which one launch may do
+constexpr int kMany = 1024;                                               // rows up to which it counts them
 constexpr int kMaxAdapters = 8192;                                        // counters of the grouping launch (LDS)
 
 struct LoraTile { int32_t start, count, adapter; };                       // rows order[start ..) of one adapter; adapter n: rows without one
@@ -58,9 +58,59 @@ __device__ __forceinline__ int tile_of_small(const LoraParams &p, int tile, int 
     if (in) rows[rank - first] = lane;
     return __popcll(__ballot(in));
 }
-template <int TR, bool GROUPED>
+// how a workgroup learns of its tile
+enum Find { SMALL, MANY, GROUPED };
+// rows of tile `tile` (16 rows), as tile_of_small, of up to kMany rows and fewer than 1024 adapters: a workgroup counts each adapter's rows, and the rows of the tile's adapter in their order
+template <int THREADS>
+__device__ __forceinline__ int tile_of_many(const LoraParams &p, int tile, int *rows, int &adapter) {
+    constexpr int PER = kMany / THREADS, OWN = 1024 / THREADS;            // rows and adapters of a thread
+    __shared__ int cnt[1024], waves[16], chosen[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = (int)p.a.T;
+    int id[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) id[e] = e * THREADS + tid < T ? adapter_of(p, e * THREADS + tid) : -1;
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) cnt[OWN * tid + e] = 0;
+    if (tid == 0) chosen[0] = -1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) if (id[e] >= 0) atomicAdd(&cnt[id[e]], 1);
+    __syncthreads();
+    int own = 0;
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) own += (cnt[OWN * tid + e] + 15) / 16;
+    const int upto = scan<int>(own, waves);
+    int from = upto - own;
+    if (from <= tile && tile < upto) {                                    // (one thread)
+        int i = OWN * tid;
+        for (int t; from + (t = (cnt[i] + 15) / 16) <= tile; ++i) from += t;
+        chosen[0] = i; chosen[1] = (tile - from) * 16;
+    }
+    __syncthreads();
+    if (chosen[0] < 0) return 0;
+    adapter = same(chosen[0]);
+    const int first = same(chosen[1]), count = same(min(16, cnt[adapter] - first));
+    unsigned long long mine[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        mine[e] = __ballot(id[e] == adapter);
+        if (lane == 0) waves[e * (THREADS / 64) + wave] = __popcll(mine[e]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        int rank = __popcll(mine[e] & ((1ull << lane) - 1)) - first;
+        for (int w = 0; w < e * (THREADS / 64) + wave; ++w) rank += waves[w];
+        if (id[e] == adapter && rank >= 0 && rank < 16) rows[rank] = e * THREADS + tid;
+    }
+    __syncthreads();
+    return count;
+}
+
+template <int TR, Find FIND, int THREADS>
 __device__ __forceinline__ int tile_rows(const LoraParams &p, int tile, int *rows, int &adapter) {
-    if constexpr (!GROUPED) return tile_of_small(p, tile, rows, adapter);
+    if constexpr (FIND == SMALL) return tile_of_small(p, tile, rows, adapter);
+    if constexpr (FIND == MANY) return tile_of_many<THREADS>(p, tile, rows, adapter);
     if (tile >= *p.num_tiles) return 0;
     const LoraTile d = p.tiles[tile];
     adapter = d.adapter;
@@ -215,13 +265,13 @@ __device__ __forceinline__ void down_sums(const LoraParams &p, const int *rows, 
     for (int i = 0; i < MT * RT; ++i) part[(wave * MT * RT + i) * 64 + lane] = acc[i / RT][i % RT];
     __syncthreads();
 }
-template <class E, int MT, int RT, bool GROUPED, int WAVES>
+template <class E, int MT, int RT, Find FIND, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void lora_down_kernel(LoraParams p) {
     constexpr int TR = MT * 16;
     __shared__ int rows[TR];
     __shared__ __attribute__((aligned(16))) char smem[WAVES * image_bytes<MT, RT>()];
     int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.x, rows, adapter);
+    const int count = tile_rows<TR, FIND, WAVES * 64>(p, blockIdx.x, rows, adapter);
     if (!count || adapter >= (int)p.a.n) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4, r0 = blockIdx.z * RT * 16;
     down_sums<E, MT, RT, WAVES>(p, rows, count, adapter, r0, blockIdx.y, smem);
@@ -343,7 +393,7 @@ __device__ __forceinline__ void up_columns(const LoraParams &p, const int *rows,
     }
 }
 
-template <class E, int MT, bool GROUPED>
+template <class E, int MT, Find FIND>
 __global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParams p, int groups) {
     typedef typename E::T T; typedef typename E::V V;
     constexpr int TR = MT * 16;
@@ -352,7 +402,7 @@ __global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParam
     __shared__ unsigned int high[TR];
     __shared__ int rows[TR];
     int adapter = -1;
-    const int count = tile_rows<TR, GROUPED>(p, blockIdx.y, rows, adapter);
+    const int count = tile_rows<TR, FIND, 256>(p, blockIdx.y, rows, adapter);
     if (!count) return;
     const int wave = threadIdx.x >> 6, R = (int)p.a.R, ldv = v_stride<E>(R);
     const bool real = adapter < (int)p.a.n;
@@ -404,49 +454,9 @@ __global__ __launch_bounds__(256, MT == 4 ? 3 : 1) void lora_up_kernel(LoraParam
     __syncthreads();
     up_columns<E, MT>(p, rows, count, adapter, hi, high, ldv, (blockIdx.x * 4 + wave) * groups, groups);
 }
-// rows of tile `tile` (16 rows), as tile_of_small, of up to kMany rows and fewer than 1024 adapters: a workgroup of 512 counts each adapter's rows, and the rows of the tile's adapter in their order
-__device__ __forceinline__ int tile_of_many(const LoraParams &p, int tile, int *rows, int &adapter) {
-    constexpr int PER = kMany / 512;
-    __shared__ int cnt[1024], waves[8 * PER], chosen[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = (int)p.a.T;
-    int id[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) id[e] = e * 512 + tid < T ? adapter_of(p, e * 512 + tid) : -1;
-    cnt[2 * tid] = cnt[2 * tid + 1] = 0;
-    if (tid == 0) chosen[0] = -1;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < PER; ++e) if (id[e] >= 0) atomicAdd(&cnt[id[e]], 1);
-    __syncthreads();
-    const int t0 = (cnt[2 * tid] + 15) / 16, t1 = (cnt[2 * tid + 1] + 15) / 16, upto = scan<int>(t0 + t1, waves), from = upto - t0 - t1;
-    if (from <= tile && tile < upto) {                                    // (one thread)
-        const bool second = tile >= from + t0;
-        chosen[0] = 2 * tid + second; chosen[1] = (tile - from - (second ? t0 : 0)) * 16;
-    }
-    __syncthreads();
-    if (chosen[0] < 0) return 0;
-    adapter = same(chosen[0]);
-    const int first = same(chosen[1]), count = same(min(16, cnt[adapter] - first));
-    unsigned long long mine[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        mine[e] = __ballot(id[e] == adapter);
-        if (lane == 0) waves[e * 8 + wave] = __popcll(mine[e]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        int rank = __popcll(mine[e] & ((1ull << lane) - 1)) - first;
-        for (int w = 0; w < e * 8 + wave; ++w) rank += waves[w];
-        if (id[e] == adapter && rank >= 0 && rank < 16) rows[rank] = e * 512 + tid;
-    }
-    __syncthreads();
-    return count;
-}
-
 // Both in one launch, where few rows (tiles of 16) meet few ranks (up to kRanks, 16 RT at a time): each workgroup forms v anew for its columns, 8 waves over K, and keeps it in LDS
 constexpr int kRanks = 96;
-template <class E, int RT, bool MANY>
+template <class E, int RT, Find FIND>
 __global__ __launch_bounds__(512) void lora_both_kernel(LoraParams p) {
     typedef typename E::T T;
     constexpr bool F = sizeof(T) == 4, H = __is_same(E, F16);
@@ -457,7 +467,7 @@ __global__ __launch_bounds__(512) void lora_both_kernel(LoraParams p) {
     __shared__ __attribute__((aligned(16))) T v[(F ? 1 : 2) * 16 * MOST];
     __shared__ float sums[RT == 1 ? 16 : kRanks][17];                     // [rank][row]
     int adapter = -1;
-    const int count = MANY ? tile_of_many(p, blockIdx.y, rows, adapter) : tile_of_small(p, blockIdx.y, rows, adapter);
+    const int count = tile_rows<16, FIND, 512>(p, blockIdx.y, rows, adapter);
     if (!count) return;
     const int tid = threadIdx.x, R = (int)p.a.R, ldv = v_stride<E>(R);
     T *hi = v, *lo = v + 16 * ldv;
@@ -506,18 +516,18 @@ size_t lora_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t R) {
     return (size_t)T * lora_splits_most(T, K) * lora_rp(R) * 4 + (T > kSmall ? ((size_t)T * (4 + sizeof(LoraTile)) + 64) : 0);
 }
 
-template <class E, int MT, bool GROUPED>
+template <class E, int MT, Find FIND>
 static void lora_launch(const LoraParams &p, int64_t tiles, hipStream_t s) {
     const int rt = (int)(p.rp / 16);
     const unsigned t = (unsigned)tiles, z = (unsigned)p.splits;
     constexpr int WAVES = MT == 4 ? 4 : 8;                                // tiles of 16 rows: more waves of a workgroup share K, and v has fewer shares to add up again
-    if (rt == 1) lora_down_kernel<E, MT, 1, GROUPED, WAVES><<<dim3(t, z, 1), WAVES * 64, 0, s>>>(p);
-    else lora_down_kernel<E, MT, 2, GROUPED, WAVES><<<dim3(t, z, (rt + 1) / 2), WAVES * 64, 0, s>>>(p);
+    if (rt == 1) lora_down_kernel<E, MT, 1, FIND, WAVES><<<dim3(t, z, 1), WAVES * 64, 0, s>>>(p);
+    else lora_down_kernel<E, MT, 2, FIND, WAVES><<<dim3(t, z, (rt + 1) / 2), WAVES * 64, 0, s>>>(p);
     constexpr int GN = E::W / 4 * 16;
     const int64_t all = (p.a.N + GN - 1) / GN;                            // groups of columns: a wave takes 1 to 4, as long as there are workgroups for two rounds of the chip
     int groups = 4;
     while (groups > 1 && (all + 4 * groups - 1) / (4 * groups) * tiles < 512) groups /= 2;
-    lora_up_kernel<E, MT, GROUPED><<<dim3((unsigned)((all + 4 * groups - 1) / (4 * groups)), t), 256, (size_t)MT * 16 * v_stride<E>((int)p.a.R) * 4, s>>>(p, groups);
+    lora_up_kernel<E, MT, FIND><<<dim3((unsigned)((all + 4 * groups - 1) / (4 * groups)), t), 256, (size_t)MT * 16 * v_stride<E>((int)p.a.R) * 4, s>>>(p, groups);
 }
 
 template <class E>
@@ -543,31 +553,32 @@ static int lora_of(const LoraArgs &a, hipStream_t s) {
     const bool apart = x0 + ((a.T - 1) * a.ldx + a.K) * size <= y0 || y0 + ((a.T - 1) * a.ldy + a.N) * size <= x0;
     const int64_t tiles16 = std::min<int64_t>(a.T, a.T / 16 + kinds);
     // One launch, as long as what its workgroups read again from the L2 caches (x and A of a tile for every 8 GN columns), and the way of one of them along K (for every 32 ranks), take less than the
-    // launches spared, one up to kSmall rows, two beyond.  us in one launch and in two or three, 16-bit types: 32 rows of 32 adapters of rank 16, 1024 -> 2048 (17 MB again) 5.3 9.0; 64 x 4096 -> 4096,
-    // rank 32 (57 MB) 10.6 10.8; 32 x 4096 -> 4096, rank 16 (134 MB) 11.2 9.6; 32 x 2048 -> 2048, rank 96 (3 x 4 KB along K) 14.2 9.6; 251 x 1024 -> 2048, rank 16 (12 MB) 6.2 13.2;
-    // 1000 x 1024 -> 4096, rank 16 (70 MB) 16.8 18.2; 512 x 1024 -> 12288, rank 16 (116 MB) 18.6 18.4; 251 x 4096 -> 4096, rank 32 (145 MB) 16.4 15.3; 200 x 4096 -> 1024, rank 96 (3 x 8 KB) 22.3 15.6.
-    // (Each workgroup reads x while others write y: they must not overlap.)
+    // launch spared and, beyond kSmall rows, the search for the tile in it.  us in one launch and in two, 16-bit types: 32 rows of 32 adapters of rank 16, 1024 -> 2048 (17 MB again) 5.3 9.0;
+    // 64 x 4096 -> 4096, rank 32 (57 MB) 10.6 10.8; 32 x 4096 -> 4096, rank 16 (134 MB) 11.2 9.6; 32 x 2048 -> 2048, rank 96 (3 x 4 KB along K) 14.2 9.6; 251 x 4096 -> 4096, rank 16 (80 MB) 10.6 12.2,
+    // rank 32 (145 MB) 16.4 13.5; 512 x 1024 -> 1024, rank 64 (2 x 24 MB) 9.7 12.4; 512 x 1024 -> 12288, rank 16 (116 MB) 19.0 17.0.  (Each workgroup reads x while others write y: they must not overlap.)
     const int64_t rounds = a.R <= 16 ? 1 : (a.R + 31) / 32, again = rounds * columns * tiles16 * (16 + p.rp) * row;
-    const bool little = a.T <= kSmall ? rounds * row <= 8192 && again <= 64ll << 20 : a.T <= kMany && a.n < 1023 && rounds * row <= 12288 && again <= 128ll << 20;
-    if (apart && a.R <= kRanks && little) {
+    const bool found = a.T <= kSmall || (a.T <= kMany && a.n < 1023), little = rounds * row <= 8192 && again <= (a.T <= kSmall ? 64ll : 96ll) << 20;
+    if (apart && found && little && a.R <= kRanks) {
         p.splits = 1;
         const dim3 grid((unsigned)columns, (unsigned)tiles16);
         if (a.T <= kSmall) {
-            if (a.R <= 16) lora_both_kernel<E, 1, false><<<grid, 512, 0, s>>>(p);
-            else lora_both_kernel<E, 2, false><<<grid, 512, 0, s>>>(p);
+            if (a.R <= 16) lora_both_kernel<E, 1, SMALL><<<grid, 512, 0, s>>>(p);
+            else lora_both_kernel<E, 2, SMALL><<<grid, 512, 0, s>>>(p);
         } else {
-            if (a.R <= 16) lora_both_kernel<E, 1, true><<<grid, 512, 0, s>>>(p);
-            else lora_both_kernel<E, 2, true><<<grid, 512, 0, s>>>(p);
+            if (a.R <= 16) lora_both_kernel<E, 1, MANY><<<grid, 512, 0, s>>>(p);
+            else lora_both_kernel<E, 2, MANY><<<grid, 512, 0, s>>>(p);
         }
-    } else if (a.T > kSmall) {
+    } else if (a.T <= kSmall) lora_launch<E, 1, SMALL>(p, tiles, s);
+    else if (tr == 16 && found) lora_launch<E, 1, MANY>(p, tiles, s);      // (251 x 4096 -> 4096, rank 64: 15.0 us, grouped by a launch 17.0)
+    else {
         char *at = (char *)a.workspace + (size_t)a.T * lora_splits_most(a.T, a.K) * p.rp * 4;
         LoraTile *td = (LoraTile *)at;
         int32_t *order = (int32_t *)(at + (size_t)a.T * sizeof(LoraTile)), *nt = order + a.T;
         p.tiles = td; p.order = order; p.num_tiles = nt;
         lora_group_kernel<<<dim3(1), dim3(1024), (size_t)(a.n + 1) * 4, s>>>(p, tr, order, td, nt);
-        if (tr == 64) lora_launch<E, 4, true>(p, tiles, s);
-        else lora_launch<E, 1, true>(p, tiles, s);
-    } else lora_launch<E, 1, false>(p, tiles, s);
+        if (tr == 64) lora_launch<E, 4, GROUPED>(p, tiles, s);
+        else lora_launch<E, 1, GROUPED>(p, tiles, s);
+    }
     NVR_KX_LAUNCHED("lora_add");
     return 0;
 }
