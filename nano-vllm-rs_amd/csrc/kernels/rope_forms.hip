@@ -8,6 +8,7 @@
 // Bound by memory: a thread takes 16 bytes of either half of a pair, everything is read and written once.  32768 tokens of 16 + 8 + 8 heads of 128, float16: 109 us, 5.5 TB/s (a large copy: 5.1; four tokens a workgroup: 117);
 // 1531 tokens of 32 + 8 + 8 heads, float32, half of each head turning: 15 us, 5.5 TB/s; 32 tokens: 3.5 us, a launch's own time.
 #include <algorithm>
+#include <type_traits>
 #include "serving.h"
 #include "elem.h"
 #include "../common.h"
@@ -15,7 +16,7 @@
 namespace nvr { namespace kx {
 
 // A unit is two pieces of W numbers that turn together (W pairs), or one piece that is passed on.  Units of a token: q heads, then k heads (each `rotary / 2W` turning ones, then the rest of the
-// head), then v pieces.  A workgroup a token.
+// head), then v pieces.  `tok` tokens a workgroup.
 template <class E, int W>
 struct Piece { typename E::T v[W]; };
 template <class E, int W>
@@ -42,21 +43,26 @@ __device__ __forceinline__ void put(typename E::T *p, const float (&x)[W]) {
     }
 }
 
-template <class E, int W, bool PAIRS>
-__global__ __launch_bounds__(256) void rope_rotate_store_kernel(RopeArgs a) {
+template <class E, int W, bool PAIRS, bool ONE>
+__global__ __launch_bounds__(256) void rope_rotate_store_kernel(RopeArgs a, int several) {
     typedef typename E::T T;
-    extern __shared__ float2 turn[];                                      // [rotary / 2]: cos, sin
+    const int tok = ONE ? 1 : several;                                    // (compiled for one: the divisions are 2 % of large steps)
+    extern __shared__ float2 turn[];                                      // [tok][rotary / 2]: cos, sin
     const int half = a.rotary / 2, D = a.D;
-    const int64_t row = blockIdx.x;
-    for (int i = threadIdx.x; i < half; i += 256) {
-        const double at = (double)a.positions[row], per = a.turns[i];
+    const int64_t t0 = (int64_t)blockIdx.x * tok;
+    const int nt = (int)min((int64_t)tok, a.T - t0);
+    for (int i = threadIdx.x; i < nt * half; i += 256) {
+        const int t = ONE ? 0 : i / half;
+        const double at = (double)a.positions[t0 + t], per = a.turns[i - t * half];
         double s, c;
         sincospi(2.0 * fma(at, per, -rint(at * per)), &s, &c);            // (the part of a turn without a rounding of the product)
         turn[i] = make_float2((float)(c * a.amplitude), (float)(s * a.amplitude));
     }
     __syncthreads();
     const int turning = half / W, per_head = turning + (D - a.rotary) / W, hk = (a.H + a.KVH) * per_head, units = hk + (a.v_cache ? a.KVH * (D / W) : 0);
-    for (int u = threadIdx.x; u < units; u += 256) {
+    for (int i = threadIdx.x; i < nt * units; i += 256) {
+        const int t = ONE ? 0 : i / units, u = i - t * units;
+        const int64_t row = t0 + t;
         int64_t slot = -1;
         if (u >= a.H * per_head && a.k_cache) { slot = a.slots[row]; if (slot >= a.num_slots) slot = -1; }
         if (u >= hk) {                                                    // v: a copy
@@ -77,7 +83,7 @@ __global__ __launch_bounds__(256) void rope_rotate_store_kernel(RopeArgs a) {
         if (in < turning) {
             const int at = PAIRS ? 2 * W * in : W * in, two = PAIRS ? at + W : at + half;
             get<E, W>(src + at, x); get<E, W>(src + two, y);
-            const float2 *cs = turn + W * in;
+            const float2 *cs = turn + t * half + W * in;
             if constexpr (PAIRS && W > 1) {                               // pairs (2 j, 2 j + 1): W / 2 of them in either piece
 #pragma unroll
                 for (int e = 0; e < W; e += 2) {
@@ -110,15 +116,20 @@ static int rope_of(const RopeArgs &a, hipStream_t s) {
     constexpr int W = E::W;
     const uintptr_t bytes = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache;
     const bool wide = (bytes & 15) == 0 && ((a.H ? a.ldq | a.ldqo : 0) | (a.KVH ? a.ldk : 0) | (a.k_out ? a.ldko : 0) | (a.v_cache ? a.ldv : 0)) % W == 0 && a.D % W == 0 && a.rotary % (2 * W) == 0;
-    const size_t lds = (size_t)(a.rotary / 2) * sizeof(float2);
-    const dim3 grid((unsigned)a.T), block(256);
-    if (wide) {
-        if (a.pairs) rope_rotate_store_kernel<E, W, true><<<grid, block, lds, s>>>(a);
-        else rope_rotate_store_kernel<E, W, false><<<grid, block, lds, s>>>(a);
-    } else {
-        if (a.pairs) rope_rotate_store_kernel<E, 1, true><<<grid, block, lds, s>>>(a);
-        else rope_rotate_store_kernel<E, 1, false><<<grid, block, lds, s>>>(a);
-    }
+    // tokens of a workgroup: as many as give its threads a unit each, as long as there are two workgroups a CU (8872 tokens of 2 + 2 + 2 heads of 128: 9.8 us, one a workgroup 12.4; 24 heads: 109, four 117)
+    const int V = wide ? W : 1, units = (a.H + a.KVH) * (a.rotary / 2 / V + (a.D - a.rotary) / V) + (a.v_cache ? a.KVH * (a.D / V) : 0);
+    const int tok = (int)std::max<int64_t>(1, std::min<int64_t>(256 / units, a.T / 512));
+    const size_t lds = (size_t)tok * (a.rotary / 2) * sizeof(float2);
+    const dim3 grid((unsigned)((a.T + tok - 1) / tok)), block(256);
+    auto launch = [&](auto w, auto one) {
+        constexpr int N = decltype(w)::value;
+        constexpr bool ONE = decltype(one)::value;
+        if (a.pairs) rope_rotate_store_kernel<E, N, true, ONE><<<grid, block, lds, s>>>(a, tok);
+        else rope_rotate_store_kernel<E, N, false, ONE><<<grid, block, lds, s>>>(a, tok);
+    };
+    if (!wide) launch(std::integral_constant<int, 1>(), std::false_type());
+    else if (tok == 1) launch(std::integral_constant<int, W>(), std::true_type());
+    else launch(std::integral_constant<int, W>(), std::false_type());
     NVR_KX_LAUNCHED("rope_rotate_store");
     return 0;
 }
