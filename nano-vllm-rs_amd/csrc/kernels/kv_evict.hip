@@ -7,6 +7,7 @@
 // 32 sequences of 1000 .. 8100 keys of 8 heads of 128 to 2048, float16, other blocks: 117 us (17 and 99), 4.2 TB/s over both, 4.9 in the copy (a large copy: 5.1); one of 4099 keys: 16 us (11 and 5).
 // The select's life is a chain of some twenty LDS round trips and barriers; ballots in place of a thread's run of keys, and a count of a digit's few keys in place of its last two passes, took as long.
 #include <algorithm>
+#include <type_traits>
 #include "serving.h"
 #include "elem.h"
 #include "scan.h"
@@ -102,54 +103,60 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     } else
         for (int i = tid; i < here; i += kPick) held[i] = a.scores[from_at(i)];
     __syncthreads();
-    auto score = [&](int i) { return i < p.held ? held[i] : a.scores[from_at(i)]; };
-    // ---- the rank of the last of the best: the `need` best of keys first .. end - 1, of equal ones the earliest `want`
-    const int first = a.first, end = len - a.last;
-    const unsigned int need = all ? 0 : a.budget - a.first - a.last;      // (fewer than compete)
-    unsigned int prefix = 0xffffffffu, want = 0;
-    if (need) {
-        unsigned int mask = 0;
-        prefix = 0; want = need;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
-            for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass * kRadix + wide - 1 - ((k >> at) & (wide - 1))], 1u); }
-            __syncthreads();
-            const unsigned int c0 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid] : 0, c1 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid + 1] : 0;
-            const unsigned int v = scan<unsigned int>(c0 + c1, waves) - c0 - c1;      // in front of this thread's two digits
-            if (v < want && v + c0 + c1 >= want) {                        // (one thread)
-                const bool odd = v + c0 < want;
-                found[pass] = 2 * tid + odd; above[pass] = odd ? v + c0 : v;
-            }
-            __syncthreads();
-            prefix |= (unsigned int)(wide - 1 - found[pass]) << at; mask |= (unsigned int)(wide - 1) << at;
-            want -= above[pass];
-        }
-    }
-    // ---- a thread's run of keys: how many of them are kept, and where they begin
-    const int per = (len + kPick - 1) / kPick, i0 = min(len, tid * per), i1 = min(len, i0 + per);
-    unsigned int more = 0, same = 0;
-    for (int i = i0; i < i1; ++i) {
-        const bool always = all || i < first || i >= end;
-        const unsigned int k = always ? 0 : rank_of(score(i));
-        more += always || (need && k > prefix); same += !always && need && k == prefix;
-    }
-    const unsigned long long own = ((unsigned long long)more << 32) | same, v = scan<unsigned long long>(own, waves2) - own;
-    // the scores at their new places: at once where LDS has them all
     const bool together = len <= p.held;
-    unsigned int seen = (unsigned int)v, at = (unsigned int)(v >> 32) + min(seen, want);
-    for (int i = i0; i < i1; ++i) {
-        const bool always = all || i < first || i >= end;
-        const float f = score(i);
-        const unsigned int k = always ? 0 : rank_of(f);
-        const bool tie = !always && need && k == prefix;
-        if (always || (need && k > prefix) || (tie && seen < want)) {
-            kept[at] = i;
-            if (together) a.scores[to_at((int)at)] = f;
-            ++at;
+    // everything: LDS has all scores, and no other place is looked at (a loop of half the instructions: 8 x 48 .. 21715 keys 32.3 -> 25.8 us)
+    auto choose = [&](auto everything) {
+        constexpr bool ALL = decltype(everything)::value;
+        auto score = [&](int i) { return ALL || i < p.held ? held[i] : a.scores[from_at(i)]; };
+        // ---- the rank of the last of the best: the `need` best of keys first .. end - 1, of equal ones the earliest `want`
+        const int first = a.first, end = len - a.last;
+        const unsigned int need = all ? 0 : a.budget - a.first - a.last;      // (fewer than compete)
+        unsigned int prefix = 0xffffffffu, want = 0;
+        if (need) {
+            unsigned int mask = 0;
+            prefix = 0; want = need;
+            for (int pass = 0; pass < 3; ++pass) {
+                const int at = pass == 0 ? 21 : pass == 1 ? 10 : 0, wide = pass == 2 ? 1024 : 2048;
+#pragma unroll 4
+                for (int i = first + tid; i < end; i += kPick) { const unsigned int k = rank_of(score(i)); if ((k & mask) == prefix) atomicAdd(&hist[pass * kRadix + wide - 1 - ((k >> at) & (wide - 1))], 1u); }
+                __syncthreads();
+                const unsigned int c0 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid] : 0, c1 = 2 * tid < wide ? hist[pass * kRadix + 2 * tid + 1] : 0;
+                const unsigned int v = scan<unsigned int>(c0 + c1, waves) - c0 - c1;      // in front of this thread's two digits
+                if (v < want && v + c0 + c1 >= want) {                        // (one thread)
+                    const bool odd = v + c0 < want;
+                    found[pass] = 2 * tid + odd; above[pass] = odd ? v + c0 : v;
+                }
+                __syncthreads();
+                prefix |= (unsigned int)(wide - 1 - found[pass]) << at; mask |= (unsigned int)(wide - 1) << at;
+                want -= above[pass];
+            }
         }
-        seen += tie;
-    }
-    if (together) return;
+        // ---- a thread's run of keys: how many of them are kept, and where they begin
+        const int per = (len + kPick - 1) / kPick, i0 = min(len, tid * per), i1 = min(len, i0 + per);
+        unsigned int more = 0, same = 0;
+        for (int i = i0; i < i1; ++i) {
+            const bool always = all || i < first || i >= end;
+            const unsigned int k = always ? 0 : rank_of(score(i));
+            more += always || (need && k > prefix); same += !always && need && k == prefix;
+        }
+        const unsigned long long own = ((unsigned long long)more << 32) | same, v = scan<unsigned long long>(own, waves2) - own;
+        // the scores at their new places: at once where LDS has them all
+        unsigned int seen = (unsigned int)v, at = (unsigned int)(v >> 32) + min(seen, want);
+        for (int i = i0; i < i1; ++i) {
+            const bool always = all || i < first || i >= end;
+            const float f = score(i);
+            const unsigned int k = always ? 0 : rank_of(f);
+            const bool tie = !always && need && k == prefix;
+            if (always || (need && k > prefix) || (tie && seen < want)) {
+                kept[at] = i;
+                if (ALL) a.scores[to_at((int)at)] = f;
+                ++at;
+            }
+            seen += tie;
+        }
+    };
+    if (together) return choose(std::true_type());
+    choose(std::false_type());
     __threadfence_block();
     __syncthreads();
     for (int j0 = 0; j0 < n; j0 += kPick) {                               // from the front: of a step all are read before any is written
