@@ -4,7 +4,7 @@
 // order (each thread owns a run of keys; one scan tells where its kept ones go) and the scores at their new places.  Second launch: the rows of K and V.
 // Into other blocks, every row is on its own: a copy, bound by memory.  In place, row i comes from row kept[i] >= i, which is overwritten by a later row: a workgroup takes a (sequence, kv head)'s
 // strip of 128 bytes of the rows, from the front in steps of kMoves requests: all of a step are read before any is written, and no later step reads what it writes.
-// 32 sequences of 1000 .. 8100 keys of 8 heads of 128 to 2048, float16, other blocks: 117 us (17 and 99), 4.2 TB/s over both, 4.9 in the copy (a large copy: 5.1); one of 4099 keys: 16 us (11 and 5).
+// 32 sequences of 1000 .. 8100 keys of 8 heads of 128 to 2048, float16, other blocks: 111 us (15 and 94), 4.4 TB/s over both, 5.2 in the copy (a large copy: 5.1); one of 4099 keys: 15 us (11 and 4).
 // The select's life is a chain of some twenty LDS round trips and barriers; ballots in place of a thread's run of keys, and a count of a digit's few keys in place of its last two passes, took as long.
 #include <algorithm>
 #include <type_traits>

@@ -18,7 +18,7 @@ namespace nvr { namespace kx {
 
 namespace {
 constexpr int kSmall = 64;                                                // rows up to which a workgroup finds its tile itself (64 x 1024 -> 2048 of rank 64: 11.1 us, grouped by a launch 12.9)
-constexpr int kMany = 1024;                                               // rows up to which it counts them
+constexpr int kMany = 1024;                                               // ... counts the adapters' rows for it
 constexpr int kMaxAdapters = 8192;                                        // counters of the grouping launch (LDS)
 
 struct LoraTile { int32_t start, count, adapter; };                       // rows order[start ..) of one adapter; adapter n: rows without one
