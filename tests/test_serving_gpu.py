@@ -939,3 +939,25 @@ def test_lora_rows_found_by_each_workgroup(arena, dtype, T, K, N, R, n):
     assert np.array_equal(a, lora_case(arena, dtype, T, K, N, R, n, rng.integers(-1, n, T), seed=1))
     lora_case(arena, dtype, T, K, N, R, n, np.full(T, n - 1))
     lora_case(arena, dtype, T, K, N, R, n, np.full(T, -1))
+
+
+def test_copies_to_the_host_wait_for_every_stream(arena):
+    """What a stream still has to write is in a copy to the host that follows its launches: products for some milliseconds, then a token a row."""
+    typed("float16")
+    stream = C.c_void_p()
+    nvr.check(L.nvr_stream_create(byref(stream)))
+    T, K = 4096, 4096
+    x, w, y = arena.space(T * K * 2, 0), arena.space(K * K * 2, 0), arena.space(T * K * 2, 0)
+    B, V = 4, 1000
+    rng = np.random.default_rng(1)
+    logits = rng.standard_normal((B, V)).astype(np.float32)
+    d, u, ids, ws = arena.dev(logits), arena.dev(np.zeros(B, np.float32)), arena.space(B * 8), arena.space(L.nvr_sample_uniform_workspace_bytes(B, V))
+    t = arena.dev(np.zeros(B, np.float32))
+    nvr.synchronize()
+    for _ in range(30):
+        nvr.check(L.nvr_linear(x.ptr, K, w.ptr, T, K, K, y.ptr, 0, stream))
+    nvr.check(L.nvr_sample_uniform(d.ptr, V, B, V, t.ptr, None, None, None, u.ptr, ids.ptr, None, ws.ptr, stream))
+    got = np.empty(B, np.int64)
+    nvr.check(L.nvr_memcpy_d2h(got.ctypes.data, ids.ptr, got.nbytes))
+    assert got.tolist() == logits.argmax(1).tolist()
+    nvr.check(L.nvr_stream_destroy(stream))
