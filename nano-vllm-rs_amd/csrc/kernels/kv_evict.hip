@@ -244,7 +244,7 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     p.per_block = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / (uint64_t)a.block_size);
     p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
     const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
-    p.held = std::min((a.max_ctx + 3) / 4 * 4, kHeld);
+    p.held = (int32_t)std::min<int64_t>(((int64_t)a.max_ctx + 3) / 4 * 4, kHeld);
     static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv_evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
     if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "%s: LDS of %d bytes: %s", me, kHeld * 4, hipGetErrorString(opted));
     kv_evict_select_kernel<<<dim3(G, B), kPick, (size_t)p.held * 4, s>>>(p);

@@ -961,3 +961,8 @@ def test_copies_to_the_host_wait_for_every_stream(arena):
     nvr.check(L.nvr_memcpy_d2h(got.ctypes.data, ids.ptr, got.nbytes))
     assert got.tolist() == logits.argmax(1).tolist()
     nvr.check(L.nvr_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_without_a_bound_on_contexts(arena, out_of_place):
+    evict_case(arena, "float16", [300, 40, 299], 2, 64, 16, 100, 4, 32, out_of_place, max_context=2 ** 31 - 1)
