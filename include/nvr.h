@@ -690,7 +690,7 @@ typedef struct nvr_rope_scaling {
 NVR_API int nvr_rope_frequencies(const nvr_rope_scaling *sc, int64_t rotary_dim, double *turns_dev, float *amplitude);
 /* Rotates the first rotary_dim columns of every head of q [T, H, D] and k [T, KVH, D] (rows ldq / ldk numbers apart): pairs are columns (j, j + rotary_dim / 2), or (2j, 2j + 1) with
  * interleaved != 0; the other columns pass through.  q_out / k_out may be q / k themselves (with the same stride).  With caches [num_slots, KVH, D], the k rows (k_out may then be null) and the v
- * rows [T, KVH, D] are also stored at slot_mapping (a slot outside 0 .. num_slots - 1: not stored; two rows of one slot: either).  Caches, v and slot_mapping may be null together.
+ * rows [T, KVH, D] are also stored at slot_mapping (a slot outside 0 .. num_slots - 1: not stored; two rows of one slot leave pieces of either).  Caches, v and slot_mapping may be null together.
  * T up to 2^23. */
 NVR_API int nvr_rope_rotate_store_kv(const nvr_half *q, int64_t ldq, const nvr_half *k, int64_t ldk, const nvr_half *v, int64_t ldv, const int64_t *positions,
                                      const int32_t *slot_mapping, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t rotary_dim, int interleaved, const double *turns,
