@@ -23,6 +23,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kUnit = 128;                                                // keys of a unit: a tile of 32 (32 bits: two of 16) for each wave
 struct ScoredParams {
     ScoredArgs a;
+    int32_t wide;                                                         // WHOLE: scores of a head in LDS
     int32_t shares, lpad;                                                 // workgroups of a kv head, scores of a head in the workspace
     float *s, *ml, *o;                                                    // [B][H][lpad], [shares + B][H][2], [shares + B][H][D]: share w's part of sequence b at w + b
     int32_t *ends;                                                        // [B][2]: the first and the last share of a sequence
@@ -41,7 +42,7 @@ struct Image {
     static constexpr int TK = sizeof(typename E::T) == 4 ? 16 : 32;                                   // keys of a tile
     static constexpr int ROW = D * (int)sizeof(typename E::T), LPR = ROW / 16, RPI = 64 / LPR, NI = TK / RPI;   // bytes of a row, lanes of it, rows of a request, requests of a tile
     static constexpr int VS = ROW + (sizeof(typename E::T) == 4 ? 16 : 32);                           // V: stride of a row (conflict-free transposed reads)
-    static constexpr int KB = TK * ROW, BYTES = KB + TK * VS, OS = D + 4;                               // K's image, both; numbers of a row of the waves' sums
+    static constexpr int KB = TK * ROW, BYTES = KB + TK * VS, OS = D + 4, ALL = 4 * BYTES > 4 * 16 * OS * 4 ? 4 * BYTES : 4 * 16 * OS * 4;                               // K's image, both; numbers of a row of the waves' sums; bytes of either for four waves
 };
 // operand of O^T += V^T P^T: column (of 16) lm of V, keys 4 lq .. at `a` and 16 further at `b`, by the transposing reads
 template <class E>
@@ -61,7 +62,9 @@ __device__ __forceinline__ typename E::V transposed(const char *a, const char *b
 }
 }  // namespace
 
-template <class E, int D>
+// WHOLE: contexts are short, and a workgroup has a sequence's keys of a kv head and answers by itself, scores in LDS: no second launch, no workspace.  us where it answers and with two launches: 5 sequences
+// of up to 60 keys 5.2 10.7, 32 of 20 .. 250 9.1 11.9, 32 of 200 .. 500 16.8 19.9, 64 of 100 .. 500 (4 heads a kv head) 19.7 26.9; 8 of 200 .. 500 14.2 11.6, 32 of 100 .. 1000 24.6 20.0
+template <class E, int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(ScoredParams p) {
     typedef typename E::T T; typedef typename E::V V;
     typedef Image<E, D> I;
@@ -70,6 +73,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float ml[4][16][2];
     __shared__ int sums[4], at[2];
+    __shared__ float big[16], inv[16];
     const int g = blockIdx.x, w = blockIdx.y;                             // (kv heads of the same keys next to each other: their rows are neighbours)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
     const int G = p.a.H / p.a.KVH;
@@ -81,7 +85,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
         u0 = (int)((int64_t)w * all / shares); u1 = (int)((int64_t)(w + 1) * all / shares);
         return true;
     };
-    if (p.a.B <= 64) {                                                    // a lane a sequence, every wave for itself
+    if constexpr (WHOLE) {
+        b = w; unit = 0; u0 = 0; u1 = units_of(p.a, b);
+        if (u1 == 0) {
+            T *out = (T *)p.a.out + ((int64_t)b * p.a.H + g * G) * D;
+            for (int i = threadIdx.x; i < G * D; i += 256) out[i] = (T)0.f;
+            return;
+        }
+    } else if (p.a.B <= 64) {                                             // a lane a sequence, every wave for itself
         const int mine = lane < p.a.B ? units_of(p.a, lane) : 0;
         int upto = mine;
 #pragma unroll
@@ -114,13 +125,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
     const int64_t row_elems = (int64_t)p.a.KVH * D;
     const T *kc = (const T *)p.a.k + (int64_t)g * D, *vc = (const T *)p.a.v + (int64_t)g * D;
     char *img = smem + wave * I::BYTES;
+    float *kept = reinterpret_cast<float *>(smem + I::ALL);               // WHOLE: scores of the heads, p.wide apart
     const int rl = lane / I::LPR, pl = lane % I::LPR;                     // this lane's row of a request and its piece
     for (int left = u1 - u0; left > 0; ++b, unit = 0) {
         const int ctx = visible(p.a, b), units = (ctx + kUnit - 1) / kUnit, take = min(left, units - unit);
         if (take <= 0) continue;                                              // (a sequence without keys)
         left -= take;
         const int first = unit * kUnit, last = min(ctx, first + take * kUnit);
-        if (g == 0 && threadIdx.x == 0) {
+        if (!WHOLE && g == 0 && threadIdx.x == 0) {
             if (unit == 0) p.ends[2 * b] = w;
             if (unit + take == units) p.ends[2 * b + 1] = w;
         }
@@ -159,7 +171,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
         for (int t = 0; t < DT; ++t) o[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
         constexpr unsigned int kAll = I::TK == 32 ? 0xffffffffu : 0xffffu;
         char *vimg = img + I::KB;
-        float *sp = p.s + ((int64_t)b * p.a.H + g * G + lm) * p.lpad;
+        float *sp = WHOLE ? kept + lm * p.wide : p.s + ((int64_t)b * p.a.H + g * G + lm) * p.lpad;
         unsigned int mask = 0;
         int page = 0;
         if (wave < tiles) {
@@ -268,9 +280,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
                 v += *reinterpret_cast<const float4_t *>(so + (i * 16 + h) * I::OS + c) * f;
                 L = fmaf(ml[i][h][1], f, L);
             }
+            if constexpr (WHOLE) {
+                const float n = L == 0.f ? 0.f : 1.f / L;                 // (no key: output and weights of 0)
+                T *out = (T *)p.a.out + ((int64_t)b * p.a.H + g * G + h) * D + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = (T)(v[e] * n);
+                if (c == 0) { big[h] = Ms; inv[h] = n; }
+                continue;
+            }
             const int64_t to = (int64_t)(w + b) * p.a.H + g * G + h;
             *reinterpret_cast<float4_t *>(p.o + to * D + c) = v;
             if (c == 0) { p.ml[2 * to] = M; p.ml[2 * to + 1] = L; }
+        }
+        if constexpr (WHOLE) {
+            __syncthreads();
+            const int scored = p.a.scored ? p.a.scored[b] : ctx - 1;
+            for (int j = threadIdx.x; j < ctx; j += 256) {
+                const int block = (int)((unsigned)j / (unsigned)p.a.block_size), page = table[block];
+                if (page < 0 || page >= p.a.num_blocks) continue;
+                const int64_t to = ((int64_t)page * p.a.KVH + g) * p.a.block_size + (j - block * p.a.block_size);
+                float sum = 0.f;
+                for (int h = 0; h < G; ++h) sum = fmaf(__builtin_amdgcn_exp2f(kept[h * p.wide + j] - big[h]), inv[h], sum);
+                p.a.new_scores[to] = j < scored ? fmaf(p.a.decay, p.a.scores[to], sum) : sum;
+            }
+            return;
         }
         if (left > 0) __syncthreads();
     }
@@ -373,21 +406,32 @@ namespace {
 int scored_shares(int64_t B, int64_t KVH, int64_t D, int64_t max_ctx) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((D == 256 ? 256 : 512) / KVH, B * ((max_ctx + kUnit - 1) / kUnit)));
 }
+// one launch: up to 256 keys; up to 512 where there are sequences enough for the chip and two workgroups fit a CU
+constexpr size_t kLds = 160 * 1024 - 2048;
+template <class E> size_t image_of(int D) { return D == 64 ? Image<E, 64>::ALL : D == 128 ? Image<E, 128>::ALL : Image<E, 256>::ALL; }
+bool whole_of(const ScoredArgs &a, int dt, int wide) {
+    size_t lds = 0;
+    NVR_BY_DTYPE(dt, lds = image_of<E>(a.D));
+    lds += (size_t)(a.H / a.KVH) * wide * 4;
+    if (a.max_ctx <= 256) return lds <= kLds;
+    return a.max_ctx <= 512 && (int64_t)a.B * a.KVH >= 256 && lds <= kLds / 2;
+}
 struct ScoredSpace { size_t s, o, ml, ends; };
 ScoredSpace scored_space(int64_t B, int64_t H, int64_t KVH, int64_t D, int64_t max_ctx, int &shares, int &lpad) {
     shares = scored_shares(B, KVH, D, max_ctx);
     lpad = (int)((max_ctx + kUnit - 1) / kUnit * kUnit);
     return ScoredSpace{(size_t)B * H * lpad * 4, (size_t)(shares + B) * H * D * 4, (size_t)(shares + B) * H * 8, (size_t)B * 8};
 }
-template <class E, int D>
+template <class E, int D, bool WHOLE>
 int scored_launch(const ScoredParams &p, hipStream_t s) {
     typedef Image<E, D> I;
-    constexpr size_t lds = 4 * I::BYTES > 4 * 16 * I::OS * 4 ? 4 * I::BYTES : 4 * 16 * I::OS * 4;
-    if constexpr (lds > 48 * 1024) {
-        static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_scored_kernel<E, D>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "nvr_paged_attn_decode_scored: LDS of %zu bytes: %s", lds, hipGetErrorString(opted));
+    constexpr size_t most = WHOLE ? kLds : I::ALL;
+    const size_t lds = I::ALL + (WHOLE ? (size_t)(p.a.H / p.a.KVH) * p.wide * 4 : 0);
+    if constexpr (most > 48 * 1024) {
+        static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_scored_kernel<E, D, WHOLE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "nvr_paged_attn_decode_scored: LDS of %zu bytes: %s", most, hipGetErrorString(opted));
     }
-    attn_scored_kernel<E, D><<<dim3((unsigned)p.a.KVH, (unsigned)p.shares), 256, lds, s>>>(p);
+    attn_scored_kernel<E, D, WHOLE><<<dim3((unsigned)p.a.KVH, (unsigned)(WHOLE ? p.a.B : p.shares)), 256, lds, s>>>(p);
     return 0;
 }
 }  // namespace
@@ -418,10 +462,17 @@ int paged_attn_scored(int dt, const ScoredArgs &a, hipStream_t s) {
     p.a.max_ctx = a.max_ctx;
     const int W = dt == DT_F32 ? 4 : 8;
     p.qw = ((uintptr_t)a.q & 15) == 0 && a.ldq % W == 0;
+    p.wide = (int)(((int64_t)a.max_ctx + 31) / 32 * 32 + 4);                // (tiles of 32 keys; rows in other banks)
     int rc = 0;
-    NVR_BY_DTYPE(dt, rc = a.D == 64 ? scored_launch<E, 64>(p, s) : a.D == 128 ? scored_launch<E, 128>(p, s) : scored_launch<E, 256>(p, s));
+    const bool whole = whole_of(a, dt, p.wide);
+    if (whole) NVR_BY_DTYPE(dt, (rc = a.D == 64 ? scored_launch<E, 64, true>(p, s) : a.D == 128 ? scored_launch<E, 128, true>(p, s) : scored_launch<E, 256, true>(p, s)));
+    else NVR_BY_DTYPE(dt, (rc = a.D == 64 ? scored_launch<E, 64, false>(p, s) : a.D == 128 ? scored_launch<E, 128, false>(p, s) : scored_launch<E, 256, false>(p, s)));
     if (rc) return rc;
-    const int64_t ctx = std::max(a.max_ctx, 1);
+    if (whole) {
+        NVR_KX_LAUNCHED("paged_attn_scored");
+        return 0;
+    }
+    const int64_t ctx = a.max_ctx;
     constexpr int keys = 4 * kJoin;
     const int64_t wide = std::max<int64_t>((ctx + keys - 1) / keys, a.H / a.KVH);       // (a head of the group each at least: 5 sequences of up to 60 keys, 8 heads a kv head 13.7 us with one workgroup for all)
     NVR_BY_DTYPE(dt, (attn_scored_join_kernel<E><<<dim3((unsigned)wide, (unsigned)a.KVH, (unsigned)a.B), kJoin, 0, s>>>(p)));

@@ -588,9 +588,9 @@ class Step:
     """One layer's decode step of a batch whose requests have adapters of their own and whose caches are held to a budget, then a token each: the framework's product, nvr_lora_add beside it,
     nvr_rope_rotate_store_kv, nvr_paged_attn_decode_scored, nvr_kv_evict, nvr_linear + nvr_lora_add for the output, logits, nvr_sample_uniform."""
 
-    def __init__(self, arena, dtype, stream=None, seed=0):
+    def __init__(self, arena, dtype, stream=None, seed=0, bound=128):
         rng = np.random.default_rng(seed)
-        self.arena, self.dtype, self.stream, self.rng = arena, dtype, stream, rng
+        self.arena, self.dtype, self.stream, self.rng, self.bound = arena, dtype, stream, rng, bound
         typed(dtype)
         self.W, self.H, self.G, self.D, self.R, self.n, self.V, self.block, self.budget, self.first, self.last = 256, 4, 2, 64, 8, 3, 1024, 16, 48, 2, 8
         self.lengths = [60, 47, 30, 52, 48]
@@ -614,7 +614,7 @@ class Step:
                   "scores": arena.dev(self.s0), "qkv": arena.space(B * N * self.w), "q": arena.space(B * self.H * self.D * self.w), "out": arena.space(B * self.H * self.D * self.w),
                   "o": arena.space(B * self.W * self.w), "logits": arena.space(B * self.V * 4), "new_lens": arena.space(B * 4), "kept": arena.space(B * self.G * self.budget * 4),
                   "token": arena.space(B * 8), "logprob": arena.space(B * 4), "ws_lora": arena.space(L.nvr_lora_workspace_bytes(B, self.H * self.D, N, self.R)),
-                  "ws_attn": arena.space(L.nvr_paged_attn_scored_workspace_bytes(B, self.H, self.G, self.D, 128)), "ws_sample": arena.space(L.nvr_sample_uniform_workspace_bytes(B, self.V)),
+                  "ws_attn": arena.space(L.nvr_paged_attn_scored_workspace_bytes(B, self.H, self.G, self.D, bound)), "ws_sample": arena.space(L.nvr_sample_uniform_workspace_bytes(B, self.V)),
                   "T": arena.dev(np.array([0.0, 0.7, 1.0, 1.3, 0.9], np.float32)), "tk": arena.dev(np.array([0, 20, 0, 50, 0], np.int64)), "tp": arena.dev(np.array([1, 1, 0.9, 0.95, 1], np.float32)),
                   "mp": arena.dev(np.array([0, 0, 0, 0.02, 0.05], np.float32)), "u": arena.space(B * 4), "pos": arena.space(B * 8), "slots": arena.space(B * 4), "lens": arena.space(B * 4), "scored": arena.space(B * 4)}
         self.positions = np.array([5000, 47, 123456, 52, 300], np.int64)
@@ -632,7 +632,7 @@ class Step:
     def launch(self):
         d, w, s = self.d, self.dev, self.stream
         B, N, W, H, G, D, R = self.B, self.N, self.W, self.H, self.G, self.D, self.R
-        m = nvr.AttnMetaC(is_prefill=0, context_lens=d["lens"].ptr, block_tables=d["table"].ptr, max_blocks=self.table.shape[1], batch=B, max_context_len=128)
+        m = nvr.AttnMetaC(is_prefill=0, context_lens=d["lens"].ptr, block_tables=d["table"].ptr, max_blocks=self.table.shape[1], batch=B, max_context_len=self.bound)
         ws, q = self.w, d["qkv"].ptr
         nvr.check(L.nvr_linear(w["x"].ptr, W, w["wqkv"].ptr, B, W, N, q, 0, s))
         nvr.check(L.nvr_lora_add(w["x"].ptr, W, w["a1"].ptr, w["b1"].ptr, d["scales"].ptr, d["ids"].ptr, self.n, B, W, N, R, q, N, q, N, d["ws_lora"].ptr, s))
@@ -657,10 +657,10 @@ class Step:
             nvr.check(L.nvr_memcpy_h2d(self.d[name].ptr, a.ctypes.data, a.nbytes))
 
 
-@pytest.mark.parametrize("dtype", DTYPES)
-def test_a_step_of_all_of_them(arena, dtype):
+@pytest.mark.parametrize("dtype,bound", [("float16", 128), ("bfloat16", 128), ("float32", 128), ("float16", 2000), ("float32", 2000)])
+def test_a_step_of_all_of_them(arena, dtype, bound):
     """Three steps; each stage against its definition on what the stage in front of it left."""
-    st = Step(arena, dtype)
+    st = Step(arena, dtype, bound=bound)
     lengths = list(st.lengths)
     B, N, W, H, G, D = st.B, st.N, st.W, st.H, st.G, st.D
     cache_k, cache_v = st.k0.copy(), st.v0.copy()
@@ -733,12 +733,12 @@ def test_a_step_of_all_of_them(arena, dtype):
         st.positions = st.positions + 1
 
 
-@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
-def test_a_captured_step_replays(arena, dtype):
+@pytest.mark.parametrize("dtype,bound", [("bfloat16", 128), ("float32", 128), ("bfloat16", 2000), ("float16", 2000)])
+def test_a_captured_step_replays(arena, dtype, bound):
     """The step in a graph, replayed with other inputs and eager work between: the bits of the eager step each time."""
     stream = C.c_void_p()
     nvr.check(L.nvr_stream_create(byref(stream)))
-    st = Step(arena, dtype, stream)
+    st = Step(arena, dtype, stream, bound=bound)
     st.feed(st.lengths)
     st.launch()
     nvr.check(L.nvr_stream_synchronize(stream))
@@ -966,3 +966,28 @@ def test_copies_to_the_host_wait_for_every_stream(arena):
 @pytest.mark.parametrize("out_of_place", [False, True])
 def test_evict_without_a_bound_on_contexts(arena, out_of_place):
     evict_case(arena, "float16", [300, 40, 299], 2, 64, 16, 100, 4, 32, out_of_place, max_context=2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D,block", [(16, 1, 64, 16), (4, 2, 128, 256), (3, 1, 256, 7), (32, 8, 128, 64), (5, 5, 64, 1)])
+def test_scored_attention_of_short_contexts(arena, dtype, H, G, D, block):
+    """Contexts of up to 128 keys, which one launch answers: the same bits as where the bound on contexts asks for two."""
+    lengths = [0, 1, 128, 2, 15, 16, 17, 0, 31, 32, 33, 63, 64, 65, 100, 127, 128]
+    one = scored_case(arena, dtype, lengths, H, G, D, block, poison=True)
+    two = scored_case(arena, dtype, lengths, H, G, D, block, poison=True, max_context=257)
+    used = [i for i, n in enumerate(lengths) if n]
+    assert np.array_equal(one[0][used], two[0][used]) and np.array_equal(one[1].view(np.uint32), two[1].view(np.uint32))
+    scored_case(arena, dtype, [60, 128, 9], H, G, D, block, scored=[0, 999, -3], decay=0.25, in_place=True, q_gap=8)
+    if block < 128:
+        scored_case(arena, dtype, [128, 100, 5], H, G, D, block, bad=[(0, 0, -1), (0, 1, 1 << 30), (2, 0, -7)])
+    scored_case(arena, dtype, [100, 7], H, G, D, block, max_context=50)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D,B,longest", [(8, 4, 64, 70, 511), (8, 8, 128, 40, 512), (8, 4, 64, 70, 513), (4, 1, 128, 20, 400), (16, 1, 256, 9, 256)])
+def test_scored_attention_of_contexts_around_one_launch(arena, dtype, H, G, D, B, longest):
+    """Sequences enough for the chip and not, contexts on either side of what one launch takes."""
+    rng = np.random.default_rng(longest + B)
+    lengths = rng.integers(0, longest, B).tolist()
+    lengths[3], lengths[5] = longest, 0
+    scored_case(arena, dtype, lengths, H, G, D, 64, poison=True)
