@@ -925,9 +925,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
 }
 
-// Tokens of a chunk.  Each has its bins and lists, which the second launch reads: large ones once they fill the chip or there would be many.  us with 4096 and 16384: 256 rows of 151936 137 114; one row of
-// 151936 with top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 22 (the walk over the drawn chunk); one of 10^6: 28 19, 64 58, 52 54, 26 25; one of 32000: 14 15, 36 42, 15 20, 14 21
-static int sample_chunk(int64_t B, int64_t V) { return V > 131072 || B * ((V + 16383) / 16384) >= 256 ? 16384 : 4096; }
+// Tokens of a chunk.  Each has its bins and lists, which the second launch reads: large ones where there would be many, and for many rows that are one.  us with 4096 and 16384, settings mixed: 256 rows of
+// 151936 137 114, 40 74 66, 256 of 131072 114 101, 32 45 44, 8 38 41; 256 of 65536 73 73, 128 57 62, 256 of 32768 61 64, 198 of 20570 59 78; 135 of 9398 52 42, 256 of 5000 48 42.  One row of 151936 with
+// top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 22 (the walk over the drawn chunk); of 32000: 14 15, 36 42, 15 20, 14 21
+static int sample_chunk(int64_t B, int64_t V) { return V > 98304 || (V <= 16384 && B >= 128) ? 16384 : 4096; }
 size_t sample_uniform_workspace_bytes(int64_t B, int64_t V) {
     if (B <= 0 || V <= 0) return 0;
     const int64_t P = (V + sample_chunk(B, V) - 1) / sample_chunk(B, V);
