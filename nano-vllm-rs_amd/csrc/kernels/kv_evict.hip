@@ -1,7 +1,7 @@
 // kv_evict.hip — a sequence's cache brought down to `budget` keys a kv head: its first and last keys, and the best of the others by their scores (ties: the earlier key), close up in their order.
 //
 // First launch, a workgroup a (sequence, kv head): the score that the last of the kept keys has, by a radix select over the scores (held in LDS up to kHeld of them), then the kept keys in
-// order (each thread owns a run of keys; one scan tells where its kept ones go) and the scores at their new places.  Second launch: the rows of K and V.
+// order (each thread owns a run of keys; one scan tells where its kept ones go) and the scores at their new places.  Second launch: the rows of K and V (a few of them the first moves itself).
 // Into other blocks, every row is on its own: a copy, bound by memory.  In place, row i comes from row kept[i] >= i, which is overwritten by a later row: a workgroup takes a (sequence, kv head)'s
 // strip of 128 bytes of the rows, from the front in steps of kMoves requests: all of a step are read before any is written, and no later step reads what it writes.
 // 32 sequences of 1000 .. 8100 keys of 8 heads of 128 to 2048, float16, other blocks: 111 us (15 and 94), 4.4 TB/s over both, 5.2 in the copy (a large copy: 5.1); one of 4099 keys: 15 us (11 and 4).
@@ -16,7 +16,7 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kPick = 1024, kHeld = 32768, kRadix = 2048, kTable = 512;      // kHeld: scores in LDS, at most (128 of 160 KB)
+constexpr int kPick = 1024, kHeld = 32768, kRadix = 2048, kTable = 512, kHere = 4;       // kHere: rows that a thread moves 16 bytes of; kHeld: scores in LDS, at most (128 of 160 KB)
 struct EvictParams {
     EvictArgs a;
     int32_t *kept;                                                        // [B][KVH][budget]
@@ -48,6 +48,9 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 }
 }  // namespace
 
+// MOVE: the rows are few, and are moved here: all are read before any is written.  us so and with a second launch, rows of 256 bytes of 8 heads: one sequence to 64 keys 7.5 8.5 (in place 7.4 9.3), to 256
+// 9.7 9.2 (9.8 11.3); 16 to 128 9.8 11.2, to 256 12.8 13.2; 32 of 500 rows of 128 bytes 18.1 19.3 (15.3 17.6)
+template <bool MOVE>
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     extern __shared__ __attribute__((aligned(16))) float held[];          // scores of keys 0 .. p.held - 1
     __shared__ unsigned int hist[2 * kRadix + kRadix / 2];                // 11, 11 and 10 bits
@@ -149,12 +152,43 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
             const bool tie = !always && need && k == prefix;
             if (always || (need && k > prefix) || (tie && seen < want)) {
                 kept[at] = i;
+                if (MOVE) hist[at] = (unsigned int)i;                 // (the counts have been looked at)
                 if (ALL) a.scores[to_at((int)at)] = f;
                 ++at;
             }
             seen += tie;
         }
     };
+    if constexpr (MOVE) {                                                 // (no more keys than LDS holds)
+        choose(std::true_type());
+        __syncthreads();
+        const int lanes = p.row_bytes / 16, rows = kPick / lanes, lead = tid / lanes;
+        const int64_t row = (int64_t)a.KVH * p.row_bytes, off = (int64_t)g * p.row_bytes + tid % lanes * 16;
+        auto row_at = [&](const int32_t *t, const int32_t *lds, int j) {
+            const Slot q = slot_of(p, j);
+            return ((int64_t)(q.block < kTable ? lds[q.block] : t[q.block]) * a.block_size + q.row) * row + off;
+        };
+        float4_t k[kHere], v[kHere];
+#pragma unroll
+        for (int u = 0; u < kHere; ++u) {
+            const int i = u * rows + lead;
+            const int64_t at = lead < rows && i < n ? row_at(table, from_table, (int)hist[i]) : -1;
+            k[u] = v[u] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            if (at >= 0) { k[u] = *reinterpret_cast<const float4_t *>((const char *)a.k + at); v[u] = *reinterpret_cast<const float4_t *>((const char *)a.v + at); }
+        }
+#pragma unroll
+        for (int u = 0; u < kHere; ++u) asm volatile("" : "+v"(k[u]), "+v"(v[u]));      // (here: all of them have arrived)
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kHere; ++u) {
+            const int i = u * rows + lead;
+            if (lead >= rows || i >= n) continue;
+            const int64_t at = row_at(to, to_table, i);
+            *reinterpret_cast<float4_t *>((char *)a.k + at) = k[u];
+            *reinterpret_cast<float4_t *>((char *)a.v + at) = v[u];
+        }
+        return;
+    }
     if (together) return choose(std::true_type());
     choose(std::false_type());
     __threadfence_block();
@@ -245,11 +279,19 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
     const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
     p.held = (int32_t)std::min<int64_t>(((int64_t)a.max_ctx + 3) / 4 * 4, kHeld);
-    static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv_evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
-    if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "%s: LDS of %d bytes: %s", me, kHeld * 4, hipGetErrorString(opted));
-    kv_evict_select_kernel<<<dim3(G, B), kPick, (size_t)p.held * 4, s>>>(p);
+    const int64_t most = std::min(a.budget, a.max_ctx);
+    const bool move = a.max_ctx <= kHeld && most <= kHere * (kPick / (p.row_bytes / 16));
+    const auto kernel = move ? &kv_evict_select_kernel<true> : &kv_evict_select_kernel<false>;
+    auto opt_in = [](const void *k) { return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4); };
+    static const hipError_t opted[2] = {opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<false>)), opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<true>))};
+    if (opted[move] != hipSuccess) return nvr::fail(NVR_ERR_HIP, "%s: LDS of %d bytes: %s", me, kHeld * 4, hipGetErrorString(opted[move]));
+    kernel<<<dim3(G, B), kPick, (size_t)p.held * 4, s>>>(p);
+    if (move) {
+        NVR_KX_LAUNCHED("kv_evict");
+        return 0;
+    }
     if (a.to_tables) {
-        const int rows = 256 / (p.row_bytes / 16), most = std::min(a.budget, a.max_ctx);
+        const int rows = 256 / (p.row_bytes / 16);
         if (most > 0) kv_evict_copy_kernel<<<dim3((unsigned)((most + rows - 1) / rows), G, B), 256, 0, s>>>(p);
     } else if (a.max_ctx > a.budget) kv_evict_close_kernel<<<dim3((unsigned)(2 * (p.row_bytes / p.strip)), G, B), kPick, 0, s>>>(p);
     NVR_KX_LAUNCHED("kv_evict");

@@ -991,3 +991,12 @@ def test_scored_attention_of_contexts_around_one_launch(arena, dtype, H, G, D, B
     lengths = rng.integers(0, longest, B).tolist()
     lengths[3], lengths[5] = longest, 0
     scored_case(arena, dtype, lengths, H, G, D, 64, poison=True)
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+@pytest.mark.parametrize("dtype,lengths,G,D,block,budget,first,last", [("float16", [300, 64, 0, 65, 1000], 3, 128, 16, 64, 4, 20), ("float32", [300, 128, 129], 2, 256, 256, 64, 0, 0), ("float32", [300, 70], 2, 256, 256, 65, 0, 64),
+                                                                      ("bfloat16", [4000, 5000], 1, 8, 7, 4096, 4, 100), ("bfloat16", [5000, 20], 1, 8, 1, 4097, 4, 100), ("float16", [700, 3], 2, 40, 64, 256, 1, 1),
+                                                                      ("float16", [33000, 40], 1, 64, 256, 40, 4, 4), ("bfloat16", [1000, 257], 2, 128, 256, 257, 4, 4)])
+def test_evict_of_few_rows(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place):
+    """Rows on either side of what the first launch moves itself."""
+    evict_case(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place)
