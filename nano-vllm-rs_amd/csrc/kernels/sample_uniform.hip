@@ -760,11 +760,12 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     const bool by_key = stop < kBins && !(key == 0 && index == 0xffffffffu);
     const int key_bin = stop, sure = min(stop, p_sure + 1), last = min(min(by_key ? stop : stop - 1, p_last), kBins - 2);
     const bool cut = filtered && last >= sure;                            // (without filters all bins are whole)
-    auto kept = [&](int b, unsigned int kk, unsigned int i, double w) {
+    // enough(): whether weight() of the token is min_p and more
+    auto kept = [&](int b, unsigned int kk, unsigned int i, auto enough) {
         if (!filtered || b < sure) return true;
         if (b > last) return false;
         if (by_key && b == key_bin && (kk < key || (kk == key && i > index))) return false;
-        return !(ask.min_p > 0.f) || w >= (double)ask.min_p;
+        return !(ask.min_p > 0.f) || enough();
     };
     if (in_lds) {
         // ---- the token among up to kList in LDS (thread t has t and t + kPick): weights are whole numbers of 2^-52 (and 1 at least), summed by the upper 11 bits of the index and then by the others
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             const unsigned int kk = sh.key[at];
             const float v = of_key(kk);
             i[e] = sh.idx[at]; w[e] = weight(v, r.m, ask.c);
-            if (kept(bin_of(v, r.m, ask.inv), kk, i[e], w[e])) q[e] = max(1ull, (unsigned long long)(w[e] * 0x1p52 + 0.5));
+            if (kept(bin_of(v, r.m, ask.inv), kk, i[e], [&] { return w[e] >= (double)ask.min_p; })) q[e] = max(1ull, (unsigned long long)(w[e] * 0x1p52 + 0.5));
         }
         unsigned long long done = 0;
         double sum = 0., goal = 0.;
@@ -828,7 +829,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     if (cut)
         r.each_gathered(here, sure, last, [&](unsigned int kk, unsigned int i, float v, int b) {
             const double w = weight(v, r.m, ask.c);
-            if (kept(b, kk, i, w)) atomicAdd(&single[i / p.chunk], (unsigned long long)(w / unit + 0.5));
+            if (kept(b, kk, i, [&] { return w >= (double)ask.min_p; })) atomicAdd(&single[i / p.chunk], (unsigned long long)(w / unit + 0.5));
         });
     __syncthreads();
     double *units = reinterpret_cast<double *>(sh.key);                   // (kList of 4 bytes: the gathered tokens have been looked at)
@@ -879,23 +880,37 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     const int per = p.chunk / kPick, base = c * p.chunk + tid * per, end = min(p.V, c * p.chunk + p.chunk);      // 4 or 16
     const bool lone = lonely(r.m, ask.inv);
     const double t_m = (double)r.m * ask.inv, whole_m = t_m + kWhole;
-    auto of = [&](float v, int i) {                                       // the weight as the cell's times the place's inside: half the work of an exponential
+    auto of = [&](float v, int i, auto enough) {                          // the weight as the cell's times the place's inside: half the work of an exponential
         if (v == -INFINITY || (lone && v != r.m)) return 0.;
         const double at = fmax((double)v * ask.inv, t_m - 2. * kBins), whole = at + kWhole;
         const int b = lone ? 0 : low_of(whole_m) - low_of(whole);
         if (b >= kBins - 1 || (filtered && b >= sure && b > last)) return 0.;
         const double w = lone ? 1. : (above_2_52(at - (whole - kWhole)) - 4503599627370496.0) * units[b];
-        return kept(b, key_of(v), (unsigned int)i, w) ? w : 0.;
+        return kept(b, key_of(v), (unsigned int)i, [&] { return enough(w, v); }) ? w : 0.;
     };
+    // That weight and weight() are within 1e-7 of each other (5e-13 of the steps inside a cell, and 2^-53 of 24 x / T, which is below 2^34 where tokens of different logits are near).  Where min_p is as close,
+    // weight() decides, as it did for the sums (it is exactly 1 for the largest logit, and the other may be below); once behind the loop: in it, 256 rows of 151936 with min-p 0.001 took 189 us in place of 186
+    auto exactly = [&](double, float v) { return weight(v, r.m, ask.c) >= (double)ask.min_p; };
     float4_t f[4];
     double here_sum = 0.;
+    unsigned int doubt = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = four(r.x, base + 4 * j, 4 * j < per ? end : 0, p.whole);
 #pragma unroll 1
     for (int j = 0; 4 * j < per; ++j) {                                   // (not unrolled: code that runs once costs its way from memory)
         const float4_t g = j & 2 ? j & 1 ? f[3] : f[2] : j & 1 ? f[1] : f[0];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) here_sum += of(g[e], base + 4 * j + e);
+        for (int e = 0; e < 4; ++e)
+            here_sum += of(g[e], base + 4 * j + e, [&](double w, float) {
+                const bool near = fabs(w - (double)ask.min_p) <= 1e-6 * w;
+                doubt |= (near ? 1u : 0u) << (4 * j + e);
+                return !near && w >= (double)ask.min_p;
+            });
+    }
+    while (doubt) {
+        const int i = base + __ffs((int)doubt) - 1;
+        doubt &= doubt - 1;
+        here_sum += of(seen(r.x[i]), i, exactly);
     }
     const double upto = scan<double>(here_sum, sh.wsum);
     int t = first_of(here_sum > 0. && sh.part + upto > goal);
@@ -912,7 +927,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
     __syncthreads();
     if (wave == 0 && t >= 0) {
-        const double w = lane < per ? of(values[lane & 15], c * p.chunk + t * per + lane) : 0., run = sh.cum[0] + wave_scan(w);
+        const double w = lane < per ? of(values[lane & 15], c * p.chunk + t * per + lane, exactly) : 0., run = sh.cum[0] + wave_scan(w);
         const unsigned long long any = __ballot(w > 0.), hit = __ballot(w > 0. && run > goal);
         const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)any);      // (sums in another order may end a rounding below the goal: the last one)
         if (lane == 0) sh.found = c * p.chunk + t * per + l;

@@ -1000,3 +1000,13 @@ def test_scored_attention_of_contexts_around_one_launch(arena, dtype, H, G, D, B
 def test_evict_of_few_rows(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place):
     """Rows on either side of what the first launch moves itself."""
     evict_case(arena, dtype, lengths, G, D, block, budget, first, last, out_of_place)
+
+
+@pytest.mark.parametrize("V", [2049, 20000, 151936])
+@pytest.mark.parametrize("T", [0.7, 1.3, 100.0])
+def test_sample_min_p_of_one_keeps_the_largest(arena, V, T):
+    """The largest logits weigh exactly 1, wherever they lie in their cell: rows with more of them than a chunk's list holds, and rows so flat that every token is near the largest."""
+    rng = np.random.default_rng(V)
+    x = np.stack([np.full(V, 2.3), np.full(V, 5.1), np.full(V, -0.9), rng.standard_normal(V), np.where(rng.random(V) < 0.5, 5.1, 5.0)])
+    for k, p, m in ((0, 1.0, 1.0), (0, 1.0, 5.0), (0, 0.7, 1.0), (V // 2, 1.0, 1.0), (V - 1, 0.9, 1.0)):
+        check_sample(arena, x, T, k, p, m, rng.random(5).astype(np.float32))
