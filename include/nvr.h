@@ -673,7 +673,7 @@ NVR_API int nvr_fill_const(nvr_half *dst, int64_t n, float value, void *stream);
 /* Rotary positions, low-rank adapters, tokens from given numbers, and a cache that forgets.  Pointers and types as above: nvr_ops_set_dtype names the type of the nvr_half
  * tensors, all three included; scores, logits, scales and probabilities are f32.  Argument errors are found before anything is enqueued; what lies on the device (slots,
  * adapter ids, block tables, lengths) is kept in bounds by the kernels as said below.  A workspace belongs to one call at a time (calls on one stream, or replays of one
- * graph, may share it), is aligned to 16 bytes, and holds nothing between calls. */
+ * graph, may share it), is aligned to 16 bytes, and holds nothing between calls; one for a larger step (more rows, columns, keys, a larger budget; the same heads) serves smaller ones. */
 
 /* How positions are stretched.  NVR_ROPE_PLAIN: freq_j = theta^(-2j/rotary_dim), j < rotary_dim / 2.  LINEAR: freq_j / factor.  NTK: theta * factor^(rotary_dim / (rotary_dim - 2))
  * in theta's place.  YARN: freq_j (1 - r_j) + freq_j / factor * r_j with r_j rising linearly from the pair that turns `high` times within original_len positions (rounded down) to the one

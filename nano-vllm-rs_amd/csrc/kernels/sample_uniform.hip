@@ -943,11 +943,15 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 // Tokens of a chunk.  Each has its bins and lists, which the second launch reads: large ones where there would be many, and for many rows that are one.  us with 4096 and 16384, settings mixed: 256 rows of
 // 151936 137 114, 40 74 66, 256 of 131072 114 101, 32 45 44, 8 38 41; 256 of 65536 73 73, 128 57 62, 256 of 32768 61 64, 198 of 20570 59 78; 135 of 9398 52 42, 256 of 5000 48 42.  One row of 151936 with
 // top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 22 (the walk over the drawn chunk); of 32000: 14 15, 36 42, 15 20, 14 21
+// (the limits stand in sample_uniform_workspace_bytes too)
 static int sample_chunk(int64_t B, int64_t V) { return V > 98304 || (V <= 16384 && B >= 128) ? 16384 : 4096; }
+// Enough for fewer rows and smaller vocabularies too, whose chunks may be smaller and more: the most there are on either side of the rule's limits
 size_t sample_uniform_workspace_bytes(int64_t B, int64_t V) {
     if (B <= 0 || V <= 0) return 0;
-    const int64_t P = (V + sample_chunk(B, V) - 1) / sample_chunk(B, V);
-    return (size_t)(B * P) * (kBins * 12 + kNear * 8 + sizeof(ChunkNote));
+    int64_t most = 0;
+    for (int64_t b : {B, std::min<int64_t>(B, 127)})
+        for (int64_t v : {V, std::min<int64_t>(V, 98304), std::min<int64_t>(V, 16384)}) most = std::max(most, b * ((v + sample_chunk(b, v) - 1) / sample_chunk(b, v)));
+    return (size_t)most * (kBins * 12 + kNear * 8 + sizeof(ChunkNote));
 }
 int sample_uniform(const SampleArgs &a, hipStream_t s) {
     if (a.B < 0 || a.V <= 0 || a.ld < a.V) return nvr::fail(NVR_ERR_INVALID_ARG, "nvr_sample_uniform: B=%ld V=%ld, rows %ld apart", (long)a.B, (long)a.V, (long)a.ld);

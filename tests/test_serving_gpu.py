@@ -1010,3 +1010,18 @@ def test_sample_min_p_of_one_keeps_the_largest(arena, V, T):
     x = np.stack([np.full(V, 2.3), np.full(V, 5.1), np.full(V, -0.9), rng.standard_normal(V), np.where(rng.random(V) < 0.5, 5.1, 5.0)])
     for k, p, m in ((0, 1.0, 1.0), (0, 1.0, 5.0), (0, 0.7, 1.0), (V // 2, 1.0, 1.0), (V - 1, 0.9, 1.0)):
         check_sample(arena, x, T, k, p, m, rng.random(5).astype(np.float32))
+
+
+@pytest.mark.parametrize("most,B,V", [((256, 10000), 127, 10000), ((256, 16384), 100, 16384), ((200, 20000), 100, 9000), ((4, 151936), 4, 98304)])
+def test_sample_in_the_workspace_of_a_larger_step(arena, most, B, V):
+    """A step of fewer rows, or of a smaller vocabulary, in the space that the largest asked for: nothing behind it is written."""
+    rng = np.random.default_rng(B + V)
+    x = (rng.standard_normal((B, V)) * 2).astype(np.float32)
+    u = rng.random(B).astype(np.float32)
+    size, guard = L.nvr_sample_uniform_workspace_bytes(*most), 1 << 16
+    assert size >= L.nvr_sample_uniform_workspace_bytes(B, V)
+    ws, ids = arena.space(size + guard), arena.space(B * 8)
+    T, k, p, m = (np.resize(np.array(a, t), B) for a, t in (([0.8, 1.0], np.float32), ([0, 50, 0], np.int64), ([0.9, 1.0], np.float32), ([0.0, 0.02, 0.0], np.float32)))
+    nvr.check(L.nvr_sample_uniform(arena.dev(x).ptr, V, B, V, *(arena.dev(a).ptr for a in (T, k, p, m, u)), ids.ptr, None, ws.ptr, None))
+    assert ids.to_numpy((B,), np.int64).tolist() == [sample(x[r], float(T[r]), int(k[r]), float(p[r]), float(m[r]), float(u[r]))[0] for r in range(B)]
+    assert (ws.to_numpy((size + guard,), np.uint8)[size:] == SENTINEL).all()

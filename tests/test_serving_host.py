@@ -166,3 +166,25 @@ def test_definitions_agree_with_hand_computed_cases():
     turns = np.array([0.25, 0.0])
     assert np.allclose(su.rope(x, np.array([1]), turns, 1.0, False)[0, 0], [-2, 1, 0, 3, 4, 5, 6, 7])
     assert np.allclose(su.rope(x, np.array([1]), turns, 1.0, True)[0, 0], [-1, 0, 2, 3, 4, 5, 6, 7])
+
+
+def test_workspaces_of_larger_steps_serve_smaller_ones():
+    """A program allocates once, for its largest step: no size falls where rows, columns, keys or a budget grow, also where a rule on sizes changes what the kernels do."""
+    l = nvr.lib()
+    rows = [1, 2, 63, 64, 65, 126, 127, 128, 129, 255, 256, 257, 512, 1000, 1024, 1025, 4000, 65535]
+    logits = [1, 33, 4095, 4096, 4097, 5000, 10000, 16383, 16384, 16385, 20570, 65536, 98303, 98304, 98305, 114688, 114689, 151936, 400000, (1 << 22) - 1, 1 << 22]
+    keys = [1, 127, 128, 129, 255, 256, 257, 511, 512, 513, 4096, 8100, 65536, 1 << 20, 1 << 23]
+    wide = [8, 511, 512, 1023, 1024, 1535, 1536, 2047, 2048, 4096, 1 << 16, 1 << 22]
+    grids = {"nvr_sample_uniform_workspace_bytes": [(rows, logits)],
+             "nvr_lora_workspace_bytes": [(rows + [1 << 17, 1 << 19], wide, [n], [1, 15, 16, 17, 64, 96, 97, 128, 129, 256]) for n in (8, 4096)],
+             "nvr_paged_attn_scored_workspace_bytes": [(rows, [h], [g], [d], keys) for h, g in ((1, 1), (32, 8), (16, 1), (64, 64)) for d in (64, 128, 256)],
+             "nvr_kv_evict_workspace_bytes": [(rows, [1, 8], [1, 16, 2048, 1 << 20], keys)]}
+    for name, all_axes in grids.items():
+        for axes in all_axes:
+            size = np.zeros([len(a) for a in axes], np.float64)
+            for at in np.ndindex(*size.shape):
+                size[at] = getattr(l, name)(*(int(a[i]) for a, i in zip(axes, at)))
+            assert (size > 0).all()
+            for d in range(size.ndim):
+                fell = np.argwhere(np.diff(size, axis=d) < 0)
+                assert len(fell) == 0, (name, "argument", d, [a[i] for a, i in zip(axes, fell[0])])
