@@ -153,7 +153,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(Scor
             const bool in = j < last && page >= 0 && page < p.a.num_blocks;
             const int r = in ? page * p.a.block_size + (int)((unsigned)j % (unsigned)p.a.block_size) : -1;
             mask = (unsigned int)__ballot(in && lane < I::TK);
-            return in ? r : mask ? __shfl(r, __ffs(mask) - 1) : -1;
+            const int other = mask ? __builtin_amdgcn_readlane(r, __ffs(mask) - 1) : -1;      // (in front of the choice: an exchange among the lanes that choose it would ask a lane that is not there)
+            return in ? r : other;
         };
         V kx[I::NI], vx[I::NI];
         auto request = [&](int rows) {
