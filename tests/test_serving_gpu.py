@@ -1025,3 +1025,23 @@ def test_sample_in_the_workspace_of_a_larger_step(arena, most, B, V):
     nvr.check(L.nvr_sample_uniform(arena.dev(x).ptr, V, B, V, *(arena.dev(a).ptr for a in (T, k, p, m, u)), ids.ptr, None, ws.ptr, None))
     assert ids.to_numpy((B,), np.int64).tolist() == [sample(x[r], float(T[r]), int(k[r]), float(p[r]), float(m[r]), float(u[r]))[0] for r in range(B)]
     assert (ws.to_numpy((size + guard,), np.uint8)[size:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scored_attention_pages_outside_the_pool_in_two_launches(arena, dtype):
+    """As above with a bound of more than 512 keys, where a second launch turns scores into weights: pages missing at a tile's begin and end, a whole tile, whole units, all of a sequence, the newest key's."""
+    lengths = [600, 600, 600, 140, 20, 600]
+    bad = [(0, 0, -1), (0, 2, -1), (0, 3, 1 << 20), (0, 37, -1)] + [(1, i, -7) for i in range(8, 24)] + [(2, i, -1) for i in range(2, 38)] + [(3, i, 1 << 30) for i in range(9)] + [(4, 1, -1)]
+    for in_place in (False, True):
+        scored_case(arena, dtype, lengths, 4, 2, 64, 16, bad=bad, in_place=in_place, poison=True)
+    scored_case(arena, dtype, [600, 1300], 8, 1, 128, 64, bad=[(0, 9, -1), (1, 0, -1), (1, 3, 1 << 30), (1, 20, -1)], poison=True)
+    scored_case(arena, dtype, [600, 530], 4, 2, 64, 7, bad=[(0, i, -1) for i in range(0, 86, 3)] + [(1, 75, -1), (1, 40, -2)], poison=True)      # (keys of a request of four in different pages)
+    rng = np.random.default_rng(6)
+    lengths = rng.integers(1, 700, 80).tolist()                    # more than 64 sequences: the shares are counted another way
+    scored_case(arena, dtype, lengths, 4, 2, 64, 64, bad=[(b, int(rng.integers(0, -(-n // 64))), -1) for b, n in enumerate(lengths) if b % 3 == 0])
+
+
+def test_scored_attention_cuts_contexts_at_their_bound_in_two_launches(arena):
+    scored_case(arena, "float16", [50, 2000, 700, 701], 4, 2, 64, 16, max_context=701, scored=[49, 1999, 699, 700])
+    scored_case(arena, "float32", [2000, 3, 5000], 4, 2, 64, 16, max_context=1025)
+    scored_case(arena, "bfloat16", [900, 40], 4, 2, 64, 16, max_context=1 << 16)
