@@ -451,7 +451,8 @@ int paged_attn_scored(int dt, const ScoredArgs &a, hipStream_t s) {
     if (a.H / a.KVH > 16) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: %d query heads a kv head (up to 16)", me, a.H / a.KVH);
     if (a.num_blocks * a.block_size > 0x7fffffffll || a.B > 65535 || a.KVH > 65535 || a.max_ctx > (1 << 23)) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: a pool of 2^31 rows and more, more than 65535 sequences, or contexts beyond 2^23", me);
     if (a.B == 0) return 0;
-    if (!a.q || !a.k || !a.v || !a.ctx_lens || !a.block_tables || !a.scores || !a.new_scores || !a.out || !a.workspace) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: null argument", me);
+    if (!a.q || !a.k || !a.v || !a.ctx_lens || !a.block_tables || !a.scores || !a.new_scores || !a.out || (a.max_ctx && !a.workspace))      // (without keys one launch answers, and has no use for it)
+        return nvr::fail(NVR_ERR_INVALID_ARG, "%s: null argument", me);
     if (a.ldq < (int64_t)a.H * a.D) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: rows of q overlap", me);
     if ((((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.workspace) & 15) != 0) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: caches and workspace have to be aligned to 16 bytes", me);
     ScoredParams p{};

@@ -1045,3 +1045,17 @@ def test_scored_attention_cuts_contexts_at_their_bound_in_two_launches(arena):
     scored_case(arena, "float16", [50, 2000, 700, 701], 4, 2, 64, 16, max_context=701, scored=[49, 1999, 699, 700])
     scored_case(arena, "float32", [2000, 3, 5000], 4, 2, 64, 16, max_context=1025)
     scored_case(arena, "bfloat16", [900, 40], 4, 2, 64, 16, max_context=1 << 16)
+
+
+def test_scored_attention_where_no_sequence_can_have_keys(arena):
+    """A bound of 0 keys: outputs of 0, scores as they were, and no workspace (its size is 0)."""
+    for dtype in DTYPES:
+        typed(dtype)
+        w = np.dtype(kind(dtype)).itemsize
+        B, H, G, D, block = 3, 4, 2, 64, 16
+        assert L.nvr_paged_attn_scored_workspace_bytes(B, H, G, D, 0) == 0
+        m = meta(arena, [5, 0, 300], np.zeros((B, 4), np.int32), 0)
+        q, kv, out = arena.space(B * H * D * w, 0), arena.space(block * G * D * w, 0), arena.space(B * H * D * w)
+        old, new = arena.space(G * block * 4, 0), arena.space(G * block * 4)
+        nvr.check(L.nvr_paged_attn_decode_scored(q.ptr, H * D, kv.ptr, kv.ptr, byref(m), H, G, D, block, 1, 0.125, old.ptr, None, 0.5, new.ptr, out.ptr, None, None))
+        assert (out.to_numpy((B * H * D * w,), np.uint8) == 0).all() and (new.to_numpy((G * block * 4,), np.uint8) == SENTINEL).all()
