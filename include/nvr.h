@@ -728,7 +728,7 @@ NVR_API int nvr_paged_attn_decode_scored(const nvr_half *q, int64_t ldq, const n
  * sequences' own (prompt blocks that other sequences share are left alone that way; shorter sequences are copied as they are).  In place, a block is one sequence's alone.
  * new_lens [B] (not meta's context_lens) gets the lengths; kept [B, KVH, budget] (nullable) the kept keys' former places, -1 behind the last.  Blocks behind the new length are the caller's to free.
  * A sequence whose tables name a block outside 0 .. num_blocks - 1 for one of its keys, or whose to_tables row has too few blocks, stays as it is: new_lens -1, kept all -1.
- * keep_first + keep_last <= budget; rows of a multiple of 16 bytes.  workspace: nvr_kv_evict_workspace_bytes (null allowed where kept is given). */
+ * keep_first + keep_last <= budget; rows of a multiple of 16 bytes; max_context_len or max_blocks * block_size up to 2^25 keys.  workspace: nvr_kv_evict_workspace_bytes (null allowed where kept is given). */
 NVR_API size_t nvr_kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_context_len);
 NVR_API int nvr_kv_evict(nvr_half *k_cache, nvr_half *v_cache, float *scores, const nvr_attn_meta *meta, int64_t KVH, int64_t D, int64_t block_size, int64_t num_blocks,
                          int64_t budget, int64_t keep_first, int64_t keep_last, const int32_t *to_tables, int64_t to_max_blocks, int32_t *new_lens, int32_t *kept,

@@ -16,7 +16,7 @@
 namespace nvr { namespace kx {
 
 namespace {
-constexpr int kPick = 1024, kHeld = 32768, kRadix = 2048, kTable = 512, kHere = 4;       // kHere: rows that a thread moves 16 bytes of; kHeld: scores in LDS, at most (128 of 160 KB)
+constexpr int kPick = 1024, kHeld = 32768, kRadix = 2048, kTable = 512, kHere = 4, kLongest = 1 << 25;       // kHere: rows that a thread moves 16 bytes of; kHeld: scores in LDS, at most (128 of 160 KB)
 struct EvictParams {
     EvictArgs a;
     int32_t *kept;                                                        // [B][KVH][budget]
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     // a sequence whose tables name a block outside the pool, or too few, stays as it is
     int bad = a.to_tables && (long long)a.to_max_blocks * a.block_size < n;
     auto look = [&](const int32_t *t, int32_t *lds, int keys) {
-        for (int i = tid; i < (keys + a.block_size - 1) / a.block_size; i += kPick) {
+        for (int i = tid, n = keys > 0 ? slot_of(p, keys - 1).block + 1 : 0; i < n; i += kPick) {
             const int block = t[i];
             bad |= block < 0 || block >= a.num_blocks;
             if (i < kTable) lds[i] = block;
@@ -77,11 +77,11 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     for (int i = tid; i < 2 * kRadix + kRadix / 2; i += kPick) hist[i] = 0;
     if (__syncthreads_or(bad)) {
         if (g == 0 && tid == 0) a.new_lens[b] = -1;
-        for (int i = tid; i < a.budget; i += kPick) kept[i] = -1;
+        for (unsigned int i = tid; i < (unsigned int)a.budget; i += kPick) kept[i] = -1;
         return;
     }
     if (g == 0 && tid == 0) a.new_lens[b] = n;
-    for (int i = n + tid; i < a.budget; i += kPick) kept[i] = -1;
+    for (unsigned int i = n + tid; i < (unsigned int)a.budget; i += kPick) kept[i] = -1;      // (a budget may be any)
     const bool all = len <= a.budget;
     if (all && !a.to_tables) {                                            // (nothing moves)
         for (int i = tid; i < n; i += kPick) kept[i] = i;
@@ -266,6 +266,9 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     const int64_t bytes = (int64_t)a.D * (dt == DT_F32 ? 4 : 2);
     if (bytes % 16 || bytes > 1024) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: rows of %ld bytes a head (multiples of 16 up to 1024)", me, (long)bytes);
     if (a.num_blocks * a.block_size > 0x7fffffffll || a.B > 65535 || a.KVH > 65535) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: a pool of 2^31 rows and more, or more than 65535 sequences", me);
+    // (sums of 32 bits over a sequence's keys, and the threads of the copy, stay below 2^32)
+    const int64_t longest = std::min<int64_t>(a.max_ctx, (int64_t)a.max_blocks * a.block_size);
+    if (longest > kLongest) return nvr::fail(NVR_ERR_UNSUPPORTED, "%s: contexts of %ld keys (the bound and the tables together allow up to %d)", me, (long)longest, kLongest);
     if (a.B == 0) return 0;
     if (!a.k || !a.v || !a.scores || !a.ctx_lens || !a.block_tables || !a.new_lens || (!a.kept && !a.workspace)) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: null argument", me);
     if (a.new_lens == a.ctx_lens) return nvr::fail(NVR_ERR_INVALID_ARG, "%s: new_lens is the context_lens that other workgroups still read", me);
@@ -278,9 +281,9 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     p.per_block = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / (uint64_t)a.block_size);
     p.strip = bytes % 128 == 0 ? 128 : (int32_t)bytes;
     const unsigned G = (unsigned)a.KVH, B = (unsigned)a.B;
-    p.held = (int32_t)std::min<int64_t>(((int64_t)a.max_ctx + 3) / 4 * 4, kHeld);
-    const int64_t most = std::min(a.budget, a.max_ctx);
-    const bool move = a.max_ctx <= kHeld && most <= kHere * (kPick / (p.row_bytes / 16));
+    p.held = (int32_t)std::min<int64_t>((longest + 3) / 4 * 4, kHeld);
+    const int64_t most = std::min<int64_t>(a.budget, longest);
+    const bool move = longest <= kHeld && most <= kHere * (kPick / (p.row_bytes / 16));
     const auto kernel = move ? &kv_evict_select_kernel<true> : &kv_evict_select_kernel<false>;
     auto opt_in = [](const void *k) { return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4); };
     static const hipError_t opted[2] = {opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<false>)), opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<true>))};
@@ -293,7 +296,7 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     if (a.to_tables) {
         const int rows = 256 / (p.row_bytes / 16);
         if (most > 0) kv_evict_copy_kernel<<<dim3((unsigned)((most + rows - 1) / rows), G, B), 256, 0, s>>>(p);
-    } else if (a.max_ctx > a.budget) kv_evict_close_kernel<<<dim3((unsigned)(2 * (p.row_bytes / p.strip)), G, B), kPick, 0, s>>>(p);
+    } else if (longest > a.budget) kv_evict_close_kernel<<<dim3((unsigned)(2 * (p.row_bytes / p.strip)), G, B), kPick, 0, s>>>(p);
     NVR_KX_LAUNCHED("kv_evict");
     return 0;
 }

@@ -188,3 +188,10 @@ def test_workspaces_of_larger_steps_serve_smaller_ones():
             for d in range(size.ndim):
                 fell = np.argwhere(np.diff(size, axis=d) < 0)
                 assert len(fell) == 0, (name, "argument", d, [a[i] for a, i in zip(axes, fell[0])])
+
+
+@pytest.mark.parametrize("kw,bs,name", [(dict(max_context_len=(1 << 25) + 1, max_blocks=1 << 22), 16, "NVR_ERR_UNSUPPORTED"), (dict(max_context_len=2 ** 31 - 1, max_blocks=2 ** 31 - 1), 1, "NVR_ERR_UNSUPPORTED"),
+                                        (dict(max_context_len=2 ** 31 - 1, max_blocks=(1 << 23) + 1), 256, "NVR_ERR_UNSUPPORTED"), (dict(max_context_len=2 ** 31 - 1, max_blocks=3), 1 << 24, "NVR_ERR_UNSUPPORTED")])
+def test_evict_refuses_contexts_that_no_launch_holds(kw, bs, name):
+    """Tables and bound together allow more than 2^25 keys: sums of 32 bits over a sequence's blocks, and the grid of the copy, would pass their ends."""
+    refused("nvr_kv_evict", name, *{**EVICT, "nb": 8, "bs": bs, "meta": C.byref(_meta(**kw))}.values())
