@@ -466,6 +466,7 @@ NVR_API int nvr_device_name(char *buf, size_t cap);
 NVR_API int nvr_device_mem_info(uint64_t *free_bytes, uint64_t *total_bytes);
 NVR_API int nvr_device_malloc(void **ptr, size_t bytes);
 NVR_API int nvr_device_free(void *ptr);
+/* Both are over when they return, and wait for no stream of nvr_stream_create or a runner: what one still reads or writes there is the caller's to wait for */
 NVR_API int nvr_device_memset(void *ptr, int value, size_t bytes);
 NVR_API int nvr_memcpy_h2d(void *dst_dev, const void *src_host, size_t bytes);
 NVR_API int nvr_memcpy_d2h(void *dst_host, const void *src_dev, size_t bytes);   /* waits for all of the device's streams first */

@@ -518,7 +518,8 @@ int nvr_device_name(char *buf, size_t cap) {
 int nvr_device_mem_info(uint64_t *f, uint64_t *t) { size_t a = 0, b = 0; NVR_HIP_CHECK(hipMemGetInfo(&a, &b)); *f = a; *t = b; return NVR_OK; }
 int nvr_device_malloc(void **p, size_t bytes) { NVR_HIP_CHECK(hipMalloc(p, bytes ? bytes : 16)); return NVR_OK; }
 int nvr_device_free(void *p) { NVR_HIP_CHECK(hipFree(p)); return NVR_OK; }
-int nvr_device_memset(void *p, int v, size_t bytes) { NVR_HIP_CHECK(hipMemset(p, v, bytes)); return NVR_OK; }
+// (a fill may still run when hipMemset returns, on a stream that the library's do not wait for)
+int nvr_device_memset(void *p, int v, size_t bytes) { NVR_HIP_CHECK(hipMemset(p, v, bytes)); NVR_HIP_CHECK(hipStreamSynchronize(nullptr)); return NVR_OK; }
 int nvr_memcpy_h2d(void *d, const void *s, size_t b) { NVR_HIP_CHECK(hipMemcpy(d, s, b, hipMemcpyHostToDevice)); return NVR_OK; }
 // (streams of the library do not wait for the default one, nor it for them: what they still write would be missed)
 int nvr_memcpy_d2h(void *d, const void *s, size_t b) { NVR_HIP_CHECK(hipDeviceSynchronize()); NVR_HIP_CHECK(hipMemcpy(d, s, b, hipMemcpyDeviceToHost)); return NVR_OK; }
