@@ -469,7 +469,7 @@ NVR_API int nvr_device_free(void *ptr);
 /* Both are over when they return, and wait for no stream of nvr_stream_create or a runner: what one still reads or writes there is the caller's to wait for */
 NVR_API int nvr_device_memset(void *ptr, int value, size_t bytes);
 NVR_API int nvr_memcpy_h2d(void *dst_dev, const void *src_host, size_t bytes);
-NVR_API int nvr_memcpy_d2h(void *dst_host, const void *src_dev, size_t bytes);   /* waits for all of the device's streams first */
+NVR_API int nvr_memcpy_d2h(void *dst_host, const void *src_dev, size_t bytes);   /* waits for all streams of src_dev's device first, so a kernel there must not wait for a launch that this thread has yet to make */
 NVR_API int nvr_device_synchronize(void);
 NVR_API int nvr_stream_create(void **stream);
 NVR_API int nvr_stream_destroy(void *stream);

@@ -521,8 +521,21 @@ int nvr_device_free(void *p) { NVR_HIP_CHECK(hipFree(p)); return NVR_OK; }
 // (a fill may still run when hipMemset returns, on a stream that the library's do not wait for)
 int nvr_device_memset(void *p, int v, size_t bytes) { NVR_HIP_CHECK(hipMemset(p, v, bytes)); NVR_HIP_CHECK(hipStreamSynchronize(nullptr)); return NVR_OK; }
 int nvr_memcpy_h2d(void *d, const void *s, size_t b) { NVR_HIP_CHECK(hipMemcpy(d, s, b, hipMemcpyHostToDevice)); return NVR_OK; }
-// (streams of the library do not wait for the default one, nor it for them: what they still write would be missed)
-int nvr_memcpy_d2h(void *d, const void *s, size_t b) { NVR_HIP_CHECK(hipDeviceSynchronize()); NVR_HIP_CHECK(hipMemcpy(d, s, b, hipMemcpyDeviceToHost)); return NVR_OK; }
+// Streams of the library do not wait for the default one, nor it for them: what they still write would be missed.  It is the device of src_dev that is waited for, which need not be the current one
+int nvr_memcpy_d2h(void *d, const void *s, size_t b) {
+    int now = 0;
+    NVR_HIP_CHECK(hipGetDevice(&now));
+    hipPointerAttribute_t at{};
+    int of = now;
+    if (hipPointerGetAttributes(&at, s) != hipSuccess) (void)hipGetLastError();      // (not the runtime's memory: the copy says so)
+    else if (at.type == hipMemoryTypeDevice) of = at.device;
+    if (of != now) NVR_HIP_CHECK(hipSetDevice(of));
+    const hipError_t waited = hipDeviceSynchronize();
+    if (of != now) NVR_HIP_CHECK(hipSetDevice(now));
+    NVR_HIP_CHECK(waited);
+    NVR_HIP_CHECK(hipMemcpy(d, s, b, hipMemcpyDeviceToHost));
+    return NVR_OK;
+}
 int nvr_device_synchronize(void) { NVR_HIP_CHECK(hipDeviceSynchronize()); return NVR_OK; }
 int nvr_stream_create(void **s) { hipStream_t st; NVR_HIP_CHECK(hipStreamCreateWithFlags(&st, hipStreamNonBlocking)); *s = st; return NVR_OK; }
 int nvr_stream_destroy(void *s) { NVR_HIP_CHECK(hipStreamDestroy((hipStream_t)s)); return NVR_OK; }

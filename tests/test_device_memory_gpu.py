@@ -27,3 +27,18 @@ def test_fills_are_over_when_the_call_returns():
         nvr.check(L.nvr_stream_synchronize(stream))
         assert (out.to_numpy((rows * cols * 2,), np.uint8) == byte).all()
     nvr.check(L.nvr_stream_destroy(stream))
+
+
+def test_copies_to_the_host_from_inside_an_allocation_and_of_nothing():
+    """Pointers into the middle of an allocation are the device's; a copy of nothing from no pointer is nothing, and leaves no error to the launches behind it."""
+    L = nvr.lib()
+    nvr.check(L.nvr_device_set(0))
+    a = np.arange(100000, dtype=np.int32)
+    b = nvr.DeviceBuffer.from_numpy(a)
+    got = np.zeros(17, np.int32)
+    nvr.check(L.nvr_memcpy_d2h(got.ctypes.data, b.ptr + 4 * 70001, got.nbytes))
+    assert np.array_equal(got, a[70001:70018])
+    nvr.check(L.nvr_memcpy_d2h(got.ctypes.data, None, 0))
+    nvr.check(L.nvr_ops_set_dtype(b"float16"))
+    nvr.check(L.nvr_fill_const(b.ptr, 64, 0.0, None))
+    assert (b.to_numpy((32,), np.int32) == 0).all()
