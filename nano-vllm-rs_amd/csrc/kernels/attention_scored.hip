@@ -429,8 +429,8 @@ int scored_launch(const ScoredParams &p, hipStream_t s) {
     constexpr size_t most = WHOLE ? kLds : I::ALL;
     const size_t lds = I::ALL + (WHOLE ? (size_t)(p.a.H / p.a.KVH) * p.wide * 4 : 0);
     if constexpr (most > 48 * 1024) {
-        static const hipError_t opted = hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_scored_kernel<E, D, WHOLE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
-        if (opted != hipSuccess) return nvr::fail(NVR_ERR_HIP, "nvr_paged_attn_decode_scored: LDS of %zu bytes: %s", most, hipGetErrorString(opted));
+        static std::atomic<uint64_t> allowed{0};
+        if (const int rc = allow_lds("nvr_paged_attn_decode_scored", reinterpret_cast<const void *>(&attn_scored_kernel<E, D, WHOLE>), most, allowed)) return rc;
     }
     attn_scored_kernel<E, D, WHOLE><<<dim3((unsigned)p.a.KVH, (unsigned)(WHOLE ? p.a.B : p.shares)), 256, lds, s>>>(p);
     return 0;

@@ -1,6 +1,8 @@
 // elem.h — the three storage types of the operators that are templates over them (serving.h), 16 bytes of each at a time.
 #pragma once
+#include <atomic>
 #include "device_utils.h"
+#include "../common.h"
 
 namespace nvr { namespace kx {
 
@@ -47,6 +49,21 @@ __device__ __forceinline__ typename E::V zero16() {
 #pragma unroll
     for (int e = 0; e < E::W; ++e) v[e] = (typename E::T)0.f;
     return v;
+}
+
+// Large dynamic LDS has to be allowed for a kernel on each device that runs it.  have: the devices that did (one a kernel); what failed is asked for again by the next call.  (May be captured: nothing is enqueued)
+inline int allow_lds(const char *me, const void *kernel, size_t bytes, std::atomic<uint64_t> &have) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e == hipSuccess && (have.load(std::memory_order_acquire) & bit)) return 0;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        return nvr::fail(NVR_ERR_HIP, "%s: LDS of %zu bytes: %s", me, bytes, hipGetErrorString(e));
+    }
+    have.fetch_or(bit, std::memory_order_release);
+    return 0;
 }
 
 #define NVR_BY_DTYPE(dt, ...)                                           \

@@ -285,9 +285,8 @@ int kv_evict(int dt, const EvictArgs &a, hipStream_t s) {
     const int64_t most = std::min<int64_t>(a.budget, longest);
     const bool move = longest <= kHeld && most <= kHere * (kPick / (p.row_bytes / 16));
     const auto kernel = move ? &kv_evict_select_kernel<true> : &kv_evict_select_kernel<false>;
-    auto opt_in = [](const void *k) { return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4); };
-    static const hipError_t opted[2] = {opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<false>)), opt_in(reinterpret_cast<const void *>(&kv_evict_select_kernel<true>))};
-    if (opted[move] != hipSuccess) return nvr::fail(NVR_ERR_HIP, "%s: LDS of %d bytes: %s", me, kHeld * 4, hipGetErrorString(opted[move]));
+    static std::atomic<uint64_t> allowed[2];
+    if (const int rc = allow_lds(me, reinterpret_cast<const void *>(kernel), kHeld * 4, allowed[move])) return rc;
     kernel<<<dim3(G, B), kPick, (size_t)p.held * 4, s>>>(p);
     if (move) {
         NVR_KX_LAUNCHED("kv_evict");

@@ -1059,3 +1059,49 @@ def test_scored_attention_where_no_sequence_can_have_keys(arena):
         old, new = arena.space(G * block * 4, 0), arena.space(G * block * 4)
         nvr.check(L.nvr_paged_attn_decode_scored(q.ptr, H * D, kv.ptr, kv.ptr, byref(m), H, G, D, block, 1, 0.125, old.ptr, None, 0.5, new.ptr, out.ptr, None, None))
         assert (out.to_numpy((B * H * D * w,), np.uint8) == 0).all() and (new.to_numpy((G * block * 4,), np.uint8) == SENTINEL).all()
+
+
+FIRST = """
+import sys
+sys.path[:0] = [%r, %r]
+import ctypes as C
+import numpy as np
+from serving_util import Arena, byref
+import test_serving_gpu as t
+nvr, L = t.nvr, t.L
+nvr.check(L.nvr_device_set(0))
+arena, stream, graph = Arena(), C.c_void_p(), C.c_void_p()
+nvr.check(L.nvr_stream_create(byref(stream)))
+st = t.Step(arena, %r, stream, bound=%d)
+st.feed(st.lengths)
+nvr.synchronize()
+nvr.check(L.nvr_graph_capture_begin(stream))
+st.launch()
+nvr.check(L.nvr_graph_capture_end(stream, byref(graph)))
+answers = []
+for turn in range(3):
+    st.restore()
+    nvr.check(L.nvr_graph_launch(graph, stream))
+    nvr.check(L.nvr_stream_synchronize(stream))
+    answers.append(st.answers())
+    st.restore()
+    st.launch()
+    nvr.check(L.nvr_stream_synchronize(stream))
+    answers.append(st.answers())
+for a in answers:
+    for name in a:
+        assert np.array_equal(a[name], answers[-1][name]), name
+nvr.check(L.nvr_graph_destroy(graph))
+print("captured first: ok")
+"""
+
+
+@pytest.mark.parametrize("dtype,bound", [("float16", 128), ("bfloat16", 2000), ("float32", 128), ("float32", 2000)])
+def test_a_first_call_may_be_captured(dtype, bound):
+    """A process whose very first calls of these operators are captured: nothing is left to an eager call before."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST % (os.path.dirname(here), here, dtype, bound)], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=100)
+    assert r.returncode == 0 and "captured first: ok" in r.stdout, r.stderr[-3000:]
