@@ -1105,3 +1105,129 @@ def test_a_first_call_may_be_captured(dtype, bound):
     here = os.path.dirname(os.path.abspath(__file__))
     r = subprocess.run([sys.executable, "-c", FIRST % (os.path.dirname(here), here, dtype, bound)], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=100)
     assert r.returncode == 0 and "captured first: ok" in r.stdout, r.stderr[-3000:]
+
+
+# ------------------------------------------------------------------------------------------------------------ the largest sizes that are accepted
+def test_rope_of_as_many_tokens_as_are_accepted(arena):
+    rng = np.random.default_rng(20)
+    typed("float16")
+    T = 1 << 23
+    bits = rng.integers(0, 0x7000, (T, 3, 2), dtype=np.uint16)     # q, k and v of one head of 2
+    positions = rng.integers(0, 1 << 40, T)
+    turns = np.array([0.1591549430918953])
+    slots = (np.arange(T)[::-1] + 3).astype(np.int32)
+    d, out, cache = arena.dev(bits), arena.space(T * 4), [arena.space((T + 3) * 4) for _ in range(2)]
+    nvr.check(L.nvr_rope_rotate_store_kv(d.ptr, 6, d.ptr + 4, 6, d.ptr + 8, 6, arena.dev(positions).ptr, arena.dev(slots).ptr, T, 1, 1, 2, 2, 0, arena.dev(turns).ptr, 1.0, out.ptr, 2, None, 0,
+                                         cache[0].ptr, cache[1].ptr, T + 3, None))
+    x = bits[:, :2].view(np.float16).astype(np.float64)
+    want = rope(x, positions, turns, 1.0, False)
+    tol = 4 * F32 * 2 * np.abs(x).max(-1, keepdims=True) + HALF_STEP["float16"] * np.abs(want) * (1 + 2 ** -10) + SMALLEST["float16"]
+    fits = np.abs(want) < 65000                                    # (float16 ends at 65504)
+    k = cache[0].to_numpy((T + 3, 2), np.float16)[3:][::-1].astype(np.float64)
+    for i, got in enumerate((out.to_numpy((T, 2), np.float16).astype(np.float64), k)):
+        ok = np.abs(got - want[:, i]) <= tol[:, i]
+        assert (ok | ~fits[:, i]).all()
+    v = cache[1].to_numpy((T + 3, 2), np.uint16)
+    assert np.array_equal(v[3:][::-1], bits[:, 2]) and (v[:3] == 0x7B7B).all()
+
+
+@pytest.mark.parametrize("dtype,T,K,N,R,n", [("bfloat16", 3, 1 << 22, 40, 4, 2), ("float32", 70, 1 << 20, 8, 3, 2), ("float16", 3, 40, 1 << 22, 4, 2), ("bfloat16", 2, 256, 1 << 22, 16, 1), ("float16", 1 << 19, 8, 16, 4, 5),
+                                             ("float16", 1 << 19, 8, 8, 130, 1)])
+def test_lora_of_the_largest_sizes(arena, dtype, T, K, N, R, n):
+    lora_case(arena, dtype, T, K, N, R, n, np.arange(T) % (n + 1) - 1)
+
+
+def test_sample_of_as_many_logits_as_are_accepted(arena):
+    """2^22 logits: 256 chunks of a row, indices of 22 bits; prefixes that end among equal logits far out, and in the lists and the row."""
+    rng = np.random.default_rng(21)
+    V = 1 << 22
+    x = np.stack([rng.standard_normal(V) * 2, np.full(V, 1.7), (rng.integers(0, 40, V) * 0.05)]).astype(np.float32)
+    x[0, rng.integers(0, V, 30)] += 9
+    for k, p, m, u in ((0, 1.0, 0.0, 1 - 2.0 ** -24), (0, 0.75, 0.0, 0.99), (3000001, 1.0, 0.0, 0.9999), (50, 0.9, 0.0, 0.5), (1500, 1.0, 0.0, 0.8), (0, 1.0, 1.0, 0.999), (0, 0.999, 0.3, 0.7)):
+        check_sample(arena, x, [0.9, 0.7, 1.1], k, p, m, np.full(3, u, np.float32))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_scored_attention_of_as_many_keys_as_are_accepted(arena, dtype):
+    """A context of 2^23 keys of which a few pages are in the pool, the first and the last among them."""
+    rng = np.random.default_rng(22)
+    typed(dtype)
+    H, G, D, block, n = 4, 2, 64, 256, 1 << 23
+    w = np.dtype(kind(dtype)).itemsize
+    blocks = 9
+    table = np.full((1, n // block), -1, np.int32)
+    at = np.array([0, 1, 777, 16383, 16384, 20000, n // block - 2, n // block - 1])
+    table[0, at] = rng.permutation(blocks)[:len(at)]
+    q, qb = encode(rng.standard_normal((1, H * D)), dtype)
+    k, kb = encode(rng.standard_normal((blocks, block, G, D)), dtype)
+    v, vb = encode(rng.standard_normal((blocks, block, G, D)), dtype)
+    scores = rng.random((blocks, G, block)).astype(np.float32)
+    m = meta(arena, [n], table)
+    out, ws = arena.space(H * D * w), arena.space(L.nvr_paged_attn_scored_workspace_bytes(1, H, G, D, n), 0xFF)
+    ds = arena.dev(scores)
+    nvr.check(L.nvr_paged_attn_decode_scored(arena.dev(qb).ptr, H * D, arena.dev(kb).ptr, arena.dev(vb).ptr, byref(m), H, G, D, block, blocks, 0.125, ds.ptr, None, 0.5, ds.ptr, out.ptr, ws.ptr, None))
+    page = np.repeat(table[0, at], block)
+    row, j = np.tile(np.arange(block), len(at)), np.repeat(at * block, block) + np.tile(np.arange(block), len(at))
+    kk, vv = k[page, row], v[page, row]
+    want, weights = attend(q.reshape(H, D), kk, vv, 0.125)
+    size = max(float((np.abs(kk[:, h // 2]) @ np.abs(q.reshape(H, D)[h])).max()) for h in range(H)) * 0.125
+    dw = 2 * (D + 4) * F32 * size + (len(j) / 4 + 64) * F32        # (as in scored_case: absent keys add exact zeros)
+    two = {"float16": 2.0 ** -21, "float32": 0.0}[dtype]
+    got = decode(out.to_numpy((H, D), kind(dtype)), dtype)
+    tol = (2 * dw + two) * np.abs(vv).max()
+    within(got, want, tol + HALF_STEP[dtype] * (np.abs(want) + tol) + SMALLEST[dtype], "out")
+    new = ds.to_numpy(scores.shape, np.float32)
+    for g in range(G):
+        old = np.where(j < n - 1, 0.5 * scores[page, g, row].astype(np.float64), 0.0)
+        within(new[page, g, row].astype(np.float64), old + weights[:, g], 2 * dw * weights[:, g] + 4 * F32 * (old + weights[:, g]) + 1e-37, "scores")
+    free = [b for b in range(blocks) if b not in table[0, at]]
+    assert np.array_equal(new[free].view(np.uint32), scores[free].view(np.uint32))
+
+
+@pytest.mark.parametrize("budget,out_of_place", [(1000, False), ((1 << 24) + 3, False), ((1 << 24) + 3, True)])
+def test_evict_of_as_many_keys_as_are_accepted(arena, budget, out_of_place):
+    """A context of 2^25 keys, each row holding its key's number."""
+    rng = np.random.default_rng(23)
+    typed("float16")
+    n, block, first, last = 1 << 25, 256, 5, 700
+    blocks = n // block
+    more = -(-budget // block) if out_of_place else 0
+    table = rng.permutation(blocks).astype(np.int32)[None]
+    to = (blocks + rng.permutation(more)).astype(np.int32)[None] if out_of_place else table
+    rows = np.zeros(((blocks + more) * block, 4), np.uint32)       # 16 bytes a key
+    where = (table[0].astype(np.int64)[:, None] * block + np.arange(block)).ravel()
+    rows[where, 0] = np.arange(n)
+    rows[where, 3] = np.arange(n)[::-1]
+    scores = np.zeros((blocks + more) * block, np.float32)
+    s = rng.integers(0, 1 << 20, n).astype(np.float32)
+    scores[where] = s
+    dk, ds = arena.dev(rows), arena.dev(scores)
+    dv = arena.dev(rows[:, ::-1])
+    new, kept, m = arena.space(4), arena.space(budget * 4), meta(arena, [n], table)
+    nvr.check(L.nvr_kv_evict(dk.ptr, dv.ptr, ds.ptr, byref(m), 1, 8, block, blocks + more, budget, first, last, arena.dev(to).ptr if out_of_place else None, more, new.ptr, kept.ptr, None, None))
+    best = np.argsort(-s[first:n - last], kind="stable")[:budget - first - last] + first
+    want = np.sort(np.concatenate([np.arange(first), best, np.arange(n - last, n)]))
+    assert new.to_numpy((1,), np.int32)[0] == budget and np.array_equal(kept.to_numpy((budget,), np.int32), want)
+    at = (to[0].astype(np.int64)[:, None] * block + np.arange(block)).ravel()[:budget]
+    got = dk.to_numpy(rows.shape, np.uint32)
+    assert np.array_equal(got[at, 0], want) and np.array_equal(got[at, 3], n - 1 - want)
+    assert np.array_equal(dv.to_numpy(rows.shape, np.uint32)[at, 3], want) and np.array_equal(ds.to_numpy(scores.shape, np.float32)[at], s[want])
+
+
+def test_as_many_sequences_as_are_accepted(arena):
+    rng = np.random.default_rng(24)
+    B = 65535
+    lengths = np.zeros(B, int)
+    some = rng.choice(B, 300, replace=False)
+    lengths[some] = rng.integers(1, 60, 300)
+    lengths[[0, B - 1]] = [33, 17]
+    scored_case(arena, "float16", lengths.tolist(), 2, 1, 64, 16)
+    lengths[some[:3]] = [700, 515, 130]
+    scored_case(arena, "bfloat16", lengths.tolist(), 2, 1, 64, 16, max_context=701)
+    for out_of_place in (False, True):
+        evict_case(arena, "float16", lengths.tolist(), 1, 8, 16, 20, 2, 5, out_of_place)
+    x = rng.standard_normal((B, 5)).astype(np.float32)
+    u = rng.random(B).astype(np.float32)
+    ids, lp = sample_rows(arena, x, None, None, np.full(B, 0.8), None, u)
+    for r in rng.choice(B, 400, replace=False).tolist() + [0, B - 1]:
+        assert ids[r] == sample(x[r], 1.0, 0, float(np.float32(0.8)), 0.0, float(u[r]))[0]
