@@ -33,6 +33,9 @@ namespace {
 constexpr int kBins = 1024, kPick = 1024, kList = 2048, kRadix = 2048, kNear = 1536;
 constexpr double kPerUnit = 24.;                                          // bins to a unit of x / T
 constexpr int kOne = 40;                                                  // weights inside a cell are integers of 2^-40
+// Sums of those are off by up to 5e-13 of themselves, and a goal by as much, so a goal that a sum ought to equal (half of two equal logits) may lie on either side of it: top-p's goals are taken a little lower (a
+// sum as large as the goal has reached it), the drawn number's a little higher (it has to be passed)
+constexpr double kReached = 1. - 4e-12, kPassed = 1. + 4e-12;
 
 // arg: first index of the maximum (greedy rows); cut: the list has every token of bins up to it (-1: there is no list); near: its length; binned: how many bins are in memory, the others are empty (0: the list
 // has all that counts); total: the weights of the bins, the chunk's maximum 1
@@ -636,7 +639,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         const unsigned int cum_n = scan<unsigned int>(cnt[tid], sh.wcnt);
         int reach = kBins;
         if (ask.k) reach = first_of(cum_n >= k);
-        else if (ask.p < 1.f) reach = first_of(cum >= (double)ask.p * everything && cum_n > 0);
+        else if (ask.p < 1.f) reach = first_of(cum >= (double)ask.p * everything * kReached && cum_n > 0);
         if (ask.min_p > 0.f && (!ask.k || ask.p == 1.f)) reach = min(reach, p_last);      // (what top-k keeps in all is wanted for top-p)
         if (reach > r.listed && ask.k && r.listed == kBins - 2) reach = r.listed;         // (fewer tokens than top-k would keep)
         if (tid == min(reach, kBins - 1)) sh.nsel = cum_n;
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                     __syncthreads();
                     total = (double)(sh.wsum64[0] + sh.wsum64[1] + sh.wsum64[2] + sh.wsum64[3]);
                 }
-                keep = keep && (rank == 1 || (double)(upto - q) < (double)ask.p * total);
+                keep = keep && (rank == 1 || (double)(upto - q) < (double)ask.p * total * kReached);
             }
             keep = keep && !(ask.min_p > 0.f && x < (double)ask.min_p);
             if (!keep) q = 0;
@@ -741,7 +744,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         double total = ask.k ? same(sh.cum[kBins - 1]) : everything;
         for (int filter = 0; filter < 2; ++filter) {                      // top-k, top-p
             if (filter == 0 ? !ask.k : ask.p == 1.f) continue;
-            const double goal = filter ? (double)ask.p * total : 0.;
+            const double goal = filter ? (double)ask.p * total * kReached : 0.;
             const int b = first_of(filter ? sh.cum[tid] >= goal && sh.cum[tid] > 0. && tid < stop : sh.cum_n[tid] >= k);
             const int bin = filter && b == kBins ? stop : b;              // (the bin that top-k ended in, or none)
             if (bin == kBins || (filter && b == kBins && key == 0 && index == 0xffffffffu)) continue;
@@ -865,7 +868,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     if (tid == kPick - 1) sh.part = upto_c;
     if (tid == 0) sh.sel = 0;
     __syncthreads();
-    const double sum = same(sh.part), goal = u * sum;
+    const double sum = same(sh.part), goal = u * sum * kPassed;
     int c = first_of(own > 0. && upto_c > goal);
     if (c == kBins) {
         if (own > 0.) atomicMax(&sh.sel, tid);

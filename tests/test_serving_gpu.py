@@ -1231,3 +1231,18 @@ def test_as_many_sequences_as_are_accepted(arena):
     ids, lp = sample_rows(arena, x, None, None, np.full(B, 0.8), None, u)
     for r in rng.choice(B, 400, replace=False).tolist() + [0, B - 1]:
         assert ids[r] == sample(x[r], 1.0, 0, float(np.float32(0.8)), 0.0, float(u[r]))[0]
+
+
+@pytest.mark.parametrize("V", [2, 20, 300, 2050, 20000, 151936, 400000])
+def test_sample_goals_that_equal_a_sum(arena, V):
+    """Equal logits away from a cell's middle, and halves, quarters and eighths of their number: a nucleus ends with the token that brings the sum to exactly top_p, a token is drawn only where the sum is more than
+    the uniform number's."""
+    rng = np.random.default_rng(V)
+    some = rng.choice(V, min(V, 16), replace=False)
+    few = np.full(V, -3.0)
+    few[some] = 5.1                                                # up to 16 equal ones above others that T leaves next to nothing
+    x = np.stack([np.full(V, 2.3), np.full(V, 1000.1), few, few - 22.8])
+    for T in ((0.7, 1.3, 0.01, 0.003), (100.0, 0.05, 0.02, 0.01)):
+        for k, p, m in ((0, 1.0, 0.0), (0, 0.5, 0.0), (0, 0.25, 0.0), (0, 0.75, 0.5), (min(V, 16), 0.5, 0.0), (8, 1.0, 0.0), (V // 2, 0.5, 1.0), (0, 1.0, 0.9)):
+            for u in (0.5, 0.25, 0.875, 2.0 ** -24, 1 - 2.0 ** -24):
+                check_sample(arena, x, T, k, p, m, u)
