@@ -709,7 +709,8 @@ NVR_API int nvr_lora_add(const nvr_half *x, int64_t ldx, const nvr_half *A, cons
 /* A token for each row of logits [B, V] (rows ld numbers apart) from the row's uniform[i] in [0, 1): the filters apply one behind the other to the weights w = exp((x - max) / temperature[i]),
  * in descending order (ties: ascending index): top_k[i] > 0 keeps the first top_k[i]; 0 <= top_p[i] < 1 keeps the prefix up to the first that brings its sum to top_p[i] of what is left; min_p[i] > 0
  * keeps weights of min_p[i] (at most 1) and more.  The token is the first in index order whose summed weight exceeds uniform[i] times the sum of all kept.  temperature 0 (or less): the largest logit, lowest
- * index on ties.  NaN counts as -inf; tokens of weight below e^-42 may be left out; a row of nothing but -inf answers -1.  Any of temperature (1), top_k, top_p, min_p may be null.
+ * index on ties.  NaN counts as -inf; tokens of weight below e^-42 may be left out; a row of nothing but -inf answers -1.  Sums of weights are right to 1e-12 of
+ * themselves; a sum that equals its goal has reached top_p, and is not more than the uniform number's.  Any of temperature (1), top_k, top_p, min_p may be null.
  * out_logprobs (nullable): ln of the token's share of the kept weights (greedy: 0; no token: -inf).  workspace: nvr_sample_uniform_workspace_bytes.  V up to 2^22. */
 NVR_API size_t nvr_sample_uniform_workspace_bytes(int64_t B, int64_t V);
 NVR_API int nvr_sample_uniform(const float *logits, int64_t ld, int64_t B, int64_t V, const float *temperature, const int64_t *top_k, const float *top_p, const float *min_p,

@@ -33,9 +33,10 @@ namespace {
 constexpr int kBins = 1024, kPick = 1024, kList = 2048, kRadix = 2048, kNear = 1536;
 constexpr double kPerUnit = 24.;                                          // bins to a unit of x / T
 constexpr int kOne = 40;                                                  // weights inside a cell are integers of 2^-40
-// Sums of those are off by up to 5e-13 of themselves, and a goal by as much, so a goal that a sum ought to equal (half of two equal logits) may lie on either side of it: top-p's goals are taken a little lower (a
-// sum as large as the goal has reached it), the drawn number's a little higher (it has to be passed)
-constexpr double kReached = 1. - 4e-12, kPassed = 1. + 4e-12;
+// A token's weight is formed alike in a goal and in the sums that are held against it (by the cell's weight, or by weight()), so that what is off in it (5e-13 by the steps, 2e-13 by the series) is off in both.
+// Left are the roundings of sums of doubles: a goal that a sum ought to equal (half of two equal logits) may still lie on either side of it, so top-p's goals are taken a little lower (a sum as large as the goal
+// has reached it), the drawn number's a little higher (it has to be passed)
+constexpr double kReached = 1. - 2e-14, kPassed = 1. + 2e-14;
 
 // arg: first index of the maximum (greedy rows); cut: the list has every token of bins up to it (-1: there is no list); near: its length; binned: how many bins are in memory, the others are empty (0: the list
 // has all that counts); total: the weights of the bins, the chunk's maximum 1
@@ -662,7 +663,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             const unsigned long long mine_v = tid < n ? t[tid].x : 0;
             const unsigned int id = (unsigned int)mine_v;
             const double x = tid < n ? weight(of_key(~(unsigned int)(mine_v >> 32)), r.m, ask.c) : 0.;
-            unsigned long long q = tid < n ? max(1ull, (unsigned long long)(x * 0x1p52 + 0.5)) : 0, upto = 0, all = 0;
+            auto whole = [&](double w) { return tid < n ? max(1ull, (unsigned long long)(w * 0x1p52 + 0.5)) : 0; };
+            unsigned long long q = whole(x), upto = 0, all = 0;
+            const unsigned long long drawn = q;
+            if (ask.p < 1.f && !ask.k) {                                  // (held against the sum of the bins: as they have it)
+                const float v = of_key(~(unsigned int)(mine_v >> 32));
+                q = whole((double)r.inside(v) * r.cell(bin_of(v, r.m, ask.inv)));
+            }
             if (tid < n) t[tid].y = q;
             __syncthreads();
             int rank = 0;
@@ -681,7 +688,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
                 keep = keep && (rank == 1 || (double)(upto - q) < (double)ask.p * total * kReached);
             }
             keep = keep && !(ask.min_p > 0.f && x < (double)ask.min_p);
-            if (!keep) q = 0;
+            q = keep ? drawn : 0;
             __syncthreads();
             if (tid < n) t[tid].y = q;
             __syncthreads();
@@ -765,7 +772,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     const bool cut = filtered && last >= sure;                            // (without filters all bins are whole)
     // enough(): whether weight() of the token is min_p and more
     auto kept = [&](int b, unsigned int kk, unsigned int i, auto enough) {
-        if (!filtered || b < sure) return true;
+        if (b < sure) return true;
         if (b > last) return false;
         if (by_key && b == key_bin && (kk < key || (kk == key && i > index))) return false;
         return !(ask.min_p > 0.f) || enough();
@@ -821,23 +828,24 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
             }
         return;
     }
-    // ---- what each chunk keeps: its whole bins, and its single tokens in steps of 2^-40 of the heaviest there may be
+    // ---- what each chunk keeps: its whole bins, and its single tokens in steps of 2^-48 of the heaviest there may be (16384 of 1.02 at most)
     __syncthreads();
-    double *sums = sh.cum;                                                // (of up to kChunks)
+    double *units = sh.cum, *sums = reinterpret_cast<double *>(sh.rmass + kChunks);      // weight of a unit of each bin (the sums of bins have been looked at); of up to kChunks
     unsigned long long *single = reinterpret_cast<unsigned long long *>(sh.rmass);
-    const double unit = cut ? r.cell(sure) : 0.;
+    static_assert(kRadix >= 2 * kChunks, "");
+    const double unit = cut ? r.cell(sure) * 0x1p-8 : 0., steps = cut ? 1. / unit : 0.;
     single[tid] = 0;
+    units[tid] = unit_of_bin;
     const bool here = cut && r.gather(sure, last);
     __syncthreads();
+    // A token's weight is the cell's times the place's inside (half the work of an exponential).  It and weight() are within 1e-7 of each other (5e-13 of the steps inside a cell, and 2^-53 of 24 x / T, which is
+    // below 2^34 where tokens of different logits are near).  Where min_p is as close, weight() decides: it is exactly 1 for the largest logit, and the product may be below
+    auto close = [&](double w) { return fabs(w - (double)ask.min_p) <= 1e-6 * w; };
     if (cut)
         r.each_gathered(here, sure, last, [&](unsigned int kk, unsigned int i, float v, int b) {
-            const double w = weight(v, r.m, ask.c);
-            if (kept(b, kk, i, [&] { return w >= (double)ask.min_p; })) atomicAdd(&single[i / p.chunk], (unsigned long long)(w / unit + 0.5));
+            const double w = (double)r.inside(v) * units[b];
+            if (kept(b, kk, i, [&] { return (close(w) ? weight(v, r.m, ask.c) : w) >= (double)ask.min_p; })) atomicAdd(&single[i / p.chunk], (unsigned long long)(w * steps + 0.5));
         });
-    __syncthreads();
-    double *units = reinterpret_cast<double *>(sh.key);                   // (kList of 4 bytes: the gathered tokens have been looked at)
-    static_assert(kList * 4 >= kBins * 8, "");
-    units[tid] = unit_of_bin;
     __syncthreads();
     for (int c = wave; c < p.P; c += kPick / 64) {
         const int s = sh.shift[c];
@@ -883,17 +891,18 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     const int per = p.chunk / kPick, base = c * p.chunk + tid * per, end = min(p.V, c * p.chunk + p.chunk);      // 4 or 16
     const bool lone = lonely(r.m, ask.inv);
     const double t_m = (double)r.m * ask.inv, whole_m = t_m + kWhole;
-    auto of = [&](float v, int i, auto enough) {                          // the weight as the cell's times the place's inside: half the work of an exponential
+    // the weight, as the chunk's sum has it
+    auto of = [&](float v, int i, auto enough) {
         if (v == -INFINITY || (lone && v != r.m)) return 0.;
         const double at = fmax((double)v * ask.inv, t_m - 2. * kBins), whole = at + kWhole;
         const int b = lone ? 0 : low_of(whole_m) - low_of(whole);
-        if (b >= kBins - 1 || (filtered && b >= sure && b > last)) return 0.;
+        if (b >= kBins - 1 || (b >= sure && b > last)) return 0.;
         const double w = lone ? 1. : (above_2_52(at - (whole - kWhole)) - 4503599627370496.0) * units[b];
         return kept(b, key_of(v), (unsigned int)i, [&] { return enough(w, v); }) ? w : 0.;
     };
-    // That weight and weight() are within 1e-7 of each other (5e-13 of the steps inside a cell, and 2^-53 of 24 x / T, which is below 2^34 where tokens of different logits are near).  Where min_p is as close,
-    // weight() decides, as it did for the sums (it is exactly 1 for the largest logit, and the other may be below); once behind the loop: in it, 256 rows of 151936 with min-p 0.001 took 189 us in place of 186
-    auto exactly = [&](double, float v) { return weight(v, r.m, ask.c) >= (double)ask.min_p; };
+    auto unfiltered = [&](float v) { const double w = weight(v, r.m, ask.c); return v == -INFINITY || w < 0x1p-61 ? 0. : w; };      // (2^-61 is e^-42.3)
+    // (near min_p alone, and once, behind the loop: weight() for every token in it took 189 us for 256 rows of 151936 with min-p 0.001, this 186)
+    auto exactly = [&](double w, float v) { return (close(w) ? weight(v, r.m, ask.c) : w) >= (double)ask.min_p; };
     float4_t f[4];
     double here_sum = 0.;
     unsigned int doubt = 0;
@@ -902,12 +911,16 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 #pragma unroll 1
     for (int j = 0; 4 * j < per; ++j) {                                   // (not unrolled: code that runs once costs its way from memory)
         const float4_t g = j & 2 ? j & 1 ? f[3] : f[2] : j & 1 ? f[1] : f[0];
+        if (!filtered) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) here_sum += unfiltered(g[e]);
+            continue;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             here_sum += of(g[e], base + 4 * j + e, [&](double w, float) {
-                const bool near = fabs(w - (double)ask.min_p) <= 1e-6 * w;
-                doubt |= (near ? 1u : 0u) << (4 * j + e);
-                return !near && w >= (double)ask.min_p;
+                doubt |= (close(w) ? 1u : 0u) << (4 * j + e);
+                return !close(w) && w >= (double)ask.min_p;
             });
     }
     while (doubt) {
@@ -924,13 +937,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
     }
     float *values = reinterpret_cast<float *>(sh.idx);                    // of thread t: the first wave looks at them, a lane a token
     if (tid == t) {
-        sh.cum[0] = sh.part + (upto - here_sum);
+        sums[0] = sh.part + (upto - here_sum);
 #pragma unroll
         for (int j = 0; j < 4; ++j) *reinterpret_cast<float4_t *>(values + 4 * j) = f[j];
     }
     __syncthreads();
     if (wave == 0 && t >= 0) {
-        const double w = lane < per ? of(values[lane & 15], c * p.chunk + t * per + lane, exactly) : 0., run = sh.cum[0] + wave_scan(w);
+        const double w = lane >= per ? 0. : filtered ? of(values[lane & 15], c * p.chunk + t * per + lane, exactly) : unfiltered(values[lane & 15]), run = sums[0] + wave_scan(w);
         const unsigned long long any = __ballot(w > 0.), hit = __ballot(w > 0. && run > goal);
         const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)any);      // (sums in another order may end a rounding below the goal: the last one)
         if (lane == 0) sh.found = c * p.chunk + t * per + l;

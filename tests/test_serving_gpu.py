@@ -1246,3 +1246,15 @@ def test_sample_goals_that_equal_a_sum(arena, V):
         for k, p, m in ((0, 1.0, 0.0), (0, 0.5, 0.0), (0, 0.25, 0.0), (0, 0.75, 0.5), (min(V, 16), 0.5, 0.0), (8, 1.0, 0.0), (V // 2, 0.5, 1.0), (0, 1.0, 0.9)):
             for u in (0.5, 0.25, 0.875, 2.0 ** -24, 1 - 2.0 ** -24):
                 check_sample(arena, x, T, k, p, m, u)
+
+
+@pytest.mark.parametrize("V", [200, 2000, 20000, 151936])
+def test_sample_goals_a_hair_from_a_sum(arena, V):
+    """Two halves whose weights differ by 2.4e-13 of themselves, so that the middle of the sum lies 1.2e-13 behind the first half's end, or in front of it; by 4e-12 where filters have the weights in steps of
+    2^-40 (of a weight of 1, 9e-13)."""
+    a, b = np.float32(2.3), np.nextafter(np.float32(2.3), np.float32(3))
+    assert 2e-7 < float(b) - float(a) < 3e-7
+    x = np.stack([np.where(np.arange(V) < V // 2, a, b), np.where(np.arange(V) < V // 2, b, a)])
+    for T, k, p, m in ((1e6, 0, 1.0, 0.0), (6e4, 0, 1 - 2.0 ** -24, 0.0), (6e4, 0, 1.0, 0.5), (6e4, V + 1, 1 - 2.0 ** -24, 0.9)):
+        ids, _ = sample_rows(arena, x, np.full(2, T), np.full(2, k), np.full(2, p), np.full(2, m), np.full(2, 0.5))
+        assert ids.tolist() == [V // 2, V // 2 - 1], (T, k, p, m)
