@@ -730,6 +730,9 @@ NVR_API int nvr_paged_attn_decode_scored(const nvr_half *q, int64_t ldq, const n
  * sequences' own (prompt blocks that other sequences share are left alone that way; shorter sequences are copied as they are).  In place, a block is one sequence's alone.
  * new_lens [B] (not meta's context_lens) gets the lengths; kept [B, KVH, budget] (nullable) the kept keys' former places, -1 behind the last.  Blocks behind the new length are the caller's to free.
  * A sequence whose tables name a block outside 0 .. num_blocks - 1 for one of its keys, or whose to_tables row has too few blocks, stays as it is: new_lens -1, kept all -1.
+ * In place, a call moves every row behind the first that goes: one key over the budget costs half as much as four times the budget (32 sequences of 2049 keys to 2048, 8 heads of 128 in 16 bits: 80 us, of
+ * 8000 keys: 150), so let sequences grow by a block or more between calls.  A block whose content is known to others, now or later (the block manager of this library keeps the prefix hash of a full block
+ * while its sequence lives, and hands it to a later prompt with that prefix), must not be evicted in place.
  * keep_first + keep_last <= budget; rows of a multiple of 16 bytes; max_context_len or max_blocks * block_size up to 2^25 keys.  workspace: nvr_kv_evict_workspace_bytes (null allowed where kept is given). */
 NVR_API size_t nvr_kv_evict_workspace_bytes(int64_t B, int64_t KVH, int64_t budget, int64_t max_context_len);
 NVR_API int nvr_kv_evict(nvr_half *k_cache, nvr_half *v_cache, float *scores, const nvr_attn_meta *meta, int64_t KVH, int64_t D, int64_t block_size, int64_t num_blocks,

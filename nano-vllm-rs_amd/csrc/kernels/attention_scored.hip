@@ -10,7 +10,7 @@
 // columns: S^T = K Q^T, O^T += V^T P^T.  Rows come from the pages whole (16 bytes a lane, the next tile's in flight) and pass through the wave's own LDS image into the layout of the operands.  Weights
 // enter the second product as two 16-bit numbers, the rounded weight and the rounded rest, so that they have 17 (bfloat16) or 22 bits there: the cores are idle most of the time anyway.
 // 48 sequences of 512 .. 8100 keys, 32 heads over 8 of 128, bfloat16: 119 us (107 and 12) for 556 MB, 4.7 TB/s; 32 x 8192 keys of 4 heads a kv head: 220 us, 4.95 TB/s, where the decode attention
-// without scores takes 212; one sequence of 2047 keys: 10 us (6 and 4), two launches and their chains of round trips.
+// without scores takes 212; one sequence of 2047 keys: 10 us (6 and 4), two launches and their chains of round trips.  float32: the 48 sequences 209 us (196 and 13, 1.1 GB), the one 14.
 #include <algorithm>
 #include "serving.h"
 #include "elem.h"
@@ -63,7 +63,8 @@ __device__ __forceinline__ typename E::V transposed(const char *a, const char *b
 }  // namespace
 
 // WHOLE: contexts are short, and a workgroup has a sequence's keys of a kv head and answers by itself, scores in LDS: no second launch, no workspace.  us where it answers and with two launches: 5 sequences
-// of up to 60 keys 5.2 10.7, 32 of 20 .. 250 9.1 11.9, 32 of 200 .. 500 16.8 19.9, 64 of 100 .. 500 (4 heads a kv head) 19.7 26.9; 8 of 200 .. 500 14.2 11.6, 32 of 100 .. 1000 24.6 20.0
+// of up to 60 keys 5.2 10.7, 32 of 20 .. 250 9.1 11.9, 32 of 200 .. 500 16.8 19.9, 64 of 100 .. 500 (4 heads a kv head) 19.7 26.9; 8 of 200 .. 500 14.2 11.6, 32 of 100 .. 1000 24.6 20.0.  (F32 of 128: 3
+// registers are spilled)
 template <class E, int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_scored_kernel(ScoredParams p) {
     typedef typename E::T T; typedef typename E::V V;

@@ -5,6 +5,8 @@
 // Into other blocks, every row is on its own: a copy, bound by memory.  In place, row i comes from row kept[i] >= i, which is overwritten by a later row: a workgroup takes a (sequence, kv head)'s
 // strip of 128 bytes of the rows, from the front in steps of kMoves requests: all of a step are read before any is written, and no later step reads what it writes.
 // 32 sequences of 1000 .. 8100 keys of 8 heads of 128 to 2048, float16, other blocks: 111 us (15 and 94), 4.4 TB/s over both, 5.2 in the copy (a large copy: 5.1); one of 4099 keys: 15 us (11 and 4).
+// In place, scores drawn anew before each call: 32 of 8000 keys 150 us (15 and 135; 536 MB read and written), of 2304 137, of 2049 80 (9 and 72; 340 MB: one key too many moves every row behind the one that goes);
+// one of 4099 keys 28 (10 and 19: 128 workgroups, each with a chain of steps).
 // The select's life is a chain of some twenty LDS round trips and barriers; ballots in place of a thread's run of keys, and a count of a digit's few keys in place of its last two passes, took as long.
 #include <algorithm>
 #include <type_traits>
@@ -48,8 +50,8 @@ __device__ __forceinline__ unsigned int rank_of(float f) {
 }
 }  // namespace
 
-// MOVE: the rows are few, and are moved here: all are read before any is written.  us so and with a second launch, rows of 256 bytes of 8 heads: one sequence to 64 keys 7.5 8.5 (in place 7.4 9.3), to 256
-// 9.7 9.2 (9.8 11.3); 16 to 128 9.8 11.2, to 256 12.8 13.2; 32 of 500 rows of 128 bytes 18.1 19.3 (15.3 17.6)
+// MOVE: the rows are few, and are moved here: all are read before any is written.  us so and with a second launch, scores drawn anew before each call, 8 heads of 256 bytes a row, other blocks (in place): one
+// sequence of 1000 keys to 64 5.7 8.0 (5.6 8.5), to 256 7.2 8.1 (7.1 9.8); 16 to 128 8.4 10.3 (7.9 11.6), to 256 11.2 12.6 (10.6 13.7); 32 of 2000 to 500 rows of 128 bytes 17.9 19.5 (17.4 21.1)
 template <bool MOVE>
 __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
     extern __shared__ __attribute__((aligned(16))) float held[];          // scores of keys 0 .. p.held - 1
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(kPick) void kv_evict_select_kernel(EvictParams p) {
 }
 
 // 16 bytes a lane, `strip` bytes of a row; the step in front of the next one's writes is on its way
-constexpr int kMoves = 4;                                                 // requests on their way (32 x 8000 keys of 8 heads of 128 to 2048, float16: 2 109 us, 4 106, 8 129)
+constexpr int kMoves = 4;                                                 // requests on their way (8 heads of 128, float16, scores drawn anew: 32 x 8000 keys to 2048 2 147 us, 4 150, 8 178; 32 x 2049 81 80 98)
 __global__ __launch_bounds__(kPick) void kv_evict_close_kernel(EvictParams p) {
     const EvictArgs &a = p.a;
     const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;

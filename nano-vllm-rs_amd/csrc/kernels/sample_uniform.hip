@@ -14,7 +14,7 @@
 // Rows of 151936 logits (their read alone: 24 us for 256 of them, 4 for one), both launches: one row 15 us with top-k 20, 35 with 1000, 60 with top-p 0.95 that keeps some ten thousand tokens; 256 rows 45, 82
 // and 137 (77 + 60), 112 with settings mixed (54 + 58).  The first is bound by 64-bit arithmetic and, for top-p, by the LDS atomics on the bins (two copies of them where a chunk is large: 95 -> 77); the
 // second, a workgroup a row, by a chain of scans and LDS round trips, and by walks over a row where the lists end too early.
-// What a chunk cannot contribute is left out by one comparison a token: with top-k, whatever lies below the k-th of the chunk's maxima of 8 neighbours (there are k tokens above it), with min-p
+// What a chunk cannot contribute is left out by one comparison a token: with top-k, whatever lies below the k-th of the chunk's maxima of 4 neighbours (there are k tokens above it), with min-p
 // alone, whatever lies below min_p of the chunk's maximum.
 #include <algorithm>
 #include <cfloat>
@@ -958,7 +958,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
 
 // Tokens of a chunk.  Each has its bins and lists, which the second launch reads: large ones where there would be many, and for many rows that are one.  us with 4096 and 16384, settings mixed: 256 rows of
 // 151936 137 114, 40 74 66, 256 of 131072 114 101, 32 45 44, 8 38 41; 256 of 65536 73 73, 128 57 62, 256 of 32768 61 64, 198 of 20570 59 78; 135 of 9398 52 42, 256 of 5000 48 42.  One row of 151936 with
-// top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 22 (the walk over the drawn chunk); of 32000: 14 15, 36 42, 15 20, 14 21
+// top-k 20 15.9 15.1, top-k 1000 42 36, top-p 0.8 37 40, unfiltered 16 21 (the walk over the drawn chunk: the rule goes by the vocabulary there, and such rows pay for it); of 32000: 14 15, 36 42, 15 20,
+// 14 21
 // (the limits stand in sample_uniform_workspace_bytes too)
 static int sample_chunk(int64_t B, int64_t V) { return V > 98304 || (V <= 16384 && B >= 128) ? 16384 : 4096; }
 // Enough for fewer rows and smaller vocabularies too, whose chunks may be smaller and more: the most there are on either side of the rule's limits
