@@ -900,7 +900,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(SampleParams p) {
         const double w = lone ? 1. : (above_2_52(at - (whole - kWhole)) - 4503599627370496.0) * units[b];
         return kept(b, key_of(v), (unsigned int)i, [&] { return enough(w, v); }) ? w : 0.;
     };
-    auto unfiltered = [&](float v) { const double w = weight(v, r.m, ask.c); return v == -INFINITY || w < 0x1p-61 ? 0. : w; };      // (2^-61 is e^-42.3)
+    auto unfiltered = [&](float v) { return bin_of(v, r.m, ask.inv) >= kBins - 1 ? 0. : weight(v, r.m, ask.c); };      // (what is left out goes by the bins, as where a chunk is)
     // (near min_p alone, and once, behind the loop: weight() for every token in it took 189 us for 256 rows of 151936 with min-p 0.001, this 186)
     auto exactly = [&](double w, float v) { return (close(w) ? weight(v, r.m, ask.c) : w) >= (double)ask.min_p; };
     float4_t f[4];

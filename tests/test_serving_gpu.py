@@ -1258,3 +1258,16 @@ def test_sample_goals_a_hair_from_a_sum(arena, V):
     for T, k, p, m in ((1e6, 0, 1.0, 0.0), (6e4, 0, 1 - 2.0 ** -24, 0.0), (6e4, 0, 1.0, 0.5), (6e4, V + 1, 1 - 2.0 ** -24, 0.9)):
         ids, _ = sample_rows(arena, x, np.full(2, T), np.full(2, k), np.full(2, p), np.full(2, m), np.full(2, 0.5))
         assert ids.tolist() == [V // 2, V // 2 - 1], (T, k, p, m)
+
+
+@pytest.mark.parametrize("V", [8192, 114688])
+def test_sample_chunks_of_hardly_any_weight(arena, V):
+    """A first chunk whose tokens weigh about e^-42, where they may be left out, and a number of 0: the first of them, or the first behind them, never none."""
+    edge = np.arange(41.0, 44.0, 0.02)
+    x = np.zeros((len(edge), V), np.float32)
+    x[:, :V // 2] = -edge[:, None]
+    for k, p, m in ((0, 1.0, 0.0), (V - 1, 1.0, 0.0), (0, 1 - 2.0 ** -24, 0.0), (0, 1.0, 1e-30)):
+        ids, _ = sample_rows(arena, x + np.float32(2.3), None, np.full(len(edge), k), np.full(len(edge), p), np.full(len(edge), m), np.zeros(len(edge)))
+        assert np.isin(ids, [0, V // 2]).all(), (k, p, m, ids)
+        if p == 1.0:
+            assert (ids[edge < 41.9] == 0).all()                   # (above e^-42: none is left out)
